@@ -54,6 +54,8 @@ EXPORTS = [
     "llm_debug_gemm_f16", "llm_debug_read_kv", "llm_gemm_i8_splitk_noalloc", "llm_set_option", "llm_set_sampling", "llm_sample_uniform", "llm_debug_sample", "llm_debug_wait_timeout",
     "llm_eval_window", "llm_debug_exp2", "llm_shard_range", "llm_comm_unique_id", "llm_comm_create",
     "llm_comm_destroy", "llm_gather_tokens", "llm_comm_last_gather_ms", "llm_linear_create", "llm_linear_eval_cf", "llm_linear_destroy",
+    "llm_pages_work_words", "llm_pages_status", "llm_pages_copy", "llm_pages_fork", "llm_pages_free",
+    "llm_pages_compact",
 ]
 
 LLM_COMM_ID_BYTES = 128
@@ -100,6 +102,11 @@ class llm_layer_weights_f32(C.Structure):
 
 class llm_model_weights_f32(C.Structure):
     _fields_ = [("embed", _FP), ("rms_final", _FP), ("lm_head", _FP), ("layers", C.POINTER(llm_layer_weights_f32))]
+
+
+class llm_page_cache(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "n_layers", "n_pages", "n_kv_heads", "head_dim", "max_seqs", "max_pages")]
+    _fields_ += [(n, C.c_void_p) for n in ("pool", "n_free", "status", "npages", "refs", "free_pages", "table", "work")]
 
 
 _lib = None
@@ -162,6 +169,13 @@ def lib() -> C.CDLL:
         "llm_linear_create": (C.c_int, [C.c_int, C.c_int, _FP, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
         "llm_linear_eval_cf": (C.c_int, [C.c_void_p, _FP, C.c_int, _FP, C.POINTER(C.c_uint64)]),
         "llm_linear_destroy": (C.c_int, [C.c_void_p]),
+        "llm_pages_work_words": (C.c_size_t, [C.c_int, C.c_int]),
+        "llm_pages_status": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
+        "llm_pages_copy": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+        "llm_pages_fork": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                     C.c_void_p]),
+        "llm_pages_free": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+        "llm_pages_compact": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
         "llm_set_option": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
         "llm_gemm_i8_splitk_noalloc": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                  C.c_void_p, C.c_void_p]),

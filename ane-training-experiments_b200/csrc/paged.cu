@@ -1,0 +1,204 @@
+// paged.cu -- C entries of the caller-owned paged caches: argument checks and launches of the
+// page requests (pages.cuh).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/llm_cuda.h"
+#include "pages.cuh"
+
+using namespace llm;
+
+// Sets the thread's last error (defined in llm_cuda.cu) and returns `code`.
+int llm_detail_fail(int code, const char* msg);
+
+namespace {
+
+int fail_fmt(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return llm_detail_fail(code, buf);
+}
+
+#define CU(call)                                                                                       \
+  do {                                                                                                 \
+    cudaError_t e_ = (call);                                                                           \
+    if (e_ != cudaSuccess) return fail_fmt(LLM_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_)); \
+  } while (0)
+#define RC(call)                   \
+  do {                             \
+    int rc_ = (call);              \
+    if (rc_ != LLM_OK) return rc_; \
+  } while (0)
+
+// Makes `device` current for the scope of a call.
+class DeviceScope {
+ public:
+  int enter(int device) {
+    CU(cudaGetDevice(&prev_));
+    if (prev_ == device) return LLM_OK;
+    const cudaError_t e = cudaSetDevice(device);
+    if (e != cudaSuccess) return fail_fmt(LLM_ERR_CUDA, "cudaSetDevice(%d) failed: %s", device, cudaGetErrorString(e));
+    changed_ = true;
+    return LLM_OK;
+  }
+  ~DeviceScope() {
+    if (changed_) cudaSetDevice(prev_);
+  }
+
+ private:
+  int prev_ = 0;
+  bool changed_ = false;
+};
+
+// Launch that may start while the stream's preceding kernel drains (the kernel waits for it).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_geometry(const llm_page_cache* c) {
+  if (!c) return fail_fmt(LLM_ERR_INVALID, "nil cache");
+  if (c->dtype != LLM_DTYPE_F16 && c->dtype != LLM_DTYPE_BF16)
+    return fail_fmt(LLM_ERR_INVALID, "cache dtype %d (LLM_DTYPE_F16 or LLM_DTYPE_BF16)", c->dtype);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail_fmt(LLM_ERR_UNSUPPORTED, "head_dim=%d (supported: 64, 128)", c->head_dim);
+  if (c->n_layers <= 0 || c->n_pages <= 0 || c->n_kv_heads <= 0 || c->max_seqs <= 0 || c->max_pages <= 0)
+    return fail_fmt(LLM_ERR_INVALID, "cache sizes must be positive");
+  if (c->n_kv_heads > 1024 || c->n_pages > (1 << 28) || c->max_seqs > (1 << 24) || c->max_pages > (1 << 24))
+    return fail_fmt(LLM_ERR_INVALID, "cache sizes out of range");
+  if (!c->pool || !aligned(c->pool, 128)) return fail_fmt(LLM_ERR_INVALID, "the pool must be device memory aligned to 128 bytes");
+  return LLM_OK;
+}
+
+int check_tables(const llm_page_cache* c) {
+  RC(check_geometry(c));
+  for (const int32_t* p : {c->n_free, c->status, c->npages, c->refs, c->free_pages, c->table, c->work})
+    if (!p || !aligned(p, 4)) return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
+  return LLM_OK;
+}
+
+PageTables tables(const llm_page_cache* c) {
+  PageTables t{};
+  t.pool = static_cast<uint8_t*>(c->pool);
+  t.n_free = c->n_free;
+  t.status = c->status;
+  t.npages = c->npages;
+  t.refs = c->refs;
+  t.free_pages = c->free_pages;
+  t.table = c->table;
+  t.work = c->work;
+  t.n_layers = c->n_layers;
+  t.n_pages = c->n_pages;
+  t.max_seqs = c->max_seqs;
+  t.max_pages = c->max_pages;
+  t.block_bytes = c->n_kv_heads * 2 * 16 * c->head_dim * 2;
+  return t;
+}
+
+// CTAs of a launch that copies up to `moves` pages of every layer.
+int copy_grid(const PageTables& t, long long moves) {
+  const long long chunks = moves * t.n_layers * (t.block_bytes / kCopyChunk);
+  return static_cast<int>(std::max(1ll, std::min(chunks, 148ll * 8)));
+}
+
+}  // namespace
+
+extern "C" size_t llm_pages_work_words(int n_pages, int max_seqs) {
+  if (n_pages <= 0 || max_seqs <= 0 || n_pages > (1 << 28) || max_seqs > (1 << 24)) return 0;
+  return PageWork::words(max_seqs, n_pages);
+}
+
+extern "C" int llm_pages_status(int device, const llm_page_cache* c, void* stream) {
+  RC(check_tables(c));
+  DeviceScope dev;
+  RC(dev.enter(device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int h = 0;
+  CU(cudaMemcpyAsync(&h, c->status, sizeof h, cudaMemcpyDeviceToHost, s));
+  CU(cudaStreamSynchronize(s));
+  if (h == 0) return LLM_OK;
+  CU(cudaMemsetAsync(c->status, 0, sizeof h, s));
+  CU(cudaStreamSynchronize(s));
+  switch (h) {
+    case kPageExhausted: return fail_fmt(LLM_ERR_OOM, "KV page pool exhausted");
+    case kPageBadRequest: return fail_fmt(LLM_ERR_INVALID, "page request names a slot, page or length out of range, or a slot twice");
+    case kDevWaitTimeout: return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (bounded wait expired)", h);
+    case kDevBadPage: return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (bad page index)", h);
+  }
+  return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (unknown)", h);
+}
+
+extern "C" int llm_pages_copy(int device, const llm_page_cache* from, const llm_page_cache* to, const int32_t* src,
+                              const int32_t* dst, int n, void* stream) {
+  RC(check_geometry(from));
+  RC(check_geometry(to));
+  if (!from->status) return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
+  if (from->dtype != to->dtype || from->n_layers != to->n_layers || from->n_kv_heads != to->n_kv_heads ||
+      from->head_dim != to->head_dim)
+    return fail_fmt(LLM_ERR_INVALID, "the caches have different layers, heads, head_dim or dtype");
+  if (n < 0 || (n > 0 && (!src || !dst))) return fail_fmt(LLM_ERR_INVALID, "nil page list or negative count");
+  if (n == 0) return LLM_OK;
+  DeviceScope dev;
+  RC(dev.enter(device));
+  const PageTables a = tables(from), b = tables(to);
+  pages_copy_kernel<<<copy_grid(a, n), kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, b, src, dst, n);
+  CU(cudaGetLastError());
+  return LLM_OK;
+}
+
+extern "C" int llm_pages_fork(int device, const llm_page_cache* c, const int32_t* parents, const int32_t* children,
+                              const int32_t* lens, const int32_t* rooms, int n, void* stream) {
+  RC(check_tables(c));
+  if (n < 0 || n > c->max_seqs) return fail_fmt(LLM_ERR_INVALID, "%d requests for %d slots", n, c->max_seqs);
+  if (n == 0) return LLM_OK;
+  if (!parents || !children || !lens || !rooms) return fail_fmt(LLM_ERR_INVALID, "nil request array");
+  DeviceScope dev;
+  RC(dev.enter(device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ForkParams p{tables(c), parents, children, lens, rooms, n};
+  pages_fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  CU(cudaGetLastError());
+  CU(launch_dependent(pages_fork_kernel, dim3(copy_grid(p.t, n)), dim3(kCopyThreads), 0, s, p));
+  return LLM_OK;
+}
+
+extern "C" int llm_pages_free(int device, const llm_page_cache* c, const int32_t* slots, int n, void* stream) {
+  RC(check_tables(c));
+  if (n < 0 || (n > 0 && !slots)) return fail_fmt(LLM_ERR_INVALID, "nil slot list or negative count");
+  if (n == 0) return LLM_OK;
+  DeviceScope dev;
+  RC(dev.enter(device));
+  pages_free_kernel<<<std::min(n, 148), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(tables(c), slots, n);
+  CU(cudaGetLastError());
+  return LLM_OK;
+}
+
+extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stream) {
+  RC(check_tables(c));
+  DeviceScope dev;
+  RC(dev.enter(device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const PageTables t = tables(c);
+  pages_compact_plan_kernel<<<(t.n_pages + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, s>>>(t);
+  CU(cudaGetLastError());
+  CU(launch_dependent(pages_compact_kernel, dim3(copy_grid(t, t.n_pages / 2 + 1)), dim3(kCopyThreads), 0, s, t));
+  return LLM_OK;
+}

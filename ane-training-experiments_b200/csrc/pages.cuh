@@ -1,0 +1,411 @@
+// pages.cuh -- page management of a K/V cache whose tables live in device memory.
+//
+// The reference keeps one dense [layer][position][dim] cache per decoder (ane/stories/infer.go:
+// 113-114) and has nothing of this kind.  Sequences that start from a common prompt (samples,
+// beams, users of one system prompt) hold the prompt's pages in common: refs[p] counts the
+// block-table entries that name page p, and a page is free when its count is 0.
+//
+//   fork     child rows share the parent's complete pages (refs + 1); a partly filled last page
+//            is copied, so a page with room left always has one owner and appending never writes
+//            into a shared page
+//   free     refs - 1 for every entry of the rows; pages that reach 0 are pushed on the free
+//            stack in ascending order (the order does not depend on which CTA came first)
+//   compact  the L live pages move to ids 0..L-1: the k-th live page at or above L goes to the
+//            k-th dead page below L, the fewest moves there are; tables follow
+//   copy     listed pages, every layer
+//
+// Every table is an int32 array on the device, so parents chosen by a kernel (beam search) need
+// no host round trip and a step can be captured in a CUDA graph.  A request that cannot be
+// served writes `status` and changes nothing.
+#pragma once
+#include "common.cuh"
+
+namespace llm {
+
+// Status words of page requests, beside DeviceError's.
+enum PageError : int {
+  kPageExhausted = 3,   // the free stack holds fewer pages than the request needs
+  kPageBadRequest = 4,  // a slot, length or page out of range, or a slot listed twice
+};
+
+struct PageTables {
+  uint8_t* pool;           // [layers][n_pages][block_bytes]
+  int* n_free;
+  int* status;
+  int* npages;             // [max_seqs]
+  int* refs;               // [n_pages]
+  int* free_pages;         // [n_pages] stack
+  int* table;              // [max_seqs][max_pages]
+  int* work;               // PageWork::words() ints, zero between calls except the lists
+  int n_layers, n_pages, max_seqs, max_pages;
+  int block_bytes;         // n_kv_heads * 2 * 16 * head_dim * 2: one page of one layer
+};
+
+// Layout of the work area.  ticket, marks and bits are zero between calls.
+struct PageWork {
+  enum { kTicket = 0, kValid = 1, kCount = 2, kLive = 3, kHeader = 16 };
+  static __host__ __device__ size_t marks() { return kHeader; }                                  // [max_seqs]
+  static __host__ __device__ size_t first(int seqs) { return marks() + seqs; }                   // [max_seqs]
+  static __host__ __device__ size_t bits(int seqs) { return first(seqs) + seqs; }                // [n_pages / 32]
+  static __host__ __device__ size_t src(int seqs, int pages) { return bits(seqs) + (pages + 31) / 32; }  // [n_pages]
+  static __host__ __device__ size_t dst(int seqs, int pages) { return src(seqs, pages) + pages; }        // [n_pages]
+  static __host__ __device__ size_t words(int seqs, int pages) { return dst(seqs, pages) + pages; }
+};
+
+constexpr int kPlanThreads = 1024;
+constexpr int kCopyThreads = 256;
+constexpr int kCopyChunk = 4096;  // bytes one CTA copies per turn: 16 per thread
+
+__device__ __forceinline__ void page_fail(int* status, int code) { atomicCAS(status, 0, code); }
+
+// Exclusive prefix sum over the CTA's kPlanThreads values; `total` is their sum.  `s` holds 33 ints.
+__device__ __forceinline__ int block_exclusive(int v, int* s, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // s is free again
+  if (lane == 31) s[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    const int w = s[lane];
+    int y = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    s[lane] = y - w;
+    if (lane == 31) s[32] = y;
+  }
+  __syncthreads();
+  total = s[32];
+  return s[warp] + x - v;
+}
+
+// Chunk `c` of page move src -> dst: chunks run over (move, layer, offset in the block).
+__device__ __forceinline__ void copy_chunk(const uint8_t* from, int from_pages, uint8_t* to, int to_pages,
+                                           int block_bytes, int src, int dst, int layer, int offset) {
+  const size_t a = (static_cast<size_t>(layer) * from_pages + src) * block_bytes + offset;
+  const size_t b = (static_cast<size_t>(layer) * to_pages + dst) * block_bytes + offset;
+  const uint4 v = *reinterpret_cast<const uint4*>(from + a + threadIdx.x * 16);
+  *reinterpret_cast<uint4*>(to + b + threadIdx.x * 16) = v;
+}
+
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(PageTables from, PageTables to, const int* src,
+                                                                  const int* dst, int n) {
+  const int chunks = from.block_bytes / kCopyChunk;
+  const long long all = static_cast<long long>(n) * from.n_layers * chunks;
+  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
+    const int chunk = static_cast<int>(w % chunks);
+    const int layer = static_cast<int>((w / chunks) % from.n_layers);
+    const int i = static_cast<int>(w / chunks / from.n_layers);
+    const int a = src[i], b = dst[i];
+    if (a < 0 || a >= from.n_pages || b < 0 || b >= to.n_pages) {
+      if (threadIdx.x == 0) page_fail(from.status, kPageBadRequest);
+      continue;
+    }
+    copy_chunk(from.pool, from.n_pages, to.pool, to.n_pages, from.block_bytes, a, b, layer, chunk * kCopyChunk);
+  }
+}
+
+// ----------------------------------------------------------------------------- fork
+struct ForkParams {
+  PageTables t;
+  const int *parents, *children, *lens, *rooms;
+  int n;
+};
+struct ForkShape {
+  int keep, fresh;
+  bool grow, tail;
+};
+// What request i asks for; false when it asks for something that is not there.
+__device__ __forceinline__ bool fork_shape(const ForkParams& p, int i, ForkShape& f) {
+  const int par = p.parents[i], child = p.children[i], len = p.lens[i], room = p.rooms[i];
+  f = {0, 0, par == child, false};
+  if (child < 0 || child >= p.t.max_seqs || par < -1 || par >= p.t.max_seqs || room < 0) return false;
+  if (room > p.t.max_pages * 16) return false;
+  if (f.grow) {
+    f.keep = p.t.npages[child];
+  } else {
+    if (p.t.npages[child] != 0 || len < 0 || len > room) return false;
+    if (len > (par < 0 ? 0 : p.t.npages[par] * 16)) return false;
+    f.keep = len >> 4;
+    f.tail = (len & 15) != 0;
+  }
+  f.fresh = max(0, (room + 15) / 16 - f.keep);
+  return true;
+}
+
+// One CTA: checks every request, numbers the new pages and takes them off the stack.
+__global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParams p) {
+  __shared__ int s_scan[33];
+  __shared__ int s_bad;
+  griddep_launch_dependents();
+  griddep_wait();
+  int* const work = p.t.work;
+  int* const mark = work + PageWork::marks();
+  int* const first = work + PageWork::first(p.t.max_seqs);
+  if (threadIdx.x == 0) s_bad = 0;
+  __syncthreads();
+  int base = 0;
+  for (int i0 = 0; i0 < p.n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    ForkShape f{0, 0, false, false};
+    if (i < p.n) {
+      if (!fork_shape(p, i, f)) s_bad = 1;
+      else if (atomicExch(mark + p.children[i], 1) != 0) s_bad = 1;
+    }
+    int total;
+    const int off = block_exclusive(f.fresh, s_scan, total);
+    if (i < p.n) first[i] = base + off;
+    base += total;
+    if (base > p.t.n_pages) break;  // more than the pool has: refused below; also keeps the sum small
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.n; i += kPlanThreads) {
+    const int c = p.children[i];
+    if (c >= 0 && c < p.t.max_seqs) mark[c] = 0;
+  }
+  if (threadIdx.x == 0) {
+    const int have = *p.t.n_free;
+    const bool bad = s_bad != 0, out = base > have;
+    if (bad) page_fail(p.t.status, kPageBadRequest);
+    else if (out) page_fail(p.t.status, kPageExhausted);
+    work[PageWork::kValid] = !bad && !out;
+    work[PageWork::kCount] = have;
+    if (!bad && !out) *p.t.n_free = have - base;
+  }
+}
+
+// Rows, reference counts and the copies of partly filled pages.  The rows are read while npages
+// still holds the old counts; the last CTA stores the new ones.
+__global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(ForkParams p) {
+  __shared__ int s_last;
+  griddep_wait();
+  int* const work = p.t.work;
+  if (!work[PageWork::kValid]) return;
+  const int* first = work + PageWork::first(p.t.max_seqs);
+  const int top = work[PageWork::kCount];  // the stack before this call
+  for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
+    ForkShape f;
+    fork_shape(p, i, f);
+    const int par = p.parents[i];
+    int* row = p.t.table + static_cast<size_t>(p.children[i]) * p.t.max_pages;
+    const int* old = p.t.table + static_cast<size_t>(par < 0 ? 0 : par) * p.t.max_pages;
+    for (int j = threadIdx.x; j < f.keep + f.fresh; j += kCopyThreads) {
+      if (j < f.keep) {
+        if (f.grow) continue;
+        const int e = old[j];
+        row[j] = e;
+        if (e >= 0 && e < p.t.n_pages) atomicAdd(p.t.refs + e, 1);
+        else page_fail(p.t.status, kDevBadPage);
+      } else {
+        const int e = p.t.free_pages[top - 1 - first[i] - (j - f.keep)];
+        row[j] = e;
+        if (e >= 0 && e < p.t.n_pages) p.t.refs[e] = 1;
+        else page_fail(p.t.status, kDevBadPage);
+      }
+    }
+  }
+  const int chunks = p.t.block_bytes / kCopyChunk;
+  const long long all = static_cast<long long>(p.n) * p.t.n_layers * chunks;
+  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
+    const int i = static_cast<int>(w / chunks / p.t.n_layers);
+    ForkShape f;
+    fork_shape(p, i, f);
+    if (!f.tail) continue;
+    const int a = p.t.table[static_cast<size_t>(p.parents[i]) * p.t.max_pages + f.keep];
+    const int b = p.t.free_pages[top - 1 - first[i]];
+    if (a < 0 || a >= p.t.n_pages || b < 0 || b >= p.t.n_pages) {
+      if (threadIdx.x == 0) page_fail(p.t.status, kDevBadPage);
+      continue;
+    }
+    const int chunk = static_cast<int>(w % chunks);
+    copy_chunk(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.block_bytes, a, b,
+               static_cast<int>((w / chunks) % p.t.n_layers), chunk * kCopyChunk);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(work + PageWork::kTicket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < p.n; i += kCopyThreads) {
+    const int par = p.parents[i], child = p.children[i];
+    const int keep = par == child ? p.t.npages[child] : p.lens[i] >> 4;
+    p.t.npages[child] = max(keep, (p.rooms[i] + 15) / 16);
+  }
+  if (threadIdx.x == 0) work[PageWork::kTicket] = 0;
+}
+
+// ----------------------------------------------------------------------------- free
+__global__ void __launch_bounds__(kPlanThreads) pages_free_kernel(PageTables t, const int* slots, int n) {
+  __shared__ int s_scan[33];
+  __shared__ int s_held, s_last;
+  int* const work = t.work;
+  unsigned* const bits = reinterpret_cast<unsigned*>(work + PageWork::bits(t.max_seqs));
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int slot = slots[i];
+    if (slot < 0 || slot >= t.max_seqs) {
+      if (threadIdx.x == 0) page_fail(t.status, kPageBadRequest);
+      continue;
+    }
+    // taking the count frees the slot once, however often it is listed
+    if (threadIdx.x == 0) s_held = min(atomicExch(t.npages + slot, 0), t.max_pages);
+    __syncthreads();
+    int* row = t.table + static_cast<size_t>(slot) * t.max_pages;
+    for (int j = threadIdx.x; j < s_held; j += kPlanThreads) {
+      const int e = row[j];
+      row[j] = -1;
+      if (e < 0 || e >= t.n_pages) {
+        page_fail(t.status, kDevBadPage);
+        continue;
+      }
+      const int was = atomicSub(t.refs + e, 1);
+      if (was == 1) {
+        atomicOr(bits + (e >> 5), 1u << (e & 31));
+      } else if (was <= 0) {  // not counted: put it back, the page is not ours to push
+        atomicAdd(t.refs + e, 1);
+        page_fail(t.status, kDevBadPage);
+      }
+    }
+    __syncthreads();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(work + PageWork::kTicket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  // the emptied pages in ascending order on the stack: each thread a run of words
+  const int words = (t.n_pages + 31) / 32;
+  const int per = (words + kPlanThreads - 1) / kPlanThreads;
+  const int w0 = min(words, static_cast<int>(threadIdx.x) * per), w1 = min(words, w0 + per);
+  int mine = 0;
+  for (int w = w0; w < w1; ++w) mine += __popc(__ldcg(bits + w));
+  int total;
+  const int base = *t.n_free;
+  int at = base + block_exclusive(mine, s_scan, total);
+  for (int w = w0; w < w1; ++w) {
+    unsigned b = __ldcg(bits + w);
+    if (b == 0) continue;
+    bits[w] = 0;
+    for (; b != 0; b &= b - 1) {
+      if (at < t.n_pages) t.free_pages[at] = w * 32 + __ffs(b) - 1;
+      ++at;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (base + total > t.n_pages) page_fail(t.status, kDevBadPage);  // the stack did not match refs
+    *t.n_free = min(base + total, t.n_pages);
+    work[PageWork::kTicket] = 0;
+  }
+}
+
+// ----------------------------------------------------------------------------- compact
+// Live pages as a bit mask; the last CTA lists the moves and the new name of every moved page.
+__global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTables t) {
+  __shared__ int s_scan[33];
+  __shared__ int s_last;
+  griddep_launch_dependents();
+  int* const work = t.work;
+  unsigned* const bits = reinterpret_cast<unsigned*>(work + PageWork::bits(t.max_seqs));
+  const int words = (t.n_pages + 31) / 32;
+  const int p = blockIdx.x * kPlanThreads + threadIdx.x;
+  const unsigned live = __ballot_sync(0xffffffffu, p < t.n_pages && t.refs[p] > 0);
+  if ((threadIdx.x & 31) == 0 && (p >> 5) < words) bits[p >> 5] = live;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(work + PageWork::kTicket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  const int per = (words + kPlanThreads - 1) / kPlanThreads;
+  const int w0 = min(words, static_cast<int>(threadIdx.x) * per), w1 = min(words, w0 + per);
+  int mine = 0, n_live;
+  for (int w = w0; w < w1; ++w) mine += __popc(__ldcg(bits + w));
+  block_exclusive(mine, s_scan, n_live);
+  // bits of word w that are live at or above n_live / dead below it
+  auto above = [&](int w) -> unsigned {
+    const int lo = n_live - w * 32;  // ids below n_live in this word
+    const unsigned keep = lo <= 0 ? 0xffffffffu : (lo >= 32 ? 0u : 0xffffffffu << lo);
+    return __ldcg(bits + w) & keep;
+  };
+  auto holes = [&](int w) -> unsigned {
+    const int lo = n_live - w * 32;
+    const unsigned below = lo <= 0 ? 0u : (lo >= 32 ? 0xffffffffu : ~(0xffffffffu << lo));
+    return ~__ldcg(bits + w) & below;
+  };
+  int n_src = 0, n_dst = 0, moves, same;
+  for (int w = w0; w < w1; ++w) {
+    n_src += __popc(above(w));
+    n_dst += __popc(holes(w));
+  }
+  int a = block_exclusive(n_src, s_scan, moves);
+  int b = block_exclusive(n_dst, s_scan, same);
+  int* src = work + PageWork::src(t.max_seqs, t.n_pages);
+  int* dst = work + PageWork::dst(t.max_seqs, t.n_pages);
+  for (int w = w0; w < w1; ++w) {
+    for (unsigned m = above(w); m != 0; m &= m - 1) src[a++] = w * 32 + __ffs(m) - 1;
+    for (unsigned m = holes(w); m != 0; m &= m - 1) dst[b++] = w * 32 + __ffs(m) - 1;
+  }
+  __syncthreads();
+  for (int w = w0; w < w1; ++w) bits[w] = 0;
+  if (threadIdx.x == 0) {
+    work[PageWork::kCount] = moves;
+    work[PageWork::kLive] = n_live;
+    work[PageWork::kTicket] = 0;
+    *t.n_free = t.n_pages - n_live;
+  }
+}
+
+// The moves (sources are at or above n_live, destinations below it, so they never overlap), the
+// renamed counts and table entries, and the free stack.
+__global__ void __launch_bounds__(kCopyThreads) pages_compact_kernel(PageTables t) {
+  griddep_wait();
+  const int* work = t.work;
+  const int moves = work[PageWork::kCount], n_live = work[PageWork::kLive];
+  const int* src = work + PageWork::src(t.max_seqs, t.n_pages);
+  const int* dst = work + PageWork::dst(t.max_seqs, t.n_pages);
+  const long long tid = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x;
+  const long long step = static_cast<long long>(gridDim.x) * kCopyThreads;
+  const long long entries = static_cast<long long>(t.max_seqs) * t.max_pages;
+  for (long long k = tid; k < entries; k += step) {
+    const int e = t.table[k];
+    if (e < n_live) continue;
+    // the rank of e among the sources: src is ascending
+    int lo = 0, hi = moves;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (src[mid] < e) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo < moves && src[lo] == e) t.table[k] = dst[lo];
+    else page_fail(t.status, kDevBadPage);  // an entry whose page has no references
+  }
+  for (long long k = tid; k < moves; k += step) {
+    t.refs[dst[k]] = t.refs[src[k]];
+    t.refs[src[k]] = 0;
+  }
+  for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
+  const int chunks = t.block_bytes / kCopyChunk;
+  const long long all = static_cast<long long>(moves) * t.n_layers * chunks;
+  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
+    const int i = static_cast<int>(w / chunks / t.n_layers);
+    copy_chunk(t.pool, t.n_pages, t.pool, t.n_pages, t.block_bytes, src[i], dst[i],
+               static_cast<int>((w / chunks) % t.n_layers), static_cast<int>(w % chunks) * kCopyChunk);
+  }
+}
+
+}  // namespace llm

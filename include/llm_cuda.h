@@ -357,6 +357,58 @@ int llm_comm_last_gather_ms(llm_comm *comm, double *ms);
 int llm_gemm_i8_splitk_noalloc(int device, const int8_t *A, const int8_t *B, int M, int N, int K, int splits,
                                int32_t *C, void *stream);
 
+/* ---------------------------------------------------------------- paged caches of the caller */
+/* A paged K/V cache in caller-owned device memory, for programs that run their own layers over
+ * this library's kernels (the context's cache of llm_kv_alloc stays the context's).  Pages hold
+ * 16 positions; the pool is [n_layers][n_pages][n_kv_heads][K, V][16 * head_dim] of 16-bit
+ * values, the 8-value chunk c of row r of a K or V block at element
+ * (c / 8) * 1024 + r * 64 + ((c % 8) ^ (r % 8)) * 8.  The tables are int32 arrays on the device,
+ * so requests whose arguments a kernel computed (the parents of beams) need no host round trip
+ * and can be captured in a CUDA graph.  No counterpart in the reference, whose decoder keeps one
+ * dense cache per sequence (ane/stories/infer.go:113-114). */
+typedef struct llm_page_cache {
+  int32_t dtype;      /* LLM_DTYPE_F16 or LLM_DTYPE_BF16 */
+  int32_t n_layers, n_pages, n_kv_heads, head_dim; /* head_dim 64 or 128 */
+  int32_t max_seqs, max_pages; /* rows and columns of the block table */
+  void *pool;
+  int32_t *n_free;     /* [1] pages on the free stack                                     */
+  int32_t *status;     /* [1] 0, or the first failed request's code (llm_pages_status)     */
+  int32_t *npages;     /* [max_seqs] pages of each slot                                   */
+  int32_t *refs;       /* [n_pages] block-table entries that name each page; 0 = free      */
+  int32_t *free_pages; /* [n_pages] the free stack; its last entry is handed out next      */
+  int32_t *table;      /* [max_seqs][max_pages] page of each slot's 16 positions, -1 none   */
+  int32_t *work;       /* [llm_pages_work_words] zero before the first call                */
+} llm_page_cache;
+
+/* int32 words of the work area (0 for sizes out of range). */
+size_t llm_pages_work_words(int n_pages, int max_seqs);
+/* The requests below are enqueued on `stream` and return without waiting; every array argument
+ * is device memory, and calls on one cache must be ordered (they share its work area).  What the
+ * host cannot see is checked on the device: a request that names a slot, page or length out of
+ * range, or needs more pages than are free, sets *status; llm_pages_status waits for the stream,
+ * returns the matching LLM_ERR_* code (LLM_OK when nothing failed) and clears it. */
+int llm_pages_status(int device, const llm_page_cache *cache, void *stream);
+/* Copy page src[i] of `from` to page dst[i] of `to` in every layer, i < n.  The caches have the
+ * same layers, heads, head_dim and dtype and may be one cache; no dst[i] appears twice or among
+ * the sources of the same pool.  Tables are not changed. */
+int llm_pages_copy(int device, const llm_page_cache *from, const llm_page_cache *to, const int32_t *src,
+                   const int32_t *dst, int n, void *stream);
+/* Request i makes slot children[i] a copy of the first lens[i] positions of slot parents[i], with
+ * pages for rooms[i] >= lens[i] positions: complete pages are shared (refs + 1), a partly filled
+ * last page is copied in every layer, the rest are taken from the free stack in request order.
+ * parents[i] = -1 (lens[i] = 0): a new sequence.  parents[i] = children[i]: the slot keeps its
+ * pages and grows to rooms[i] positions (lens[i] is not read).  Children other than growing slots
+ * are empty, and no slot is a child twice.  All requests are served or none. */
+int llm_pages_fork(int device, const llm_page_cache *cache, const int32_t *parents, const int32_t *children,
+                   const int32_t *lens, const int32_t *rooms, int n, void *stream);
+/* Empty slots[i], i < n: refs - 1 for each of their pages; pages that reach 0 go on the free stack
+ * in ascending order.  An empty slot, or one listed again, changes nothing. */
+int llm_pages_free(int device, const llm_page_cache *cache, const int32_t *slots, int n, void *stream);
+/* Move the live pages to pages 0..L-1 (L = pages with references) in every layer with the fewest
+ * moves: the k-th live page at or above L goes to the k-th free page below it.  Block table and
+ * references follow; the free stack hands out L, L + 1, ... next. */
+int llm_pages_compact(int device, const llm_page_cache *cache, void *stream);
+
 /* ---------------------------------------------------------------- bit-exact debug hooks */
 /* RMSNorm + per-token quantiser on host rows x [rows, cols] run on the device with the
  * model kernel (w NULL: quantise only). */
