@@ -55,7 +55,7 @@ EXPORTS = [
     "llm_eval_window", "llm_debug_exp2", "llm_shard_range", "llm_comm_unique_id", "llm_comm_create",
     "llm_comm_destroy", "llm_gather_tokens", "llm_comm_last_gather_ms", "llm_linear_create", "llm_linear_eval_cf", "llm_linear_destroy",
     "llm_pages_work_words", "llm_pages_status", "llm_pages_copy", "llm_pages_fork", "llm_pages_free",
-    "llm_pages_compact",
+    "llm_pages_compact", "llm_prefix_plan_create", "llm_prefix_attend", "llm_prefix_plan_destroy",
 ]
 
 LLM_COMM_ID_BYTES = 128
@@ -176,6 +176,11 @@ def lib() -> C.CDLL:
                                      C.c_void_p]),
         "llm_pages_free": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
         "llm_pages_compact": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
+        "llm_prefix_plan_create": (C.c_int, [C.c_int] * 5 + [i32p, i32p, C.c_int, i32p, i32p, C.c_int, C.c_int,
+                                                             C.POINTER(C.c_void_p)]),
+        "llm_prefix_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                        C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
+        "llm_prefix_plan_destroy": (C.c_int, [C.c_void_p]),
         "llm_set_option": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
         "llm_gemm_i8_splitk_noalloc": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                                  C.c_void_p, C.c_void_p]),

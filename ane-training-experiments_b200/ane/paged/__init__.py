@@ -6,7 +6,8 @@ programs that run their own layers over this library's kernels (the cache inside
 pages in common: `fork` shares the complete pages and copies a partly filled last one, `free`
 counts references, `compact` gathers the live pages at the pool's start, `copy` moves listed pages.
 Requests are enqueued on the calling thread's current CUDA stream and return without waiting;
-`check` waits and raises for what the device refused.  The reference keeps one dense cache per
+`check` waits and raises for what the device refused.  `PrefixPlan.attend` is the attention of a
+batch in groups that share their first positions, the shared pages read once per group.  The reference keeps one dense cache per
 decoder (ane/stories/infer.go:113-114) and has no counterpart.
 
 torch is used for device memory and streams only; there is no CPU fallback.
@@ -123,3 +124,64 @@ class PagedCache:
         r = torch.arange(PAGE, device=self.device)[:, None]
         d = torch.arange(self.head_dim, device=self.device)[None]
         return (d // 64) * 1024 + r * 64 + (((d // 8) % 8) ^ (r % 8)) * 8 + d % 8
+
+
+class PrefixPlan:
+    """Attention of a batch over `cache` whose sequences share prefixes (llm_prefix_attend).
+
+    Sequence s reads slot slots[s] and has rows[s] query rows (1 when decoding); sequences come
+    group by group, group_sizes[g] of them sharing their first prefixes[g] positions, a multiple
+    of 16.  max_ctx bounds the positions a sequence may have.  The plan keeps the batch's layout
+    and workspace for every layer and step; calls on one plan must be ordered."""
+
+    def __init__(self, cache: PagedCache, n_heads: int, slots, rows, group_sizes, prefixes, max_ctx: int):
+        self.cache, self.n_heads, self._lib = cache, n_heads, cache._lib
+        slots, rows, sizes, prefixes = (_abi.i32(list(a)) for a in (slots, rows, group_sizes, prefixes))
+        if len(slots) != len(rows) or len(sizes) != len(prefixes):
+            raise LLMError(_abi.LLM_ERR_INVALID, "slots and rows, group_sizes and prefixes must have one length")
+        self.n_seqs, self.n_rows = len(slots), int(rows.sum())
+        h = C.c_void_p()
+        self.h = None
+        _abi.check(self._lib.llm_prefix_plan_create(
+            cache.device.index, _abi.DTYPES[cache.dtype], n_heads, cache.n_kv_heads, cache.head_dim,
+            _abi.ptr(slots, C.c_int32), _abi.ptr(rows, C.c_int32), self.n_seqs, _abi.ptr(sizes, C.c_int32),
+            _abi.ptr(prefixes, C.c_int32), len(sizes), max_ctx, C.byref(h)))
+        self.h = h
+
+    def _rows(self, t, what: str):
+        c = self.cache
+        if not isinstance(t, torch.Tensor) or t.dtype != c.torch_dtype or t.device != c.device or \
+                t.shape != (self.n_rows, self.n_heads, c.head_dim) or t.stride(2) != 1:
+            raise LLMError(_abi.LLM_ERR_INVALID, f"{what} must be a {c.torch_dtype} tensor [{self.n_rows}, {self.n_heads}, "
+                                                 f"{c.head_dim}] on {c.device} with contiguous rows of a head")
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+    def attend(self, layer: int, q, ctx, scale: float = 0.0, out=None, lse=None):
+        """Attention of query rows q [rows, n_heads, head_dim] in `layer`, sequence s having ctx[s]
+        positions of which its rows are the last; returns out (new when None).  lse (optional)
+        receives the log-sum-exp [rows, n_heads] in f32.  scale 0: 1 / sqrt(head_dim)."""
+        c = self.cache
+        qp, qr, qh = self._rows(q, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        op, orow, oh = self._rows(out, "out")
+        if lse is not None:
+            lp = _need(lse, "lse", torch.float32, c.device)
+            if lse.shape != (self.n_rows, self.n_heads):
+                raise LLMError(_abi.LLM_ERR_INVALID, f"lse has shape {tuple(lse.shape)}, not {(self.n_rows, self.n_heads)}")
+        else:
+            lp = None
+        _abi.check(self._lib.llm_prefix_attend(self.h, c._ref, layer, c._ints(ctx, "ctx", self.n_seqs), qp, qr, qh, scale,
+                                               op, orow, oh, lp, c._stream()))
+        return out
+
+    def close(self) -> None:
+        if self.h is not None:
+            self._lib.llm_prefix_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

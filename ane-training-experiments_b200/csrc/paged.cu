@@ -1,12 +1,16 @@
-// paged.cu -- C entries of the caller-owned paged caches: argument checks and launches of the
-// page requests (pages.cuh).
+// paged.cu -- C entries of the caller-owned paged caches: argument checks, plans and launches of
+// the page requests (pages.cuh) and of the attention over shared prefixes (attn_prefix.cuh).
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <new>
+#include <vector>
 
 #include "../../include/llm_cuda.h"
+#include "attn_prefix.cuh"
 #include "pages.cuh"
 
 using namespace llm;
@@ -200,5 +204,150 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
   pages_compact_plan_kernel<<<(t.n_pages + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, s>>>(t);
   CU(cudaGetLastError());
   CU(launch_dependent(pages_compact_kernel, dim3(copy_grid(t, t.n_pages / 2 + 1)), dim3(kCopyThreads), 0, s, t));
+  return LLM_OK;
+}
+
+// ============================================================================ shared prefixes
+struct llm_prefix_plan {
+  int device = 0, dtype = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0;
+  int n_seqs = 0, n_rows = 0, max_ctx = 0, top_slot = -1;
+  int* ints = nullptr;  // one device block: slots, row_start, row_seq
+  const int *slots = nullptr, *row_start = nullptr, *row_seq = nullptr;
+};
+
+extern "C" int llm_prefix_plan_destroy(llm_prefix_plan* plan) {
+  if (!plan) return fail_fmt(LLM_ERR_INVALID, "nil plan");
+  DeviceScope dev;
+  const int rc = dev.enter(plan->device);
+  if (rc == LLM_OK && plan->ints) cudaFree(plan->ints);
+  delete plan;
+  return rc;
+}
+
+extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_kv_heads, int head_dim,
+                                      const int32_t* slots, const int32_t* rows, int n_seqs,
+                                      const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
+                                      llm_prefix_plan** out) {
+  if (!out) return fail_fmt(LLM_ERR_INVALID, "nil output handle");
+  *out = nullptr;
+  if (dtype != LLM_DTYPE_F16 && dtype != LLM_DTYPE_BF16)
+    return fail_fmt(LLM_ERR_INVALID, "dtype %d (LLM_DTYPE_F16 or LLM_DTYPE_BF16)", dtype);
+  if (head_dim != 64 && head_dim != 128) return fail_fmt(LLM_ERR_UNSUPPORTED, "head_dim=%d (supported: 64, 128)", head_dim);
+  if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 1024)
+    return fail_fmt(LLM_ERR_INVALID, "n_heads=%d must be a multiple of n_kv_heads=%d", n_heads, n_kv_heads);
+  if (n_seqs <= 0 || n_groups <= 0 || max_ctx <= 0 || max_ctx > (1 << 28))
+    return fail_fmt(LLM_ERR_INVALID, "sequences, groups and max_ctx must be positive");
+  if (!slots || !rows || !group_sizes || !prefixes) return fail_fmt(LLM_ERR_INVALID, "nil plan array");
+  long long seqs = 0, total = 0;
+  for (int g = 0; g < n_groups; ++g) {
+    if (group_sizes[g] <= 0) return fail_fmt(LLM_ERR_INVALID, "group %d has %d sequences", g, group_sizes[g]);
+    if (prefixes[g] < 0 || prefixes[g] % 16 != 0 || prefixes[g] > max_ctx)
+      return fail_fmt(LLM_ERR_INVALID, "prefix %d of group %d is not a multiple of 16 within max_ctx=%d", prefixes[g], g, max_ctx);
+    seqs += group_sizes[g];
+  }
+  if (seqs != n_seqs) return fail_fmt(LLM_ERR_INVALID, "groups of %lld sequences in all, not %d", seqs, n_seqs);
+  int top = -1;
+  for (int s = 0; s < n_seqs; ++s) {
+    if (slots[s] < 0) return fail_fmt(LLM_ERR_INVALID, "sequence %d out of range", slots[s]);
+    if (rows[s] < 0) return fail_fmt(LLM_ERR_INVALID, "sequence %d has %d rows", s, rows[s]);
+    top = std::max(top, slots[s]);
+    total += rows[s];
+  }
+  if (total > (1 << 24)) return fail_fmt(LLM_ERR_INVALID, "%lld query rows", total);
+  try {
+    std::vector<int> ints(slots, slots + n_seqs);
+    ints.push_back(0);
+    for (int s = 0; s < n_seqs; ++s) ints.push_back(ints.back() + rows[s]);
+    for (int s = 0; s < n_seqs; ++s) ints.insert(ints.end(), rows[s], s);
+    DeviceScope dev;
+    RC(dev.enter(device));
+    llm_prefix_plan* p = new llm_prefix_plan;
+    p->device = device;
+    p->dtype = dtype;
+    p->n_heads = n_heads;
+    p->n_kv_heads = n_kv_heads;
+    p->head_dim = head_dim;
+    p->n_seqs = n_seqs;
+    p->n_rows = static_cast<int>(total);
+    p->max_ctx = max_ctx;
+    p->top_slot = top;
+    cudaError_t e = cudaMalloc(&p->ints, ints.size() * 4);
+    if (e != cudaSuccess) {
+      p->ints = nullptr;
+      llm_prefix_plan_destroy(p);
+      return fail_fmt(LLM_ERR_OOM, "cudaMalloc(%zu) failed: %s", ints.size() * 4, cudaGetErrorString(e));
+    }
+    e = cudaMemcpy(p->ints, ints.data(), ints.size() * 4, cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+      llm_prefix_plan_destroy(p);
+      return fail_fmt(LLM_ERR_CUDA, "plan upload failed: %s", cudaGetErrorString(e));
+    }
+    p->slots = p->ints;
+    p->row_start = p->slots + n_seqs;
+    p->row_seq = p->row_start + n_seqs + 1;
+    *out = p;
+    return LLM_OK;
+  } catch (const std::bad_alloc&) {
+    return fail_fmt(LLM_ERR_OOM, "host memory exhausted");
+  }
+}
+
+extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c, int layer, const int32_t* ctx,
+                                 const void* q, int64_t q_row, int64_t q_head, float scale, void* out, int64_t o_row,
+                                 int64_t o_head, float* lse, void* stream) {
+  if (!plan) return fail_fmt(LLM_ERR_INVALID, "nil plan");
+  RC(check_geometry(c));
+  if (!c->table || !c->status || !aligned(c->table, 4) || !aligned(c->status, 4))
+    return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
+  if (c->dtype != plan->dtype || c->n_kv_heads != plan->n_kv_heads || c->head_dim != plan->head_dim)
+    return fail_fmt(LLM_ERR_INVALID, "the cache's dtype, heads or head_dim are not the plan's");
+  if (plan->top_slot >= c->max_seqs) return fail_fmt(LLM_ERR_INVALID, "sequence %d out of range", plan->top_slot);
+  if (layer < 0 || layer >= c->n_layers) return fail_fmt(LLM_ERR_INVALID, "layer %d out of range", layer);
+  if (plan->n_rows == 0) return LLM_OK;
+  if (!ctx || !q || !out) return fail_fmt(LLM_ERR_INVALID, "nil buffer");
+  if (!aligned(ctx, 4) || !aligned(q, 16) || !aligned(out, 16) || !aligned(lse, 4))
+    return fail_fmt(LLM_ERR_INVALID, "misaligned buffer (q and out need 16-byte, ctx and lse 4-byte alignment)");
+  for (int64_t s : {q_row, q_head, o_row, o_head})
+    if (s % 8 != 0 || s < 0 || s > (int64_t{1} << 40))
+      return fail_fmt(LLM_ERR_INVALID, "stride %lld (a multiple of 8 elements is needed)", static_cast<long long>(s));
+  if (!std::isfinite(scale)) return fail_fmt(LLM_ERR_INVALID, "scale is not finite");
+  DeviceScope dev;
+  RC(dev.enter(plan->device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  PrefixParams p{};
+  p.q = q;
+  p.out = out;
+  p.lse = lse;
+  p.q_row = q_row;
+  p.q_head = q_head;
+  p.o_row = o_row;
+  p.o_head = o_head;
+  p.pool = static_cast<const uint8_t*>(c->pool) +
+           static_cast<size_t>(layer) * c->n_pages * c->n_kv_heads * (2 * 16 * 2) * c->head_dim;
+  p.table = c->table;
+  p.ctx = ctx;
+  p.slots = plan->slots;
+  p.row_start = plan->row_start;
+  p.row_seq = plan->row_seq;
+  p.status = c->status;
+  p.n_seqs = plan->n_seqs;
+  p.n_rows = plan->n_rows;
+  p.n_heads = plan->n_heads;
+  p.n_kv_heads = plan->n_kv_heads;
+  p.n_pages = c->n_pages;
+  p.max_pages = c->max_pages;
+  p.max_ctx = plan->max_ctx;
+  const double sc = scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim));
+  p.scale_log2 = static_cast<float>(sc * 1.4426950408889634);
+  const int grid = static_cast<int>((static_cast<long long>(p.n_rows) * p.n_heads + 3) / 4);
+  const bool bf = plan->dtype == LLM_DTYPE_BF16;
+  if (plan->head_dim == 64) {
+    if (bf) prefix_rows_kernel<__nv_bfloat16, 64><<<grid, 128, 0, s>>>(p);
+    else prefix_rows_kernel<__half, 64><<<grid, 128, 0, s>>>(p);
+  } else {
+    if (bf) prefix_rows_kernel<__nv_bfloat16, 128><<<grid, 128, 0, s>>>(p);
+    else prefix_rows_kernel<__half, 128><<<grid, 128, 0, s>>>(p);
+  }
+  CU(cudaGetLastError());
   return LLM_OK;
 }

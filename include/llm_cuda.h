@@ -409,6 +409,35 @@ int llm_pages_free(int device, const llm_page_cache *cache, const int32_t *slots
  * references follow; the free stack hands out L, L + 1, ... next. */
 int llm_pages_compact(int device, const llm_page_cache *cache, void *stream);
 
+/* ---------------------------------------------------------------- attention over shared prefixes */
+/* Causal attention of a batch of sequences in a paged cache, in groups that share their first
+ * positions: the shared pages are read once for all query rows of a group, each sequence's own
+ * pages once, and the two softmax states are joined.  Row r of sequence s (its rows are
+ * consecutive, sequences in order) stands at position ctx[s] - rows[s] + r and sees every position
+ * up to its own; a row that sees nothing gives 0.  K and V of a sequence's rows are in the cache
+ * before the call.  Replaces attend (ane/stories/infer.go:267-299) for such batches.
+ *
+ * A plan holds what stays while a batch runs (its layout, work lists and workspace), for every
+ * layer and step.  Sequence s reads block-table row slots[s] and has rows[s] >= 0 query rows;
+ * sequences come group by group, group_sizes[g] each, and share their first prefixes[g] positions
+ * (a multiple of 16, 0 = nothing: the first prefixes[g] / 16 block-table entries of a group's
+ * sequences name the same pages).  max_ctx bounds ctx.  n_heads is a multiple of n_kv_heads.
+ * All arrays are host memory. */
+typedef struct llm_prefix_plan llm_prefix_plan;
+int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_kv_heads, int head_dim, const int32_t *slots,
+                           const int32_t *rows, int n_seqs, const int32_t *group_sizes, const int32_t *prefixes,
+                           int n_groups, int max_ctx, llm_prefix_plan **out);
+/* Enqueue the attention of `layer` on `stream`; returns without waiting.  ctx [n_seqs] (int32), q and
+ * out (the cache's dtype; row and head strides in elements, head_dim contiguous, strides multiples
+ * of 8, 16-byte aligned) and lse (NULL, or f32 [rows][n_heads]: the log of each row's sum of
+ * exp(scale * q.k), -inf for a row that sees nothing) are device memory.  scale <= 0 means
+ * 1 / sqrt(head_dim).  Calls on one plan must be ordered (they share its workspace).  A context
+ * beyond max_ctx or the block table, or a bad page, sets the cache's status. */
+int llm_prefix_attend(llm_prefix_plan *plan, const llm_page_cache *cache, int layer, const int32_t *ctx, const void *q,
+                      int64_t q_row_stride, int64_t q_head_stride, float scale, void *out, int64_t out_row_stride,
+                      int64_t out_head_stride, float *lse, void *stream);
+int llm_prefix_plan_destroy(llm_prefix_plan *plan);
+
 /* ---------------------------------------------------------------- bit-exact debug hooks */
 /* RMSNorm + per-token quantiser on host rows x [rows, cols] run on the device with the
  * model kernel (w NULL: quantise only). */

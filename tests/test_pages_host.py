@@ -58,3 +58,28 @@ def test_work_words():
     L = _abi.lib()
     assert L.llm_pages_work_words(0, 4) == 0 and L.llm_pages_work_words(4, 0) == 0 and L.llm_pages_work_words(1 << 29, 4) == 0
     assert L.llm_pages_work_words(64, 4) == 16 + 2 * 4 + 2 + 2 * 64
+
+
+def plan_args(**kw):
+    """Arguments of llm_prefix_plan_create for two sequences, with some of them replaced."""
+    i32 = lambda *a: (C.c_int32 * len(a))(*a)  # noqa: E731
+    v = dict(device=0, dtype=_abi.LLM_DTYPE_F16, n_heads=4, n_kv_heads=2, head_dim=64, slots=i32(0, 1), rows=i32(1, 1), n_seqs=2,
+             sizes=i32(2), prefixes=i32(32), n_groups=1, max_ctx=64)
+    v |= {k: i32(*x) if isinstance(x, tuple) else x for k, x in kw.items()}
+    return list(v.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dtype=_abi.LLM_DTYPE_W8A8_BF16), INVALID, "dtype"), (dict(head_dim=80), UNSUPPORTED, "head_dim"),
+    (dict(n_heads=5), INVALID, "multiple"), (dict(n_kv_heads=0), INVALID, "multiple"), (dict(n_seqs=0), INVALID, "positive"),
+    (dict(n_groups=0), INVALID, "positive"), (dict(max_ctx=-1), INVALID, "positive"), (dict(slots=None), INVALID, "nil"),
+    (dict(rows=None), INVALID, "nil"), (dict(sizes=(0,)), INVALID, "group 0"), (dict(sizes=(3,)), INVALID, "in all"),
+    (dict(prefixes=(8,)), INVALID, "multiple of 16"), (dict(prefixes=(-16,)), INVALID, "multiple of 16"),
+    (dict(prefixes=(80,)), INVALID, "max_ctx"), (dict(slots=(0, -1)), INVALID, "out of range"), (dict(rows=(1, -1)), INVALID, "rows"),
+])
+def test_bad_plans_are_refused(kw, code, text):
+    L, h = _abi.lib(), C.c_void_p()
+    assert L.llm_prefix_plan_create(*plan_args(**kw), C.byref(h)) == code
+    assert text in _abi.last_error() and not h.value
+    assert L.llm_prefix_plan_create(*plan_args(), None) == INVALID
+    assert L.llm_prefix_plan_destroy(None) == INVALID
