@@ -5,13 +5,38 @@
 // with any m; m, l and the sum form a state that joins with another set of positions' state as
 //   M = max(m, m'), l = 2^(m-M) l + 2^(m'-M) l', o = 2^(m-M) o + 2^(m'-M) o'.
 // A row that sees nothing (ctx 0, or a row before position 0) gives o = 0 and lse = -inf.
+//
+// The plan cuts the work into items, each a run of score rows (query row, head of the kv head's
+// group) against a run of positions of one block-table row, for every kv head:
+//   part items   the shared positions of a group, all of the group's rows stacked, so a shared
+//                page is read once per 128 score rows; and pieces of a long own range.  They
+//                leave the state of each row in the workspace.
+//   final items  a sequence's own positions (the rest after the parts).  They join the row's
+//                part states to their own and write the output.
+// Two kernels take items of either kind: prefix_tile_kernel up to 128 score rows on the tcgen05
+// tensor cores, prefix_cols_kernel up to 8 on warp-level MMAs (eight columns cost it nothing, and
+// its CTAs need no tensor memory and a third of the registers).  The part launches come first;
+// the final launches start beside them (programmatic dependent launch), stream their own pages, and
+// wait for the parts only before they join.
 #pragma once
+#include "attention.cuh"
 #include "common.cuh"
 #include "pages.cuh"
+#include "umma.cuh"
 
 namespace llm {
 
+struct PrefixItem {
+  int row0;        // query row of score row 0's first head
+  int rho0;        // score rows rho0 .. rho0 + n_rho - 1 counted from row0's first head
+  int n_rho;
+  int pos0, pos1;  // positions [pos0, pos1), cut at the last one a row of the item sees
+  int part;        // part items: the state's number; final items: states to join (0 .. part - 1)
+};
+
 struct PrefixParams {
+  const PrefixItem* items;
+  int final;                  // the items are final items
   const void* q;
   void* out;
   float* lse;                 // [rows][n_heads] natural log, or nullptr
@@ -21,10 +46,11 @@ struct PrefixParams {
   const int* table;
   const int* ctx;             // [n_seqs]
   const int* slots;           // [n_seqs]
-  const int* row_start;       // [n_seqs + 1]
-  const int* row_seq;         // [n_rows]
+  const int2* row_info;       // [n_rows] sequence, rows of the sequence from this one on
+  float* ws_o;                // [parts][n_kv_heads][n_rows * group][HD] unnormalised sums
+  float2* ws_ml;              // [parts][n_kv_heads][n_rows * group] (m in log2 units, l)
   int* status;
-  int n_seqs, n_rows, n_heads, n_kv_heads, n_pages, max_pages, max_ctx;
+  int n_rows, n_heads, n_kv_heads, n_pages, max_pages, max_ctx;
   float scale_log2;
 };
 
@@ -34,54 +60,692 @@ __device__ __forceinline__ int seq_ctx(const PrefixParams& p, int s) {
   if (c > most) page_fail(p.status, kPageBadRequest);
   return max(0, min(c, most));
 }
+// Last position that query row `row` sees (negative: none), and its sequence.
+__device__ __forceinline__ int row_last(const PrefixParams& p, int row, int& seq) {
+  const int2 ri = p.row_info[row];
+  seq = ri.x;
+  return seq_ctx(p, ri.x) - ri.y;
+}
+__device__ __forceinline__ int page_entry(const PrefixParams& p, const int* bt, int lp) {
+  int e = bt[lp];
+  if (e < 0 || e >= p.n_pages) {
+    page_fail(p.status, kDevBadPage);
+    e = 0;
+  }
+  return e;
+}
+__device__ __forceinline__ float natural_lse(float m, float l) {
+  return l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
 
-// One warp per (row, head): a position at a time, lanes over the head's dimensions.
+// ============================================================================ up to 8 score rows
+// The arithmetic of attn_kernel (attention.cuh): S^T[16 positions x 8 columns] = K . Q^T, online
+// softmax per column, O^T += V^T . P^T with P as two terms; warp w takes pages w, w + 4, ... of
+// the item's range, and the four warps' states are joined once at the end.
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) prefix_rows_kernel(PrefixParams p) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (unit >= static_cast<long long>(p.n_rows) * p.n_heads) return;
-  const int row = static_cast<int>(unit / p.n_heads), head = static_cast<int>(unit % p.n_heads);
-  const int kvh = head / (p.n_heads / p.n_kv_heads);
-  const int s = p.row_seq[row];
-  const int ctx = seq_ctx(p, s);
-  const int last = ctx - (p.row_start[s + 1] - row);
-  const int* bt = p.table + static_cast<size_t>(p.slots[s]) * p.max_pages;
-  const T* q = static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
+__global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix_cols_kernel(PrefixParams p) {
+  using Cfg = AttnCfg<T, HD>;
+  constexpr int STAGES = Cfg::STAGES;
+  constexpr int PB = Cfg::PAGE_BYTES;
+  constexpr int KS = HD / 16;
+  constexpr int ROWB = HD * (int)sizeof(T);
+
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kAttnWarps][STAGES];
+  __shared__ float s_m[8], s_l[8];
+
+  griddep_launch_dependents();
+  const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
+  const int kvh = blockIdx.x % p.n_kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int group = p.n_heads / p.n_kv_heads;
+
+  // last visible position of this lane's two score columns; none for columns past the item
+  const int c0 = 2 * t, c1 = 2 * t + 1;
+  int seq = 0, seq1 = 0;
+  const int lim0 = c0 < it.n_rho ? row_last(p, it.row0 + (it.rho0 + c0) / group, seq) : -1;
+  const int lim1 = c1 < it.n_rho ? row_last(p, it.row0 + (it.rho0 + c1) / group, seq1) : -1;
+  if (lim1 > lim0) seq = seq1;
+  const int last = __reduce_max_sync(0xffffffffu, max(lim0, lim1));
+  // the sequence that sees furthest names the pages (an idle one's row may be empty)
+  seq = __shfl_sync(0xffffffffu, seq, __ffs(__ballot_sync(0xffffffffu, max(lim0, lim1) == last)) - 1);
+  const int end = min(it.pos1, last + 1);  // positions [it.pos0, end) are read
+  const int p_begin = it.pos0 >> 4, p_end = end > it.pos0 ? (end + 15) >> 4 : p_begin;
+
+  uint8_t* wbuf = smem + warp * Cfg::WARP_BYTES;
+  float* const fold_area = reinterpret_cast<float*>(smem + kAttnWarps * Cfg::WARP_BYTES);
+  float* const slot0 = fold_area;
+  float* const slot1 = fold_area + Cfg::SLOT_FLOATS;
+  const uint32_t wbase = smem_u32(wbuf);
+  const uint32_t bar0 = smem_u32(&bars[warp][0]);
+  const int* bt = p.table + static_cast<size_t>(p.slots[seq]) * p.max_pages;
+  auto page_src = [&](int lp) -> const uint8_t* {
+    return p.pool + (static_cast<size_t>(page_entry(p, bt, lp)) * p.n_kv_heads + kvh) * PB;
+  };
+
+  if (lane == 0) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = ActTraits<T>::to_f(q[lane * E + e]) * p.scale_log2;
-    o[e] = 0.f;
-  }
-  const T* block = nullptr;
-  for (int t = 0; t <= last; ++t) {
-    if ((t & 15) == 0) {
-      int page = bt[t >> 4];
-      if (page < 0 || page >= p.n_pages) {
-        page_fail(p.status, kDevBadPage);
-        page = 0;
+    for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_mbar_init();
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+      const int lp = p_begin + warp + kAttnWarps * s;
+      if (lp < p_end) {
+        mbar_arrive_expect_tx(bar0 + 8 * s, PB);
+        bulk_g2s(wbase + s * PB, page_src(lp), PB, bar0 + 8 * s);
       }
-      block = reinterpret_cast<const T*>(p.pool) + (static_cast<size_t>(page) * p.n_kv_heads + kvh) * (2 * 16 * HD);
     }
-    const int at = kv_off(t & 15, lane * E / 8) / 2 + (lane * E) % 8;
-    float x = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x += qv[e] * ActTraits<T>::to_f(block[at + e]);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-    const float mn = fmaxf(m, x), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2_det_lo(m - mu), w = exp2_det_lo(x - mu);
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * ActTraits<T>::to_f(block[16 * HD + at + e]);
-    m = mn;
   }
-  T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head;
+  __syncwarp();
+  // Q^T fragments: column g of the B operand is score row rho0 + g.
+  uint32_t qb[KS][2];
+  {
+    const bool ok = g < it.n_rho;
+    const int rho = it.rho0 + (ok ? g : 0);
+    const T* qrow = static_cast<const T*>(p.q) + (it.row0 + rho / group) * p.q_row + (kvh * group + rho % group) * p.q_head;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[lane * E + e] = ActTraits<T>::from_f(l > 0.f ? o[e] / l : 0.f);
-  if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = l > 0.f ? (m + log2f(l)) * 0.69314718056f : -INFINITY;
+    for (int ks = 0; ks < KS; ++ks) {
+      qb[ks][0] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t) : 0u;
+      qb[ks][1] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * t) : 0u;
+    }
+  }
+
+  WarpState<KS> st;
+  st.clear();
+  int seen = 0;       // pages this warp has consumed (ring position)
+  int fail_at = -1;   // ring position of an expired wait
+  for (int lp = p_begin + warp; lp < p_end; lp += kAttnWarps, ++seen) {
+    const int s = seen % STAGES;
+    if (!mbar_wait_bounded(bar0 + 8 * s, (seen / STAGES) & 1)) {
+      if (lane == 0) page_fail(p.status, kDevWaitTimeout);
+      fail_at = seen;
+      break;
+    }
+    const uint32_t kb = wbase + s * PB;
+    const uint32_t vb = kb + 16 * ROWB;
+    const int tok_base = lp * 16;
+    if (tok_base + 16 > end) {
+      // zero V rows past the range so 0-weight x stale data can never produce NaN
+      uint8_t* vblk = wbuf + s * PB + 16 * ROWB;
+      for (int i = lane; i < 16 * HD / 8; i += 32) {
+        const int rr = i / (HD / 8), c = i % (HD / 8);
+        if (tok_base + rr >= end) *reinterpret_cast<uint4*>(vblk + kv_off(rr, c)) = make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+    }
+    float sacc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a[4];
+      const int row = (lane & 7) + 8 * ((lane >> 3) & 1);
+      ldmatrix_x4(a, kb + kv_off(row, 2 * ks + (lane >> 4)));
+      mma_16816(sacc, a, qb[ks][0], qb[ks][1], T());
+    }
+    const int tk0 = tok_base + g, tk1 = tk0 + 8;
+    const int e0 = min(lim0, end - 1), e1 = min(lim1, end - 1);
+    const float s0 = tk0 <= e0 ? sacc[0] * p.scale_log2 : -INFINITY;
+    const float s1 = tk0 <= e1 ? sacc[1] * p.scale_log2 : -INFINITY;
+    const float s2 = tk1 <= e0 ? sacc[2] * p.scale_log2 : -INFINITY;
+    const float s3 = tk1 <= e1 ? sacc[3] * p.scale_log2 : -INFINITY;
+    float pm0 = fmaxf(s0, s2), pm1 = fmaxf(s1, s3);
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      pm0 = fmaxf(pm0, __shfl_xor_sync(0xffffffffu, pm0, off));
+      pm1 = fmaxf(pm1, __shfl_xor_sync(0xffffffffu, pm1, off));
+    }
+    const float mn0 = fmaxf(st.m0, pm0), mn1 = fmaxf(st.m1, pm1);
+    const float2 mu = make_float2(mn0 == -INFINITY ? 0.f : mn0, mn1 == -INFINITY ? 0.f : mn1);
+    const float2 al = exp2_det_lo2(sub2_rn(make_float2(st.m0, st.m1), mu));
+    const float2 p01 = exp2_det_lo2(sub2_rn(make_float2(s0, s1), mu));
+    const float2 p23 = exp2_det_lo2(sub2_rn(make_float2(s2, s3), mu));
+    st.l0 = st.l0 * al.x + (p01.x + p23.x);
+    st.l1 = st.l1 * al.y + (p01.y + p23.y);
+    st.m0 = mn0;
+    st.m1 = mn1;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      st.o[i][0] *= al.x;
+      st.o[i][1] *= al.y;
+      st.o[i][2] *= al.x;
+      st.o[i][3] *= al.y;
+    }
+    // P^T fragments of column g, positions (2t, 2t+1) and (2t+8, 2t+9), as hi + lo terms of the
+    // cache's type: one term would add its 2^-9 (bf16) to every weight; the pages take longer to
+    // arrive than the second term's MMAs
+    const uint32_t ph01 = ActTraits<T>::pack2(p01.x, p01.y), ph23 = ActTraits<T>::pack2(p23.x, p23.y);
+    const float2 h01 = ActTraits<T>::unpack2(ph01), h23 = ActTraits<T>::unpack2(ph23);
+    const uint32_t pl01 = ActTraits<T>::pack2(p01.x - h01.x, p01.y - h01.y);
+    const uint32_t pl23 = ActTraits<T>::pack2(p23.x - h23.x, p23.y - h23.y);
+    const int srcA = 8 * t + (g >> 1), srcB = srcA + 4;
+    const int sh = (g & 1) ? 16 : 0;
+    auto gather = [&](uint32_t v01, uint32_t v23, uint32_t& b0, uint32_t& b1) {
+      const uint32_t xa01 = __shfl_sync(0xffffffffu, v01, srcA), xa23 = __shfl_sync(0xffffffffu, v23, srcA);
+      const uint32_t xb01 = __shfl_sync(0xffffffffu, v01, srcB), xb23 = __shfl_sync(0xffffffffu, v23, srcB);
+      b0 = ((xa01 >> sh) & 0xffffu) | (((xb01 >> sh) & 0xffffu) << 16);
+      b1 = ((xa23 >> sh) & 0xffffu) | (((xb23 >> sh) & 0xffffu) << 16);
+    };
+    uint32_t bh0, bh1, bl0, bl1;
+    gather(ph01, ph23, bh0, bh1);
+    gather(pl01, pl23, bl0, bl1);
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) {
+      uint32_t a[4];
+      const int row = (lane & 7) + 8 * (lane >> 4);
+      ldmatrix_x4_trans(a, vb + kv_off(row, 2 * mt + ((lane >> 3) & 1)));
+      mma_16816(st.o[mt], a, bh0, bh1, T());
+      mma_16816(st.o[mt], a, bl0, bl1, T());
+    }
+    __syncwarp();
+    if (lane == 0) {
+      const int nlp = lp + kAttnWarps * STAGES;
+      if (nlp < p_end) {
+        fence_proxy_async_smem();
+        mbar_arrive_expect_tx(bar0 + 8 * s, PB);
+        bulk_g2s(kb, page_src(nlp), PB, bar0 + 8 * s);
+      }
+    }
+  }
+  if (fail_at >= 0) {
+    st.clear();  // an expired wait contributes nothing (the status is set)
+    for (int j = fail_at + 1; j < fail_at + STAGES; ++j) {  // copies still in flight (bounded)
+      if (p_begin + warp + kAttnWarps * j >= p_end) break;
+      mbar_wait_bounded(bar0 + 8 * (j % STAGES), (j / STAGES) & 1);
+    }
+  }
+#pragma unroll
+  for (int off = 4; off < 32; off <<= 1) {
+    st.l0 += __shfl_xor_sync(0xffffffffu, st.l0, off);
+    st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, off);
+  }
+  // (w0 + w1) + (w2 + w3), then the columns as rows [8][HD] in the fold area
+  if (warp == 1) store_slot(slot0, st, lane);
+  if (warp == 3) store_slot(slot1, st, lane);
+  __syncthreads();
+  if (warp == 0) fold_from_slot(st, slot0, lane);
+  if (warp == 2) {
+    fold_from_slot(st, slot1, lane);
+    store_slot(slot1, st, lane);  // each lane rewrites only the values it read
+  }
+  __syncthreads();
+  if (warp == 0) fold_from_slot(st, slot1, lane);
+  __syncthreads();
+  float* const stage = fold_area;
+  if (warp == 0) {
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) {
+      const int d = mt * 16 + g;
+      stage[c0 * HD + d] = st.o[mt][0];
+      stage[c1 * HD + d] = st.o[mt][1];
+      stage[c0 * HD + d + 8] = st.o[mt][2];
+      stage[c1 * HD + d + 8] = st.o[mt][3];
+    }
+    if (g == 0) {
+      s_m[c0] = st.m0;
+      s_m[c1] = st.m1;
+      s_l[c0] = st.l0;
+      s_l[c1] = st.l1;
+    }
+  }
+  __syncthreads();
+  const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
+  const size_t rho_all = static_cast<size_t>(it.row0) * group + it.rho0;
+  if (!p.final) {
+    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
+    for (int i = threadIdx.x; i < it.n_rho * HD / 4; i += kAttnWarps * 32)
+      __stcg(reinterpret_cast<float4*>(p.ws_o + at * HD) + i, reinterpret_cast<const float4*>(stage)[i]);
+    if (threadIdx.x < it.n_rho) __stcg(p.ws_ml + at + threadIdx.x, make_float2(s_m[threadIdx.x], s_l[threadIdx.x]));
+    griddep_wait();  // whoever waits for this launch has then waited for the ones before it
+    return;
+  }
+  griddep_wait();
+  // join: warp w takes columns w, w + 4
+  for (int c = warp; c < it.n_rho; c += kAttnWarps) {
+    constexpr int V = HD / 32;
+    float M = s_m[c];
+    for (int k = 0; k < it.part; ++k) {
+      const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all + c;
+      M = fmaxf(M, __ldcg(&p.ws_ml[at].x));
+    }
+    const float mu = M == -INFINITY ? 0.f : M;
+    const float w0 = exp2_det_lo(s_m[c] - mu);
+    float L = s_l[c] * w0, O[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) O[e] = stage[c * HD + lane * V + e] * w0;
+    for (int k = 0; k < it.part; ++k) {
+      const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all + c;
+      const float2 ml = __ldcg(p.ws_ml + at);
+      if (ml.x == -INFINITY) continue;  // a part without visible positions stores no sums
+      const float w = exp2_det_lo(ml.x - mu);
+      L += ml.y * w;
+#pragma unroll
+      for (int e = 0; e < V; ++e) O[e] += __ldcg(p.ws_o + at * HD + lane * V + e) * w;
+    }
+    const int row = it.row0 + (it.rho0 + c) / group, head = kvh * group + (it.rho0 + c) % group;
+    T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = ActTraits<T>::from_f(L > 0.f ? O[e] / L : 0.f);
+    if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+  }
+}
+
+// ============================================================================ up to 128 score rows
+// TMEM lane = score row.  64 positions at a time: S = Q . K^T into one of two TMEM buffers, one
+// softmax thread per row, P back into the S columns as hi + lo terms, O += P . V with P from
+// TMEM; the reference max of a row moves only when a tile exceeds it by 2^8 (the pipeline of
+// attn_prefill_tc_kernel, whose header explains it).  Here rows of many sequences share a tile
+// and every row has its own last position.
+template <typename T, int HD>
+struct PrefixTileCfg {
+  static constexpr int HALVES = HD / 64;              // 64-element halves of a K / V row
+  static constexpr int SUB = 16 * 128;                // one page's half sub-block (bytes)
+  static constexpr int REGION = 4 * SUB;              // 64 positions of one half (bytes)
+  static constexpr int TILE_BYTES = HALVES * REGION;  // K (or V) of one 64-position tile
+  static constexpr int K_STAGES = HD == 64 ? 3 : 2;
+  static constexpr int V_STAGES = HD == 64 ? 3 : 2;
+  static constexpr int Q_BYTES = HALVES * 128 * 128;  // 128 rows x HD, K-major halves
+  static constexpr int SMEM = Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + 1024;
+  static constexpr uint32_t TMEM_COLS = 256;          // S/P: 2 x 64 columns, O: HD columns at 128
+  static constexpr float RESCALE_LOG2 = 8.0f;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
+  using Cfg = PrefixTileCfg<T, HD>;
+  constexpr int KS = Cfg::K_STAGES, VS = Cfg::V_STAGES;
+  constexpr int HALVES = Cfg::HALVES;
+  constexpr int SUB = Cfg::SUB;
+  constexpr int REGION = Cfg::REGION;
+  constexpr int ROWB = HD * (int)sizeof(T);
+  constexpr uint32_t V_LBO = HALVES > 1 ? REGION : 1024;  // with one half never applied
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_ready[2],
+      pv_done, q_ready, drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ int2 s_last[4];
+
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_s = sbase;
+  const uint32_t k_ring = q_s + Cfg::Q_BYTES;
+  const uint32_t v_ring = k_ring + KS * Cfg::TILE_BYTES;
+  uint8_t* const gbase = smem_raw + (sbase - smem_u32(smem_raw));  // generic pointer of sbase
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
+  const int kvh = blockIdx.x % p.n_kv_heads;
+  const int group = p.n_heads / p.n_kv_heads;
+  // warps 2..5: this thread's score row (TMEM lane) and the last position it sees
+  const int tl = (warp & 3) * 32 + lane;
+  const bool row_ok = warp >= 2 && tl < it.n_rho;
+  const int rho = it.rho0 + (row_ok ? tl : 0);
+  const int row = it.row0 + rho / group, head = kvh * group + rho % group;
+  int seq = 0;
+  const int lim_row = row_ok ? row_last(p, row, seq) : -1;
+  if (warp >= 2) {
+    const int m = __reduce_max_sync(0xffffffffu, lim_row);
+    const int from = __ffs(__ballot_sync(0xffffffffu, lim_row == m)) - 1;
+    if (lane == from) s_last[warp & 3] = make_int2(m, seq);
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(smem_u32(&k_full[s]), 1);
+      mbar_init(smem_u32(&k_empty[s]), 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(smem_u32(&v_full[s]), 1);
+      mbar_init(smem_u32(&v_empty[s]), 1);
+    }
+    mbar_init(smem_u32(&s_full[0]), 1);
+    mbar_init(smem_u32(&s_full[1]), 1);
+    mbar_init(smem_u32(&p_ready[0]), 128);
+    mbar_init(smem_u32(&p_ready[1]), 128);
+    mbar_init(smem_u32(&pv_done), 1);
+    mbar_init(smem_u32(&q_ready), 128);
+    mbar_init(smem_u32(&drain), 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&s_tmem), Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  // dependents launch only after every CTA of this grid holds its TMEM columns
+  griddep_launch_dependents();
+
+  // the sequence that sees furthest names the pages (an idle one's row may be empty)
+  int2 far = s_last[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w)
+    if (s_last[w].x > far.x) far = s_last[w];
+  const int last = far.x;
+  const int end = min(it.pos1, last + 1);  // positions [it.pos0, end) are read
+  const int nkv = end > it.pos0 ? (end - it.pos0 + 63) >> 6 : 0;
+  const int page0 = it.pos0 >> 4;
+  const int n_pages_it = nkv > 0 ? ((end + 15) >> 4) - page0 : 0;
+  bool failed = false;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ bulk-copy producer
+    // The whole warp reads the block table, 32 pages (8 tiles) per coalesced load, one batch
+    // ahead of use; lane 0 issues the copies.  Waits run on every lane and are made uniform.
+    const int* bt = p.table + static_cast<size_t>(p.slots[far.y]) * p.max_pages + page0;
+    auto entries = [&](int first_page) -> int {
+      const int pg = first_page + lane;
+      return pg < n_pages_it ? page_entry(p, bt, pg) : 0;
+    };
+    int ent = entries(0), ent_next = entries(32);
+    // one tile of K (v = 0) or V (v = 1): its pages' half sub-blocks into one ring stage
+    auto load = [&](int t, int v, uint32_t dst, uint32_t bar) {
+      const int np = min(4, n_pages_it - 4 * t);
+      int phys[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) phys[j] = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + j);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, np * HALVES * SUB);
+        for (int j = 0; j < np; ++j) {
+          const uint8_t* blk = p.pool + (static_cast<size_t>(phys[j]) * p.n_kv_heads + kvh) * (2 * 16 * ROWB) + v * 16 * ROWB;
+          for (int hh = 0; hh < HALVES; ++hh) bulk_g2s(dst + hh * REGION + j * SUB, blk + hh * SUB, SUB, bar);
+        }
+      }
+    };
+    int k_issued = 0, v_issued = 0;
+    for (int t = 0; t < nkv; ++t) {
+      if (t > 0 && (t & 7) == 0) {
+        ent = ent_next;
+        ent_next = entries(4 * t + 32);
+      }
+      if (t >= KS && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&k_empty[t % KS]), ((t / KS) + 1) & 1))) {
+        failed = true;
+        break;
+      }
+      load(t, 0, k_ring + (t % KS) * Cfg::TILE_BYTES, smem_u32(&k_full[t % KS]));
+      k_issued = t + 1;
+      if (t >= VS && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&v_empty[t % VS]), ((t / VS) + 1) & 1))) {
+        failed = true;
+        break;
+      }
+      load(t, 1, v_ring + (t % VS) * Cfg::TILE_BYTES, smem_u32(&v_full[t % VS]));
+      v_issued = t + 1;
+    }
+    // copies still in flight must land before the CTA's shared memory goes away
+    if (lane == 0) {
+      for (int t = max(0, k_issued - KS); t < k_issued; ++t) mbar_wait_bounded(smem_u32(&k_full[t % KS]), (t / KS) & 1);
+      for (int t = max(0, v_issued - VS); t < v_issued; ++t) mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc<T>(128, 64);
+      constexpr uint32_t idesc_pv = umma_idesc<T>(128, HD) | (1u << 16);  // B (V) MN-major
+      const uint32_t o_tmem = tmem + 128;
+      // S_t into TMEM columns (t & 1) * 64; frees the K stage when the MMAs complete
+      auto issue_s = [&](int t) -> bool {
+        const int s = t % KS;
+        if (!mbar_wait_bounded(smem_u32(&k_full[s]), (t / KS) & 1)) return false;
+        tc_fence_after();
+        const uint32_t kst = k_ring + s * Cfg::TILE_BYTES;
+        const uint32_t d = tmem + (t & 1) * 64;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const int hh = k >> 2, kk = k & 3;
+          umma<false>(d, sw128_desc(q_s + hh * 128 * 128 + 32 * kk), sw128_desc(kst + hh * REGION + 32 * kk), idesc_s,
+                      k > 0 ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&k_empty[s]));
+        tc_commit(smem_u32(&s_full[t & 1]));
+        return true;
+      };
+      bool ok = mbar_wait_bounded(smem_u32(&q_ready), 0);
+      if (ok && nkv > 0) ok = issue_s(0);
+      if (ok && nkv > 1) ok = issue_s(1);
+      for (int t = 0; ok && t < nkv; ++t) {
+        if (!mbar_wait_bounded(smem_u32(&p_ready[t & 1]), (t >> 1) & 1) ||
+            !mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t vst = v_ring + (t % VS) * Cfg::TILE_BYTES;
+        const uint32_t pa = tmem + (t & 1) * 64;  // P_hi at +0, P_lo at +32 (16-bit pairs)
+#pragma unroll
+        for (int term = 0; term < 2; ++term) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 16 positions per MMA
+            umma_ts(o_tmem, pa + term * 32 + kk * 8, sw128_desc_mn(vst + kk * 2048, V_LBO, 1024), idesc_pv,
+                    (t > 0 || term > 0 || kk > 0) ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&v_empty[t % VS]));
+        tc_commit(smem_u32(&pv_done));
+        if (t + 2 < nkv) {
+          // S_{t+2} overwrites the columns P_t is read from: PV_t must be complete
+          if (!mbar_wait_bounded(smem_u32(&pv_done), t & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          ok = issue_s(t + 2);
+        }
+      }
+      if (!ok) failed = true;
+      // every MMA this thread issued has completed before O is read and TMEM is freed
+      tc_commit(smem_u32(&drain));
+      mbar_wait_bounded(smem_u32(&drain), 0);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax / epilogue warps
+    const int lim = min(lim_row, end - 1);     // last visible position of this row in the range
+    const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+
+    // Q row -> shared memory, K-major 128B-swizzled halves
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = row_ok ? src[c] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(gbase + (c >> 3) * 128 * 128 + tl * 128 + (((c & 7) ^ (tl & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&q_ready));
+    }
+
+    const float sl2 = p.scale_log2;
+    float m_ref = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int t = 0; t < nkv; ++t) {
+      // wait results are made warp-uniform: the TMEM accesses below are warp-collective
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&s_full[t & 1]), (t >> 1) & 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t scol = trow + (t & 1) * 64;
+      float sv[64];
+      {
+        uint32_t ra[32], rb[32];
+        tmem_ld32(scol, ra);
+        tmem_ld32(scol + 32, rb);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          sv[j] = __uint_as_float(ra[j]);
+          sv[32 + j] = __uint_as_float(rb[j]);
+        }
+      }
+      const int kbase = it.pos0 + t * 64;
+      if (__any_sync(0xffffffffu, kbase + 63 > lim)) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (kbase + j > lim) sv[j] = -INFINITY;
+      }
+      float m8[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m8[j] = sv[j];
+#pragma unroll
+      for (int j = 8; j < 64; ++j) m8[j & 7] = fmaxf(m8[j & 7], sv[j]);
+      const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                             fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * sl2;  // scale > 0
+      // move the reference max only past the gap; the first visible tile always sets it
+      const bool move = mx > m_ref + Cfg::RESCALE_LOG2;
+      const float m_new = move ? mx : m_ref;
+      const float mu = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = move ? exp2_det_lo(m_ref - mu) : 1.0f;
+      float2 r4[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r4[k] = make_float2(0.f, 0.f);
+      {
+        const float2 sl22 = make_float2(sl2, sl2), nmu = make_float2(-mu, -mu);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 pe = exp2_det_lo2(fma2_rn(make_float2(sv[2 * e], sv[2 * e + 1]), sl22, nmu));
+          sv[2 * e] = pe.x;
+          sv[2 * e + 1] = pe.y;
+          r4[e & 3] = add2_rn(r4[e & 3], pe);
+        }
+      }
+      l_run = l_run * alpha + (((r4[0].x + r4[0].y) + (r4[1].x + r4[1].y)) + ((r4[2].x + r4[2].y) + (r4[3].x + r4[3].y)));
+      m_ref = m_new;
+
+      // O holds PV of tiles < t: rescale rows whose reference moved, after PV_{t-1} completed
+      if (t > 0 && __any_sync(0xffffffffu, move)) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&pv_done), (t - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(trow + 128 + c * 32, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+          tmem_st32(trow + 128 + c * 32, r);
+        }
+      }
+      // V rows past the range were not loaded (or belong to nobody): zero them so a zero weight
+      // times stale data cannot make NaN (only the last tile is ragged; its V copies land first)
+      const int valid = end - kbase;
+      if (valid < 64) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1))) {
+          ok = false;
+          break;
+        }
+        uint8_t* vreg = gbase + (v_ring - sbase) + (t % VS) * Cfg::TILE_BYTES;
+        for (int idx = tl; idx < (64 - valid) * HALVES * 8; idx += 128) {
+          const int rr = valid + idx / (HALVES * 8), rem = idx % (HALVES * 8);
+          *reinterpret_cast<uint4*>(vreg + (rem >> 3) * REGION + rr * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      {
+        uint32_t hi[32], lo[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float a = sv[2 * e], b = sv[2 * e + 1];
+          hi[e] = ActTraits<T>::pack2(a, b);
+          const float2 hv = ActTraits<T>::unpack2(hi[e]);
+          lo[e] = ActTraits<T>::pack2(a - hv.x, b - hv.y);
+        }
+        tmem_st32(scol, hi);
+        tmem_st32(scol + 32, lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&p_ready[t & 1]));
+    }
+    if (ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&drain), 0));
+      tc_fence_after();
+    }
+    if (!ok) {
+      failed = true;
+      m_ref = -INFINITY;  // contributes nothing
+      l_run = 0.f;
+    }
+    if (l_run == 0.f) m_ref = -INFINITY;
+    const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
+    const size_t rho_all = static_cast<size_t>(it.row0) * group + rho;
+    const bool has = m_ref > -INFINITY;  // O of a row that saw nothing is not read
+    if (!p.final) {
+      const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
+      if (row_ok) __stcg(p.ws_ml + at, make_float2(m_ref, l_run));
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(trow + 128 + c * 32, r);
+        tmem_wait_ld();
+        if (!row_ok || !has) continue;
+        float4* dst = reinterpret_cast<float4*>(p.ws_o + at * HD + c * 32);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          __stcg(dst + j / 4, make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                                          __uint_as_float(r[j + 3])));
+      }
+    } else {
+      griddep_wait();
+      float M = m_ref;
+      if (row_ok)
+        for (int k = 0; k < it.part; ++k)
+          M = fmaxf(M, __ldcg(&p.ws_ml[(static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all].x));
+      const float mu = M == -INFINITY ? 0.f : M;
+      const float w0 = exp2_det_lo(m_ref - mu);
+      float L = l_run * w0;
+      if (row_ok)
+        for (int k = 0; k < it.part; ++k) {
+          const float2 ml = __ldcg(p.ws_ml + (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all);
+          if (ml.x > -INFINITY) L += ml.y * exp2_det_lo(ml.x - mu);
+        }
+      const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(trow + 128 + c * 32, r);
+        tmem_wait_ld();
+        if (!row_ok) continue;
+        float o[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = has ? __uint_as_float(r[j]) * w0 : 0.f;
+        for (int k = 0; k < it.part; ++k) {
+          const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all;
+          const float m = __ldcg(&p.ws_ml[at].x);
+          if (m == -INFINITY) continue;
+          const float w = exp2_det_lo(m - mu);
+          const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * HD + c * 32);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 v = __ldcg(src + j / 4);
+            o[j] += v.x * w;
+            o[j + 1] += v.y * w;
+            o[j + 2] += v.z * w;
+            o[j + 3] += v.w * w;
+          }
+        }
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + c * 32);
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint4 v;
+          v.x = ActTraits<T>::pack2(o[j] * inv, o[j + 1] * inv);
+          v.y = ActTraits<T>::pack2(o[j + 2] * inv, o[j + 3] * inv);
+          v.z = ActTraits<T>::pack2(o[j + 4] * inv, o[j + 5] * inv);
+          v.w = ActTraits<T>::pack2(o[j + 6] * inv, o[j + 7] * inv);
+          dst[j / 8] = v;
+        }
+      }
+      if (p.lse && row_ok) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+    }
+  }
+  if (failed) page_fail(p.status, kDevWaitTimeout);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+  griddep_wait();  // whoever waits for this launch has then waited for the ones before it
 }
 
 }  // namespace llm

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <new>
 #include <vector>
 
@@ -211,15 +212,168 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
 struct llm_prefix_plan {
   int device = 0, dtype = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0;
   int n_seqs = 0, n_rows = 0, max_ctx = 0, top_slot = -1;
-  int* ints = nullptr;  // one device block: slots, row_start, row_seq
-  const int *slots = nullptr, *row_start = nullptr, *row_seq = nullptr;
+  void* block = nullptr;  // one device allocation: items, row_info, slots, states, sums
+  const PrefixItem* items[2][2] = {};  // [part, final][tile, columns]
+  int n_items[2][2] = {};
+  const int2* row_info = nullptr;
+  const int* slots = nullptr;
+  float* ws_o = nullptr;
+  float2* ws_ml = nullptr;
 };
+
+namespace {
+
+enum { kPart = 0, kFinal = 1, kTile = 0, kCols = 1 };
+constexpr int kTileRows = 128;   // score rows of a tile item
+constexpr int kColRows = 8;      // score rows of a column item
+constexpr int kMaxParts = 64;    // states a row may have to join
+constexpr int kOpenEnd = 1 << 30;
+// Cost of starting and ending a CTA, in 64-position steps of its main loop.
+constexpr int kItemOverhead = 4;
+
+struct PlanGroup {
+  int seq0, n_seqs, prefix;
+  bool shared;
+  long long rho;  // score rows per kv head
+};
+
+int kernel_slots(int kind, int head_dim) { return 148 * (kind == kTile ? 2 : head_dim == 64 ? 5 : 3); }
+
+// Positions per part item of the shared prefixes: a multiple of 64 that finishes first when every
+// CTA slot takes ceil(items / slots) items of that length.
+int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, int slots) {
+  long long work = 0, longest = 0;
+  for (const PlanGroup& g : groups) {
+    if (!g.shared || (g.rho > kColRows) != (kind == kTile)) continue;
+    work += ((g.rho + kTileRows - 1) / kTileRows) * n_kv_heads * ((g.prefix + 63) / 64);
+    longest = std::max<long long>(longest, (g.prefix + 63) / 64);
+  }
+  if (work == 0) return 64;
+  const long long shortest = (longest + kMaxParts / 2 - 1) / (kMaxParts / 2);
+  long long best = longest, best_cost = -1;
+  for (int waves = 1; waves <= 4; ++waves) {
+    for (long long c = std::max(shortest, work / (static_cast<long long>(slots) * waves)), end = c + 8; c <= end; ++c) {
+      if (c < 1) continue;
+      long long items = 0;
+      for (const PlanGroup& g : groups)
+        if (g.shared && (g.rho > kColRows) == (kind == kTile))
+          items += ((g.rho + kTileRows - 1) / kTileRows) * n_kv_heads * (((g.prefix + 63) / 64 + c - 1) / c);
+      const long long cost = ((items + slots - 1) / slots) * (std::min(c, longest) + kItemOverhead);
+      if (best_cost < 0 || cost < best_cost) best = c, best_cost = cost;
+    }
+  }
+  return static_cast<int>(std::min(best, longest) * 64);
+}
+
+// The items of a batch.  Returns the number of states its rows may have.
+int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
+               int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2][2]) {
+  std::vector<PlanGroup> groups;
+  std::vector<int> row_start(1, 0);
+  long long final_ctas = 0;
+  int seq = 0;
+  for (int g = 0; g < n_groups; ++g) {
+    PlanGroup pg{seq, group_sizes[g], prefixes[g], false, 0};
+    int active = 0;
+    long long alone = 0;
+    for (int i = 0; i < group_sizes[g]; ++i, ++seq) {
+      const long long rho = static_cast<long long>(rows[seq]) * group;
+      row_start.push_back(row_start.back() + rows[seq]);
+      active += rho > 0;
+      pg.rho += rho;
+      alone += (rho + kTileRows - 1) / kTileRows;
+    }
+    final_ctas += alone * n_kv_heads;
+    // sharing pays when stacking the rows makes fewer passes over the prefix's pages
+    const long long stacked = (pg.rho + kTileRows - 1) / kTileRows;
+    pg.shared = active >= 2 && prefixes[g] > 0 && stacked * 10 <= alone * 7;
+    groups.push_back(pg);
+  }
+  // pieces of the own ranges, when the final items alone leave most of the machine idle
+  const int pieces = final_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, final_ctas)));
+  const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim)),
+                      part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim))};
+  int parts = 0;
+  for (const PlanGroup& g : groups) {
+    int shared_parts = 0;
+    if (g.shared) {
+      const int kind = g.rho > kColRows ? kTile : kCols;
+      for (int pos = 0; pos < g.prefix; pos += len[kind], ++shared_parts)
+        for (long long r = 0; r < g.rho; r += kTileRows)
+          items[kPart][kind].push_back({row_start[g.seq0], static_cast<int>(r),
+                                        static_cast<int>(std::min<long long>(kTileRows, g.rho - r)), pos,
+                                        std::min(g.prefix, pos + len[kind]), shared_parts});
+    }
+    const int start = g.shared ? g.prefix : 0;
+    const int bound = max_ctx - start;  // most own positions
+    int n = std::max(1, std::min(pieces, bound / 512)), piece = kOpenEnd;
+    if (n > 1) piece = ((bound + n - 1) / n + 63) / 64 * 64;
+    for (int s = g.seq0; s < g.seq0 + g.n_seqs; ++s) {
+      const long long rho = static_cast<long long>(rows[s]) * group;
+      const int kind = rho > kColRows ? kTile : kCols;
+      int own = 0;
+      for (int pos = start + piece; n > 1 && pos < max_ctx; pos += piece, ++own)
+        for (long long r = 0; r < rho; r += kTileRows)
+          items[kPart][kind].push_back({row_start[s], static_cast<int>(r), static_cast<int>(std::min<long long>(kTileRows, rho - r)),
+                                        pos, pos + piece, shared_parts + own});
+      for (long long r = (rho - 1) / kTileRows * kTileRows; rho > 0 && r >= 0; r -= kTileRows)  // longest first
+        items[kFinal][kind].push_back({row_start[s], static_cast<int>(r), static_cast<int>(std::min<long long>(kTileRows, rho - r)),
+                                       start, n > 1 ? start + piece : kOpenEnd, shared_parts + own});
+      parts = std::max(parts, shared_parts + own);
+    }
+  }
+  for (auto& v : items[kPart])
+    std::stable_sort(v.begin(), v.end(), [](const PrefixItem& a, const PrefixItem& b) { return a.pos1 - a.pos0 > b.pos1 - b.pos0; });
+  return parts;
+}
+
+template <typename T, int HD>
+cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStream_t s, bool prepare) {
+  if (prepare) {
+    cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         PrefixTileCfg<T, HD>::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(prefix_cols_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnCfg<T, HD>::SMEM);
+    return e;
+  }
+  bool first = true;  // the first launch waits for the stream's earlier work as a whole
+  for (int final = 0; final < 2; ++final)
+    for (int kind = 0; kind < 2; ++kind) {
+      const int n = plan->n_items[final][kind];
+      if (n == 0) continue;
+      p.items = plan->items[final][kind];
+      p.final = final;
+      const dim3 grid(n * plan->n_kv_heads);
+      cudaError_t e;
+      if (kind == kTile) {
+        constexpr int smem = PrefixTileCfg<T, HD>::SMEM;
+        if (first) prefix_tile_kernel<T, HD><<<grid, 192, smem, s>>>(p), e = cudaGetLastError();
+        else e = launch_dependent(prefix_tile_kernel<T, HD>, grid, dim3(192), smem, s, p);
+      } else {
+        constexpr int smem = AttnCfg<T, HD>::SMEM;
+        if (first) prefix_cols_kernel<T, HD><<<grid, kAttnWarps * 32, smem, s>>>(p), e = cudaGetLastError();
+        else e = launch_dependent(prefix_cols_kernel<T, HD>, grid, dim3(kAttnWarps * 32), smem, s, p);
+      }
+      if (e != cudaSuccess) return e;
+      first = false;
+    }
+  return cudaSuccess;
+}
+
+cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, cudaStream_t s, bool prepare) {
+  const bool bf = plan->dtype == LLM_DTYPE_BF16;
+  if (plan->head_dim == 64)
+    return bf ? prefix_launch<__nv_bfloat16, 64>(plan, p, s, prepare) : prefix_launch<__half, 64>(plan, p, s, prepare);
+  return bf ? prefix_launch<__nv_bfloat16, 128>(plan, p, s, prepare) : prefix_launch<__half, 128>(plan, p, s, prepare);
+}
+
+}  // namespace
 
 extern "C" int llm_prefix_plan_destroy(llm_prefix_plan* plan) {
   if (!plan) return fail_fmt(LLM_ERR_INVALID, "nil plan");
   DeviceScope dev;
   const int rc = dev.enter(plan->device);
-  if (rc == LLM_OK && plan->ints) cudaFree(plan->ints);
+  if (rc == LLM_OK && plan->block) cudaFree(plan->block);
   delete plan;
   return rc;
 }
@@ -253,15 +407,19 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     top = std::max(top, slots[s]);
     total += rows[s];
   }
-  if (total > (1 << 24)) return fail_fmt(LLM_ERR_INVALID, "%lld query rows", total);
+  if (total > (1 << 20)) return fail_fmt(LLM_ERR_INVALID, "%lld query rows", total);
+  llm_prefix_plan* p = nullptr;
   try {
-    std::vector<int> ints(slots, slots + n_seqs);
-    ints.push_back(0);
-    for (int s = 0; s < n_seqs; ++s) ints.push_back(ints.back() + rows[s]);
-    for (int s = 0; s < n_seqs; ++s) ints.insert(ints.end(), rows[s], s);
+    const int group = n_heads / n_kv_heads;
+    std::vector<PrefixItem> items[2][2];
+    const int parts = plan_items(rows, group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items);
+    std::vector<int2> info;
+    info.reserve(total);
+    for (int s = 0; s < n_seqs; ++s)
+      for (int r = 0; r < rows[s]; ++r) info.push_back(make_int2(s, rows[s] - r));
     DeviceScope dev;
     RC(dev.enter(device));
-    llm_prefix_plan* p = new llm_prefix_plan;
+    p = new llm_prefix_plan;
     p->device = device;
     p->dtype = dtype;
     p->n_heads = n_heads;
@@ -271,23 +429,49 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     p->n_rows = static_cast<int>(total);
     p->max_ctx = max_ctx;
     p->top_slot = top;
-    cudaError_t e = cudaMalloc(&p->ints, ints.size() * 4);
+    // the device block: host-built arrays first, then the workspace
+    std::vector<uint8_t> host;
+    auto place = [&host](const void* src, size_t bytes) -> size_t {
+      const size_t at = (host.size() + 255) / 256 * 256;
+      host.resize(at + bytes);
+      if (bytes) memcpy(host.data() + at, src, bytes);
+      return at;
+    };
+    size_t at_items[2][2];
+    for (int f = 0; f < 2; ++f)
+      for (int k = 0; k < 2; ++k) {
+        p->n_items[f][k] = static_cast<int>(items[f][k].size());
+        at_items[f][k] = place(items[f][k].data(), items[f][k].size() * sizeof(PrefixItem));
+      }
+    const size_t at_info = place(info.data(), info.size() * sizeof(int2));
+    const size_t at_slots = place(slots, static_cast<size_t>(n_seqs) * 4);
+    const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
+    const size_t at_ml = (host.size() + 255) / 256 * 256, at_o = (at_ml + states * 8 + 255) / 256 * 256;
+    const size_t bytes = at_o + states * head_dim * 4;
+    cudaError_t e = cudaMalloc(&p->block, bytes);
     if (e != cudaSuccess) {
-      p->ints = nullptr;
+      p->block = nullptr;
+      cudaGetLastError();
       llm_prefix_plan_destroy(p);
-      return fail_fmt(LLM_ERR_OOM, "cudaMalloc(%zu) failed: %s", ints.size() * 4, cudaGetErrorString(e));
+      return fail_fmt(LLM_ERR_OOM, "cudaMalloc(%zu) failed: %s", bytes, cudaGetErrorString(e));
     }
-    e = cudaMemcpy(p->ints, ints.data(), ints.size() * 4, cudaMemcpyHostToDevice);
+    e = cudaMemcpy(p->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = prefix_any(p, PrefixParams{}, nullptr, true);
     if (e != cudaSuccess) {
       llm_prefix_plan_destroy(p);
-      return fail_fmt(LLM_ERR_CUDA, "plan upload failed: %s", cudaGetErrorString(e));
+      return fail_fmt(LLM_ERR_CUDA, "plan set-up failed: %s", cudaGetErrorString(e));
     }
-    p->slots = p->ints;
-    p->row_start = p->slots + n_seqs;
-    p->row_seq = p->row_start + n_seqs + 1;
+    uint8_t* base = static_cast<uint8_t*>(p->block);
+    for (int f = 0; f < 2; ++f)
+      for (int k = 0; k < 2; ++k) p->items[f][k] = reinterpret_cast<const PrefixItem*>(base + at_items[f][k]);
+    p->row_info = reinterpret_cast<const int2*>(base + at_info);
+    p->slots = reinterpret_cast<const int*>(base + at_slots);
+    p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
+    p->ws_o = reinterpret_cast<float*>(base + at_o);
     *out = p;
     return LLM_OK;
   } catch (const std::bad_alloc&) {
+    if (p) llm_prefix_plan_destroy(p);
     return fail_fmt(LLM_ERR_OOM, "host memory exhausted");
   }
 }
@@ -313,7 +497,6 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   if (!std::isfinite(scale)) return fail_fmt(LLM_ERR_INVALID, "scale is not finite");
   DeviceScope dev;
   RC(dev.enter(plan->device));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   PrefixParams p{};
   p.q = q;
   p.out = out;
@@ -327,10 +510,10 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   p.table = c->table;
   p.ctx = ctx;
   p.slots = plan->slots;
-  p.row_start = plan->row_start;
-  p.row_seq = plan->row_seq;
+  p.row_info = plan->row_info;
+  p.ws_o = plan->ws_o;
+  p.ws_ml = plan->ws_ml;
   p.status = c->status;
-  p.n_seqs = plan->n_seqs;
   p.n_rows = plan->n_rows;
   p.n_heads = plan->n_heads;
   p.n_kv_heads = plan->n_kv_heads;
@@ -339,15 +522,6 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   p.max_ctx = plan->max_ctx;
   const double sc = scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim));
   p.scale_log2 = static_cast<float>(sc * 1.4426950408889634);
-  const int grid = static_cast<int>((static_cast<long long>(p.n_rows) * p.n_heads + 3) / 4);
-  const bool bf = plan->dtype == LLM_DTYPE_BF16;
-  if (plan->head_dim == 64) {
-    if (bf) prefix_rows_kernel<__nv_bfloat16, 64><<<grid, 128, 0, s>>>(p);
-    else prefix_rows_kernel<__half, 64><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (bf) prefix_rows_kernel<__nv_bfloat16, 128><<<grid, 128, 0, s>>>(p);
-    else prefix_rows_kernel<__half, 128><<<grid, 128, 0, s>>>(p);
-  }
-  CU(cudaGetLastError());
+  CU(prefix_any(plan, p, static_cast<cudaStream_t>(stream), false));
   return LLM_OK;
 }
