@@ -9,11 +9,11 @@
 // The plan cuts the work into items, each a run of score rows (query row, head of the kv head's
 // group) against a run of positions of one block-table row, for every kv head:
 //   part items   the shared positions of a group, all of the group's rows stacked, so a shared
-//                page is read once per 128 score rows; and pieces of a long own range.  They
+//                page is read once per 256 score rows; and pieces of a long own range.  They
 //                leave the state of each row in the workspace.
 //   final items  a sequence's own positions (the rest after the parts).  They join the row's
 //                part states to their own and write the output.
-// Two kernels take items of either kind: prefix_tile_kernel up to 128 score rows on the tcgen05
+// Two kernels take items of either kind: prefix_tile_kernel up to 256 score rows on the tcgen05
 // tensor cores, prefix_cols_kernel up to 8 on warp-level MMAs (eight columns cost it nothing, and
 // its CTAs need no tensor memory and a third of the registers).  The part launches come first;
 // the final launches start beside them (programmatic dependent launch), stream their own pages, and
@@ -299,60 +299,148 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
     return;
   }
   griddep_wait();
-  // join: warp w takes columns w, w + 4
-  for (int c = warp; c < it.n_rho; c += kAttnWarps) {
-    constexpr int V = HD / 32;
-    float M = s_m[c];
-    for (int k = 0; k < it.part; ++k) {
-      const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all + c;
-      M = fmaxf(M, __ldcg(&p.ws_ml[at].x));
+  // Join.  SUB warps share a column, each taking every SUB-th state; lane k holds the weights of
+  // states k and k + 32 (kMaxParts is 64), and a lane adds its HD / 32 dimensions of eight states at
+  // a time.
+  constexpr int V = HD / 32;
+  const int share = it.n_rho == 1 ? 4 : it.n_rho == 2 ? 2 : 1;  // warps per column
+  const int sub = warp % share;
+  float* const partial = reinterpret_cast<float*>(smem);  // [4][HD]: the page ring is idle
+  for (int c0w = 0; c0w < it.n_rho; c0w += kAttnWarps / share) {
+    const int c = c0w + warp / share;
+    const bool on = c < it.n_rho;
+    float M = -INFINITY, L = 0.f, O[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) O[e] = 0.f;
+    if (on) {
+      const size_t step = static_cast<size_t>(p.n_kv_heads) * rows_all;
+      const size_t at = static_cast<size_t>(kvh) * rows_all + rho_all + c;
+      float2 a = make_float2(-INFINITY, 0.f), b = a;
+      if (lane < it.part) a = __ldcg(p.ws_ml + at + lane * step);
+      if (lane + 32 < it.part) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
+      M = fmaxf(warp_max(fmaxf(a.x, b.x)), s_m[c]);
+      const float mu = M == -INFINITY ? 0.f : M;
+      const float wa = exp2_det_lo(a.x - mu), wb = exp2_det_lo(b.x - mu), w0 = exp2_det_lo(s_m[c] - mu);
+      L = a.y * wa + b.y * wb;
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+      L += s_l[c] * w0;
+      if (sub == 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) O[e] = stage[c * HD + lane * V + e] * w0;
+      }
+      const float* src = p.ws_o + at * HD + lane * V;
+      for (int k0 = sub; k0 < it.part; k0 += 8 * share) {
+        float v[8][V], w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = k0 + i * share;
+          w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
+          if (k >= it.part) w[i] = 0.f;
+          if (w[i] > 0.f) {  // a state without visible positions holds no sums
+            if constexpr (V == 4) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(src + k * step * HD));
+              v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+            } else {
+              const float2 x = __ldcg(reinterpret_cast<const float2*>(src + k * step * HD));
+              v[i][0] = x.x, v[i][1] = x.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
+      }
     }
-    const float mu = M == -INFINITY ? 0.f : M;
-    const float w0 = exp2_det_lo(s_m[c] - mu);
-    float L = s_l[c] * w0, O[V];
+    if (share > 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) O[e] = stage[c * HD + lane * V + e] * w0;
-    for (int k = 0; k < it.part; ++k) {
-      const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all + c;
-      const float2 ml = __ldcg(p.ws_ml + at);
-      if (ml.x == -INFINITY) continue;  // a part without visible positions stores no sums
-      const float w = exp2_det_lo(ml.x - mu);
-      L += ml.y * w;
+      for (int e = 0; e < V; ++e) partial[warp * HD + lane * V + e] = O[e];
+      __syncthreads();
+      if (sub == 0)
+        for (int k = 1; k < share; ++k)
 #pragma unroll
-      for (int e = 0; e < V; ++e) O[e] += __ldcg(p.ws_o + at * HD + lane * V + e) * w;
+          for (int e = 0; e < V; ++e) O[e] += partial[(warp + k) * HD + lane * V + e];
     }
-    const int row = it.row0 + (it.rho0 + c) / group, head = kvh * group + (it.rho0 + c) % group;
-    T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
+    if (on && sub == 0) {
+      const int row = it.row0 + (it.rho0 + c) / group, head = kvh * group + (it.rho0 + c) % group;
+      T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
+      const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = ActTraits<T>::from_f(L > 0.f ? O[e] / L : 0.f);
-    if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+      for (int e = 0; e < V; e += 2)
+        *reinterpret_cast<uint32_t*>(out + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
+      if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+    }
   }
 }
 
-// ============================================================================ up to 128 score rows
-// TMEM lane = score row.  64 positions at a time: S = Q . K^T into one of two TMEM buffers, one
-// softmax thread per row, P back into the S columns as hi + lo terms, O += P . V with P from
+// ============================================================================ up to 256 score rows
+// One CTA per SM with two streams, each of 128 TMEM lanes, 256 TMEM columns (two S / P buffers of
+// 64 and O) and four softmax warps with one score row per thread.  64 positions at a time a stream
+// runs S = Q . K^T, softmax, P back over the S columns as hi + lo terms, O += P . V with P from
 // TMEM; the reference max of a row moves only when a tile exceeds it by 2^8 (the pipeline of
-// attn_prefill_tc_kernel, whose header explains it).  Here rows of many sequences share a tile
-// and every row has its own last position.
+// attn_prefill_tc_kernel, whose header explains it).
+//   more than 128 rows  the streams are two row tiles that share every K/V tile.  One SM streams
+//                       about 25 bytes a clock into shared memory, 1300 clocks for the 32 KB of a
+//                       64-position tile of head_dim 128; 128 rows would give the tensor core 770
+//                       clocks of work for it, 256 rows give 1540.
+//   up to 128 rows      the streams take the even and the odd K/V tiles of the same rows, and are
+//                       joined at the end.
+// Warp 0 = bulk-copy producer, warps 1 and 2 = the streams' MMA issuers (warp 1 allocates TMEM), warps
+// 3..6 stream 0, warps 7..10 stream 1.  Each stream issues PV(u), then S(u + 2) once PV(u) has read the
+// P that it overwrites; S(u + 1) is done by then, and the other stream's MMAs fill the tensor core.
 template <typename T, int HD>
 struct PrefixTileCfg {
   static constexpr int HALVES = HD / 64;              // 64-element halves of a K / V row
   static constexpr int SUB = 16 * 128;                // one page's half sub-block (bytes)
   static constexpr int REGION = 4 * SUB;              // 64 positions of one half (bytes)
   static constexpr int TILE_BYTES = HALVES * REGION;  // K (or V) of one 64-position tile
-  static constexpr int K_STAGES = HD == 64 ? 3 : 2;
-  static constexpr int V_STAGES = HD == 64 ? 3 : 2;
+  static constexpr int STAGES = HD == 64 ? 10 : 5;    // of K and of V
   static constexpr int Q_BYTES = HALVES * 128 * 128;  // 128 rows x HD, K-major halves
-  static constexpr int SMEM = Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + 1024;
-  static constexpr uint32_t TMEM_COLS = 256;          // S/P: 2 x 64 columns, O: HD columns at 128
+  static constexpr int SMEM = 2 * Q_BYTES + 2 * STAGES * TILE_BYTES + 1024;
+  static constexpr uint32_t TMEM_COLS = 512;
   static constexpr float RESCALE_LOG2 = 8.0f;
+  static constexpr int HALF_PITCH = HD / 2 + 4;       // floats of a row of half the sums, staged
+  static_assert(2 * 128 * (HALF_PITCH * 4 + 8) <= 2 * STAGES * TILE_BYTES, "the ring holds both streams' half sums");
 };
+constexpr int kTileThreads = 352;
+constexpr int kTileRows = 256;  // score rows of a tile item
+constexpr int kColRows = 8;     // score rows of a column item
+
+__device__ __forceinline__ float ex2_approx(float x) {  // 2 ulp; 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// Bounded wait that polls without suspending the thread.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kMaxWaitPolls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+// One lane of a converged warp, chosen so that the compiler keeps warp-uniform operands in uniform
+// registers (a branch on lane == 0 moved every descriptor across per MMA: 75 clocks each).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void streams_bar() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixParams p) {
   using Cfg = PrefixTileCfg<T, HD>;
-  constexpr int KS = Cfg::K_STAGES, VS = Cfg::V_STAGES;
+  constexpr int ST = Cfg::STAGES;
   constexpr int HALVES = Cfg::HALVES;
   constexpr int SUB = Cfg::SUB;
   constexpr int REGION = Cfg::REGION;
@@ -360,49 +448,52 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
   constexpr uint32_t V_LBO = HALVES > 1 ? REGION : 1024;  // with one half never applied
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], p_ready[2],
-      pv_done, q_ready, drain;
+  __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2][2], p_ready[2][2],
+      pv_done[2], q_ready, drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int2 s_last[4];
+  __shared__ int2 s_last[8];
 
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_s = sbase;
-  const uint32_t k_ring = q_s + Cfg::Q_BYTES;
-  const uint32_t v_ring = k_ring + KS * Cfg::TILE_BYTES;
+  const uint32_t k_ring = q_s + 2 * Cfg::Q_BYTES;
+  const uint32_t v_ring = k_ring + ST * Cfg::TILE_BYTES;
   uint8_t* const gbase = smem_raw + (sbase - smem_u32(smem_raw));  // generic pointer of sbase
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
   const int kvh = blockIdx.x % p.n_kv_heads;
   const int group = p.n_heads / p.n_kv_heads;
-  // warps 2..5: this thread's score row (TMEM lane) and the last position it sees
+  const bool pair = it.n_rho > 128;  // two row tiles; otherwise even and odd K/V tiles
+  // warps 3..10: stream, TMEM lane, score row and the last position it sees
+  const int sg = warp >= 7 ? 1 : 0;
   const int tl = (warp & 3) * 32 + lane;
-  const bool row_ok = warp >= 2 && tl < it.n_rho;
-  const int rho = it.rho0 + (row_ok ? tl : 0);
+  const int local = pair ? sg * 128 + tl : tl;
+  const bool row_ok = warp >= 3 && local < it.n_rho;
+  const int rho = it.rho0 + (row_ok ? local : 0);
   const int row = it.row0 + rho / group, head = kvh * group + rho % group;
   int seq = 0;
   const int lim_row = row_ok ? row_last(p, row, seq) : -1;
-  if (warp >= 2) {
+  if (warp >= 3) {
     const int m = __reduce_max_sync(0xffffffffu, lim_row);
     const int from = __ffs(__ballot_sync(0xffffffffu, lim_row == m)) - 1;
-    if (lane == from) s_last[warp & 3] = make_int2(m, seq);
+    if (lane == from) s_last[warp - 3] = make_int2(m, seq);
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < KS; ++s) {
+    for (int s = 0; s < ST; ++s) {
       mbar_init(smem_u32(&k_full[s]), 1);
-      mbar_init(smem_u32(&k_empty[s]), 1);
-    }
-    for (int s = 0; s < VS; ++s) {
+      mbar_init(smem_u32(&k_empty[s]), pair ? 2 : 1);
       mbar_init(smem_u32(&v_full[s]), 1);
-      mbar_init(smem_u32(&v_empty[s]), 1);
+      mbar_init(smem_u32(&v_empty[s]), pair ? 2 : 1);
     }
-    mbar_init(smem_u32(&s_full[0]), 1);
-    mbar_init(smem_u32(&s_full[1]), 1);
-    mbar_init(smem_u32(&p_ready[0]), 128);
-    mbar_init(smem_u32(&p_ready[1]), 128);
-    mbar_init(smem_u32(&pv_done), 1);
-    mbar_init(smem_u32(&q_ready), 128);
-    mbar_init(smem_u32(&drain), 1);
+    for (int g = 0; g < 2; ++g) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(smem_u32(&s_full[g][b]), 1);
+        mbar_init(smem_u32(&p_ready[g][b]), 128);
+      }
+      mbar_init(smem_u32(&pv_done[g]), 1);
+    }
+    mbar_init(smem_u32(&q_ready), 256);
+    mbar_init(smem_u32(&drain), 2);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -419,13 +510,15 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
   // the sequence that sees furthest names the pages (an idle one's row may be empty)
   int2 far = s_last[0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w)
+  for (int w = 1; w < 8; ++w)
     if (s_last[w].x > far.x) far = s_last[w];
   const int last = far.x;
   const int end = min(it.pos1, last + 1);  // positions [it.pos0, end) are read
   const int nkv = end > it.pos0 ? (end - it.pos0 + 63) >> 6 : 0;
   const int page0 = it.pos0 >> 4;
   const int n_pages_it = nkv > 0 ? ((end + 15) >> 4) - page0 : 0;
+  // steps of each stream; step u of stream g works on K/V tile (pair ? u : 2 u + g)
+  const int n0 = pair ? nkv : (nkv + 1) >> 1, n1 = pair ? nkv : nkv >> 1;
   bool failed = false;
 
   if (warp == 0) {
@@ -438,19 +531,16 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
       return pg < n_pages_it ? page_entry(p, bt, pg) : 0;
     };
     int ent = entries(0), ent_next = entries(32);
-    // one tile of K (v = 0) or V (v = 1): its pages' half sub-blocks into one ring stage
+    // one tile of K (v = 0) or V (v = 1): its pages' half sub-blocks into one ring stage, a lane each
     auto load = [&](int t, int v, uint32_t dst, uint32_t bar) {
       const int np = min(4, n_pages_it - 4 * t);
-      int phys[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) phys[j] = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + j);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, np * HALVES * SUB);
-        for (int j = 0; j < np; ++j) {
-          const uint8_t* blk = p.pool + (static_cast<size_t>(phys[j]) * p.n_kv_heads + kvh) * (2 * 16 * ROWB) + v * 16 * ROWB;
-          for (int hh = 0; hh < HALVES; ++hh) bulk_g2s(dst + hh * REGION + j * SUB, blk + hh * SUB, SUB, bar);
-        }
-      }
+      const int j = lane / HALVES, hh = lane % HALVES;
+      const int phys = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + (j & 3));
+      if (lane == 0) mbar_arrive_expect_tx(bar, np * HALVES * SUB);
+      __syncwarp();
+      if (j < np)
+        bulk_g2s(dst + hh * REGION + j * SUB,
+                 p.pool + (static_cast<size_t>(phys) * p.n_kv_heads + kvh) * (2 * 16 * ROWB) + v * 16 * ROWB + hh * SUB, SUB, bar);
     };
     int k_issued = 0, v_issued = 0;
     for (int t = 0; t < nkv; ++t) {
@@ -458,111 +548,141 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
         ent = ent_next;
         ent_next = entries(4 * t + 32);
       }
-      if (t >= KS && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&k_empty[t % KS]), ((t / KS) + 1) & 1))) {
+      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&k_empty[t % ST]), ((t / ST) + 1) & 1))) {
         failed = true;
         break;
       }
-      load(t, 0, k_ring + (t % KS) * Cfg::TILE_BYTES, smem_u32(&k_full[t % KS]));
+      load(t, 0, k_ring + (t % ST) * Cfg::TILE_BYTES, smem_u32(&k_full[t % ST]));
       k_issued = t + 1;
-      if (t >= VS && !__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&v_empty[t % VS]), ((t / VS) + 1) & 1))) {
+      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&v_empty[t % ST]), ((t / ST) + 1) & 1))) {
         failed = true;
         break;
       }
-      load(t, 1, v_ring + (t % VS) * Cfg::TILE_BYTES, smem_u32(&v_full[t % VS]));
+      load(t, 1, v_ring + (t % ST) * Cfg::TILE_BYTES, smem_u32(&v_full[t % ST]));
       v_issued = t + 1;
     }
     // copies still in flight must land before the CTA's shared memory goes away
     if (lane == 0) {
-      for (int t = max(0, k_issued - KS); t < k_issued; ++t) mbar_wait_bounded(smem_u32(&k_full[t % KS]), (t / KS) & 1);
-      for (int t = max(0, v_issued - VS); t < v_issued; ++t) mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1);
+      for (int t = max(0, k_issued - ST); t < k_issued; ++t) mbar_poll(smem_u32(&k_full[t % ST]), (t / ST) & 1);
+      for (int t = max(0, v_issued - ST); t < v_issued; ++t) mbar_poll(smem_u32(&v_full[t % ST]), (t / ST) & 1);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = umma_idesc<T>(128, 64);
-      constexpr uint32_t idesc_pv = umma_idesc<T>(128, HD) | (1u << 16);  // B (V) MN-major
-      const uint32_t o_tmem = tmem + 128;
-      // S_t into TMEM columns (t & 1) * 64; frees the K stage when the MMAs complete
-      auto issue_s = [&](int t) -> bool {
-        const int s = t % KS;
-        if (!mbar_wait_bounded(smem_u32(&k_full[s]), (t / KS) & 1)) return false;
-        tc_fence_after();
-        const uint32_t kst = k_ring + s * Cfg::TILE_BYTES;
-        const uint32_t d = tmem + (t & 1) * 64;
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------ MMA issuer of stream warp - 1
+    const int g = warp - 1;
+    const int steps = __shfl_sync(0xffffffffu, g ? n1 : n0, 0);
+    const uint32_t tbase = __shfl_sync(0xffffffffu, tmem, 0) + g * 256;
+    constexpr uint32_t idesc_s = umma_idesc<T>(128, 64);
+    constexpr uint32_t idesc_pv = umma_idesc<T>(128, HD) | (1u << 16);  // B (V) MN-major
+    const uint64_t qd = sw128_desc(q_s + (pair ? g * Cfg::Q_BYTES : 0));
+    const uint64_t kd0 = sw128_desc(k_ring), vd0 = sw128_desc_mn(v_ring, V_LBO, 1024);
+    // S of step u into the stream's buffer u & 1, whose P the stream's PV(u - 2) has read
+    auto issue_s = [&](int u) -> bool {
+      const int t = pair ? u : 2 * u + g, s = t % ST;
+      bool ok = u < 2 || mbar_poll(smem_u32(&pv_done[g]), u & 1);
+      ok = ok && mbar_poll(smem_u32(&k_full[s]), (t / ST) & 1);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      const uint64_t kd = kd0 + static_cast<uint64_t>(s * (Cfg::TILE_BYTES >> 4));
+      const uint32_t d = tbase + (u & 1) * 64;
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const int hh = k >> 2, kk = k & 3;
-          umma<false>(d, sw128_desc(q_s + hh * 128 * 128 + 32 * kk), sw128_desc(kst + hh * REGION + 32 * kk), idesc_s,
-                      k > 0 ? 1u : 0u);
+          umma<false>(d, qd + ((hh * 128 * 128 + 32 * kk) >> 4), kd + ((hh * REGION + 32 * kk) >> 4), idesc_s, k > 0 ? 1u : 0u);
         }
+        tc_commit(smem_u32(&s_full[g][u & 1]));
         tc_commit(smem_u32(&k_empty[s]));
-        tc_commit(smem_u32(&s_full[t & 1]));
-        return true;
-      };
-      bool ok = mbar_wait_bounded(smem_u32(&q_ready), 0);
-      if (ok && nkv > 0) ok = issue_s(0);
-      if (ok && nkv > 1) ok = issue_s(1);
-      for (int t = 0; ok && t < nkv; ++t) {
-        if (!mbar_wait_bounded(smem_u32(&p_ready[t & 1]), (t >> 1) & 1) ||
-            !mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t vst = v_ring + (t % VS) * Cfg::TILE_BYTES;
-        const uint32_t pa = tmem + (t & 1) * 64;  // P_hi at +0, P_lo at +32 (16-bit pairs)
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](int u) -> bool {
+      const int t = pair ? u : 2 * u + g, s = t % ST;
+      bool ok = mbar_poll(smem_u32(&v_full[s]), (t / ST) & 1);
+      ok = ok && mbar_poll(smem_u32(&p_ready[g][u & 1]), (u >> 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      const uint64_t vd = vd0 + static_cast<uint64_t>(s * (Cfg::TILE_BYTES >> 4));
+      const uint32_t pa = tbase + (u & 1) * 64;  // P_hi at +0, P_lo at +32 (16-bit pairs)
+      if (elect_one()) {
 #pragma unroll
         for (int term = 0; term < 2; ++term) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 16 positions per MMA
-            umma_ts(o_tmem, pa + term * 32 + kk * 8, sw128_desc_mn(vst + kk * 2048, V_LBO, 1024), idesc_pv,
-                    (t > 0 || term > 0 || kk > 0) ? 1u : 0u);
+            umma_ts(tbase + 128, pa + term * 32 + kk * 8, vd + ((kk * 2048) >> 4), idesc_pv, (u > 0 || term > 0 || kk > 0) ? 1u : 0u);
         }
-        tc_commit(smem_u32(&v_empty[t % VS]));
-        tc_commit(smem_u32(&pv_done));
-        if (t + 2 < nkv) {
-          // S_{t+2} overwrites the columns P_t is read from: PV_t must be complete
-          if (!mbar_wait_bounded(smem_u32(&pv_done), t & 1)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          ok = issue_s(t + 2);
-        }
+        tc_commit(smem_u32(&pv_done[g]));
+        tc_commit(smem_u32(&v_empty[s]));
       }
-      if (!ok) failed = true;
-      // every MMA this thread issued has completed before O is read and TMEM is freed
-      tc_commit(smem_u32(&drain));
-      mbar_wait_bounded(smem_u32(&drain), 0);
+      __syncwarp();
+      return true;
+    };
+    bool ok = __all_sync(0xffffffffu, mbar_poll(smem_u32(&q_ready), 0));
+    if (ok && steps > 0) ok = issue_s(0);
+    if (ok && steps > 1) ok = issue_s(1);
+    for (int u = 0; ok && u < steps; ++u) {
+      ok = issue_pv(u);
+      if (ok && u + 2 < steps) ok = issue_s(u + 2);
     }
+    if (!ok) failed = true;
+    // every MMA of this stream has completed before O is read and TMEM is freed
+    if (elect_one()) tc_commit(smem_u32(&drain));
+    __syncwarp();
+    mbar_poll(smem_u32(&drain), 0);
   } else {
     // ------------------------------------------------------------ softmax / epilogue warps
     const int lim = min(lim_row, end - 1);     // last visible position of this row in the range
-    const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const bool busy = __any_sync(0xffffffffu, row_ok);  // some row of this warp is the item's
+    const uint32_t trow = tmem + sg * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 
     // Q row -> shared memory, K-major 128B-swizzled halves
-    {
+    if (pair || sg == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head);
+      uint8_t* dst = gbase + sg * Cfg::Q_BYTES + tl * 128;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c) {
         const uint4 v = row_ok ? src[c] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(gbase + (c >> 3) * 128 * 128 + tl * 128 + (((c & 7) ^ (tl & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (tl & 7)) << 4)) = v;
       }
       fence_proxy_async_smem();
-      mbar_arrive(smem_u32(&q_ready));
     }
+    mbar_arrive(smem_u32(&q_ready));
 
     const float sl2 = p.scale_log2;
     float m_ref = -INFINITY, l_run = 0.f;
     bool ok = true;
-    for (int t = 0; t < nkv; ++t) {
+    const int steps = sg ? n1 : n0;
+    for (int u = 0; u < steps; ++u) {
+      const int t = pair ? u : 2 * u + sg;
       // wait results are made warp-uniform: the TMEM accesses below are warp-collective
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&s_full[t & 1]), (t >> 1) & 1))) {
+      if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&s_full[sg][u & 1]), (u >> 1) & 1))) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t scol = trow + (t & 1) * 64;
+      const int kbase = it.pos0 + t * 64;
+      // V rows past the range were not loaded (or belong to nobody): zero them so a zero weight
+      // times stale data cannot make NaN (only the last tile is ragged; its V copies land first).
+      // Both streams of a pair do it, each before its own PV.
+      const int valid = end - kbase;
+      if (valid < 64) {
+        if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&v_full[t % ST]), (t / ST) & 1))) {
+          ok = false;
+          break;
+        }
+        uint8_t* vreg = gbase + (v_ring - sbase) + (t % ST) * Cfg::TILE_BYTES;
+        for (int idx = tl; idx < (64 - valid) * HALVES * 8; idx += 128) {
+          const int rr = valid + idx / (HALVES * 8), rem = idx % (HALVES * 8);
+          *reinterpret_cast<uint4*>(vreg + (rem >> 3) * REGION + rr * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      if (!busy) {  // the lanes' P is never read back: whatever S left there is as good
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_ready[sg][u & 1]));
+        continue;
+      }
+      const uint32_t scol = trow + (u & 1) * 64;
       float sv[64];
       {
         uint32_t ra[32], rb[32];
@@ -575,7 +695,6 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
           sv[32 + j] = __uint_as_float(rb[j]);
         }
       }
-      const int kbase = it.pos0 + t * 64;
       if (__any_sync(0xffffffffu, kbase + 63 > lim)) {
 #pragma unroll
         for (int j = 0; j < 64; ++j)
@@ -592,7 +711,7 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
       const bool move = mx > m_ref + Cfg::RESCALE_LOG2;
       const float m_new = move ? mx : m_ref;
       const float mu = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = move ? exp2_det_lo(m_ref - mu) : 1.0f;
+      const float alpha = move ? ex2_approx(m_ref - mu) : 1.0f;
       float2 r4[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) r4[k] = make_float2(0.f, 0.f);
@@ -600,7 +719,8 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
         const float2 sl22 = make_float2(sl2, sl2), nmu = make_float2(-mu, -mu);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float2 pe = exp2_det_lo2(fma2_rn(make_float2(sv[2 * e], sv[2 * e + 1]), sl22, nmu));
+          const float2 x = fma2_rn(make_float2(sv[2 * e], sv[2 * e + 1]), sl22, nmu);
+          const float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           sv[2 * e] = pe.x;
           sv[2 * e + 1] = pe.y;
           r4[e & 3] = add2_rn(r4[e & 3], pe);
@@ -609,9 +729,9 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
       l_run = l_run * alpha + (((r4[0].x + r4[0].y) + (r4[1].x + r4[1].y)) + ((r4[2].x + r4[2].y) + (r4[3].x + r4[3].y)));
       m_ref = m_new;
 
-      // O holds PV of tiles < t: rescale rows whose reference moved, after PV_{t-1} completed
-      if (t > 0 && __any_sync(0xffffffffu, move)) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&pv_done), (t - 1) & 1))) {
+      // O holds PV of steps < u: rescale rows whose reference moved, after PV(u - 1) completed
+      if (u > 0 && __any_sync(0xffffffffu, move)) {
+        if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&pv_done[sg]), (u - 1) & 1))) {
           ok = false;
           break;
         }
@@ -626,95 +746,118 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
           tmem_st32(trow + 128 + c * 32, r);
         }
       }
-      // V rows past the range were not loaded (or belong to nobody): zero them so a zero weight
-      // times stale data cannot make NaN (only the last tile is ragged; its V copies land first)
-      const int valid = end - kbase;
-      if (valid < 64) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&v_full[t % VS]), (t / VS) & 1))) {
-          ok = false;
-          break;
-        }
-        uint8_t* vreg = gbase + (v_ring - sbase) + (t % VS) * Cfg::TILE_BYTES;
-        for (int idx = tl; idx < (64 - valid) * HALVES * 8; idx += 128) {
-          const int rr = valid + idx / (HALVES * 8), rem = idx % (HALVES * 8);
-          *reinterpret_cast<uint4*>(vreg + (rem >> 3) * REGION + rr * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
       {
         uint32_t hi[32], lo[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float a = sv[2 * e], b = sv[2 * e + 1];
-          hi[e] = ActTraits<T>::pack2(a, b);
-          const float2 hv = ActTraits<T>::unpack2(hi[e]);
-          lo[e] = ActTraits<T>::pack2(a - hv.x, b - hv.y);
+          const float2 pe = make_float2(sv[2 * e], sv[2 * e + 1]);
+          hi[e] = ActTraits<T>::pack2(pe.x, pe.y);
+          const float2 rest = sub2_rn(pe, ActTraits<T>::unpack2(hi[e]));
+          lo[e] = ActTraits<T>::pack2(rest.x, rest.y);
         }
         tmem_st32(scol, hi);
         tmem_st32(scol + 32, lo);
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&p_ready[t & 1]));
+      mbar_arrive(smem_u32(&p_ready[sg][u & 1]));
     }
     if (ok) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&drain), 0));
+      ok = __all_sync(0xffffffffu, mbar_poll(smem_u32(&drain), 0));
       tc_fence_after();
     }
     if (!ok) {
       failed = true;
-      m_ref = -INFINITY;  // contributes nothing
-      l_run = 0.f;
+      l_run = 0.f;  // contributes nothing
     }
-    if (l_run == 0.f) m_ref = -INFINITY;
-    const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
-    const size_t rho_all = static_cast<size_t>(it.row0) * group + rho;
-    const bool has = m_ref > -INFINITY;  // O of a row that saw nothing is not read
-    if (!p.final) {
-      const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
-      if (row_ok) __stcg(p.ws_ml + at, make_float2(m_ref, l_run));
+    if (l_run == 0.f) m_ref = -INFINITY;  // O of a row that saw nothing is not read
+
+    // This thread's columns of the row's sum, 32 at a time: all of them for a pair; otherwise a
+    // half, the streams having exchanged the other halves through the idle ring.
+    const int chunks = pair ? HD / 32 : HD / 64, chunk0 = pair ? 0 : sg * (HD / 64);
+    float m = m_ref, l = l_run, w_own = 1.f, w_other = 0.f;
+    float* const stage = reinterpret_cast<float*>(gbase + (k_ring - sbase));
+    float2* const s_ml = reinterpret_cast<float2*>(stage + 2 * 128 * Cfg::HALF_PITCH);  // [2][128]
+    if (!pair) {
+      float* mine = stage + (sg * 128 + tl) * Cfg::HALF_PITCH;  // the half that the other stream keeps
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; c < HD / 64; ++c) {
         uint32_t r[32];
-        tmem_ld32(trow + 128 + c * 32, r);
+        tmem_ld32(trow + 128 + ((1 - sg) * (HD / 64) + c) * 32, r);
         tmem_wait_ld();
-        if (!row_ok || !has) continue;
-        float4* dst = reinterpret_cast<float4*>(p.ws_o + at * HD + c * 32);
 #pragma unroll
         for (int j = 0; j < 32; j += 4)
-          __stcg(dst + j / 4, make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
-                                          __uint_as_float(r[j + 3])));
+          *reinterpret_cast<float4*>(mine + c * 32 + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                                                                      __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+      }
+      s_ml[sg * 128 + tl] = make_float2(m_ref, l_run);
+      streams_bar();
+      const float2 ml = s_ml[(1 - sg) * 128 + tl];
+      m = fmaxf(m_ref, ml.x);
+      const float mu = m == -INFINITY ? 0.f : m;
+      w_own = ex2_approx(m_ref - mu);
+      w_other = ex2_approx(ml.x - mu);
+      l = l_run * w_own + ml.y * w_other;
+    }
+    const float* theirs = stage + ((1 - sg) * 128 + tl) * Cfg::HALF_PITCH;
+    const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
+    const size_t rho_all = static_cast<size_t>(it.row0) * group + rho;
+    const bool first = pair || sg == 0;  // of the threads that hold a row, the one that stores m, l, lse
+    auto sums = [&](int c, float (&o)[32]) {  // w_own * own + w_other * other of columns 32 (chunk0 + c) ..
+      uint32_t r[32];
+      tmem_ld32(trow + 128 + (chunk0 + c) * 32, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = w_own > 0.f && l_run > 0.f ? __uint_as_float(r[j]) * w_own : 0.f;
+      if (!pair && w_other > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(theirs + c * 32 + j);
+          o[j] += v.x * w_other;
+          o[j + 1] += v.y * w_other;
+          o[j + 2] += v.z * w_other;
+          o[j + 3] += v.w * w_other;
+        }
+      }
+    };
+    if (!p.final) {
+      const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
+      if (row_ok && first) __stcg(p.ws_ml + at, make_float2(m, l));
+      for (int c = 0; c < chunks; ++c) {
+        float o[32];
+        sums(c, o);
+        if (!row_ok || l == 0.f) continue;
+        float4* dst = reinterpret_cast<float4*>(p.ws_o + at * HD + (chunk0 + c) * 32);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) __stcg(dst + j / 4, make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
       }
     } else {
       griddep_wait();
-      float M = m_ref;
+      float M = m;
       if (row_ok)
         for (int k = 0; k < it.part; ++k)
           M = fmaxf(M, __ldcg(&p.ws_ml[(static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all].x));
       const float mu = M == -INFINITY ? 0.f : M;
-      const float w0 = exp2_det_lo(m_ref - mu);
-      float L = l_run * w0;
+      const float w0 = ex2_approx(m - mu);
+      float L = l * w0;
       if (row_ok)
         for (int k = 0; k < it.part; ++k) {
           const float2 ml = __ldcg(p.ws_ml + (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all);
-          if (ml.x > -INFINITY) L += ml.y * exp2_det_lo(ml.x - mu);
+          if (ml.x > -INFINITY) L += ml.y * ex2_approx(ml.x - mu);
         }
       const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(trow + 128 + c * 32, r);
-        tmem_wait_ld();
-        if (!row_ok) continue;
+      for (int c = 0; c < chunks; ++c) {
         float o[32];
+        sums(c, o);
+        if (!row_ok) continue;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = has ? __uint_as_float(r[j]) * w0 : 0.f;
+        for (int j = 0; j < 32; ++j) o[j] *= w0;
         for (int k = 0; k < it.part; ++k) {
           const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all;
-          const float m = __ldcg(&p.ws_ml[at].x);
-          if (m == -INFINITY) continue;
-          const float w = exp2_det_lo(m - mu);
-          const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * HD + c * 32);
+          const float mk = __ldcg(&p.ws_ml[at].x);
+          if (mk == -INFINITY) continue;
+          const float w = ex2_approx(mk - mu);
+          const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * HD + (chunk0 + c) * 32);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 v = __ldcg(src + j / 4);
@@ -724,7 +867,7 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
             o[j + 3] += v.w * w;
           }
         }
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + c * 32);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + (chunk0 + c) * 32);
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           uint4 v;
@@ -735,7 +878,7 @@ __global__ void __launch_bounds__(192, 2) prefix_tile_kernel(PrefixParams p) {
           dst[j / 8] = v;
         }
       }
-      if (p.lse && row_ok) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+      if (p.lse && row_ok && first) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
     }
   }
   if (failed) page_fail(p.status, kDevWaitTimeout);

@@ -224,8 +224,6 @@ struct llm_prefix_plan {
 namespace {
 
 enum { kPart = 0, kFinal = 1, kTile = 0, kCols = 1 };
-constexpr int kTileRows = 128;   // score rows of a tile item
-constexpr int kColRows = 8;      // score rows of a column item
 constexpr int kMaxParts = 64;    // states a row may have to join
 constexpr int kOpenEnd = 1 << 30;
 // Cost of starting and ending a CTA, in 64-position steps of its main loop.
@@ -237,7 +235,7 @@ struct PlanGroup {
   long long rho;  // score rows per kv head
 };
 
-int kernel_slots(int kind, int head_dim) { return 148 * (kind == kTile ? 2 : head_dim == 64 ? 5 : 3); }
+int kernel_slots(int kind, int head_dim) { return 148 * (kind == kTile ? 1 : head_dim == 64 ? 5 : 3); }
 
 // Positions per part item of the shared prefixes: a multiple of 64 that finishes first when every
 // CTA slot takes ceil(items / slots) items of that length.
@@ -347,8 +345,8 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
       cudaError_t e;
       if (kind == kTile) {
         constexpr int smem = PrefixTileCfg<T, HD>::SMEM;
-        if (first) prefix_tile_kernel<T, HD><<<grid, 192, smem, s>>>(p), e = cudaGetLastError();
-        else e = launch_dependent(prefix_tile_kernel<T, HD>, grid, dim3(192), smem, s, p);
+        if (first) prefix_tile_kernel<T, HD><<<grid, kTileThreads, smem, s>>>(p), e = cudaGetLastError();
+        else e = launch_dependent(prefix_tile_kernel<T, HD>, grid, dim3(kTileThreads), smem, s, p);
       } else {
         constexpr int smem = AttnCfg<T, HD>::SMEM;
         if (first) prefix_cols_kernel<T, HD><<<grid, kAttnWarps * 32, smem, s>>>(p), e = cudaGetLastError();
