@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
 //                       clocks of work for it, 256 rows give 1540.
 //   up to 128 rows      the streams take the even and the odd K/V tiles of the same rows, and are
 //                       joined at the end.
-// Warp 0 = bulk-copy producer, warps 1 and 2 = the streams' MMA issuers (warp 1 allocates TMEM), warps
+// Warps 0 and 11 = bulk-copy producers, warps 1 and 2 = the streams' MMA issuers (warp 1 allocates TMEM), warps
 // 3..6 stream 0, warps 7..10 stream 1.  Each stream issues PV(u), then S(u + 2) once PV(u) has read the
 // P that it overwrites; S(u + 1) is done by then, and the other stream's MMAs fill the tensor core.
 template <typename T, int HD>
@@ -406,7 +406,7 @@ struct PrefixTileCfg {
   static constexpr int HALF_PITCH = HD / 2 + 4;       // floats of a row of half the sums, staged
   static_assert(2 * 128 * (HALF_PITCH * 4 + 8) <= 2 * STAGES * TILE_BYTES, "the ring holds both streams' half sums");
 };
-constexpr int kTileThreads = 352;
+constexpr int kTileThreads = 384;
 constexpr int kTileRows = 256;  // score rows of a tile item
 constexpr int kColRows = 8;     // score rows of a column item
 
@@ -445,7 +445,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
   constexpr int SUB = Cfg::SUB;
   constexpr int REGION = Cfg::REGION;
   constexpr int ROWB = HD * (int)sizeof(T);
-  constexpr uint32_t V_LBO = HALVES > 1 ? REGION : 1024;  // with one half never applied
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2][2], p_ready[2][2],
@@ -468,12 +467,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
   const int sg = warp >= 7 ? 1 : 0;
   const int tl = (warp & 3) * 32 + lane;
   const int local = pair ? sg * 128 + tl : tl;
-  const bool row_ok = warp >= 3 && local < it.n_rho;
+  const bool softmax_warp = warp >= 3 && warp <= 10;
+  const bool row_ok = softmax_warp && local < it.n_rho;
   const int rho = it.rho0 + (row_ok ? local : 0);
   const int row = it.row0 + rho / group, head = kvh * group + rho % group;
   int seq = 0;
   const int lim_row = row_ok ? row_last(p, row, seq) : -1;
-  if (warp >= 3) {
+  if (softmax_warp) {
     const int m = __reduce_max_sync(0xffffffffu, lim_row);
     const int from = __ffs(__ballot_sync(0xffffffffu, lim_row == m)) - 1;
     if (lane == from) s_last[warp - 3] = make_int2(m, seq);
@@ -521,51 +521,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
   const int n0 = pair ? nkv : (nkv + 1) >> 1, n1 = pair ? nkv : nkv >> 1;
   bool failed = false;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ bulk-copy producer
-    // The whole warp reads the block table, 32 pages (8 tiles) per coalesced load, one batch
-    // ahead of use; lane 0 issues the copies.  Waits run on every lane and are made uniform.
+  if (warp == 0 || warp == 11) {
+    // ------------------------------------------------------------ bulk-copy producers
+    // Warp 0 fetches K, warp 11 V (one warp issues a copy each 50 to 80 clocks).  A warp reads the
+    // block table 32 pages (8 tiles) per coalesced load, one batch ahead of use, and a lane issues
+    // each copy: a page's half sub-block of K, both halves of V at once.
+    const bool is_v = warp == 11;
+    const uint32_t ring = is_v ? v_ring : k_ring;
+    const uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    const int per_page = is_v ? 1 : HALVES, size = is_v ? HALVES * SUB : SUB;
+    const int j = lane / per_page, hh = lane % per_page;
+    const uint32_t place = is_v ? j * HALVES * SUB : hh * REGION + j * SUB;
+    const uint8_t* const src = p.pool + static_cast<size_t>(kvh) * (2 * 16 * ROWB) + (is_v ? 16 * ROWB : hh * SUB);
     const int* bt = p.table + static_cast<size_t>(p.slots[far.y]) * p.max_pages + page0;
     auto entries = [&](int first_page) -> int {
       const int pg = first_page + lane;
       return pg < n_pages_it ? page_entry(p, bt, pg) : 0;
     };
     int ent = entries(0), ent_next = entries(32);
-    // one tile of K (v = 0) or V (v = 1): its pages' half sub-blocks into one ring stage, a lane each
-    auto load = [&](int t, int v, uint32_t dst, uint32_t bar) {
-      const int np = min(4, n_pages_it - 4 * t);
-      const int j = lane / HALVES, hh = lane % HALVES;
-      const int phys = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + (j & 3));
-      if (lane == 0) mbar_arrive_expect_tx(bar, np * HALVES * SUB);
-      __syncwarp();
-      if (j < np)
-        bulk_g2s(dst + hh * REGION + j * SUB,
-                 p.pool + (static_cast<size_t>(phys) * p.n_kv_heads + kvh) * (2 * 16 * ROWB) + v * 16 * ROWB + hh * SUB, SUB, bar);
-    };
-    int k_issued = 0, v_issued = 0;
+    int issued = 0;
     for (int t = 0; t < nkv; ++t) {
       if (t > 0 && (t & 7) == 0) {
         ent = ent_next;
         ent_next = entries(4 * t + 32);
       }
-      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&k_empty[t % ST]), ((t / ST) + 1) & 1))) {
+      const int st = t % ST, np = min(4, n_pages_it - 4 * t);
+      const size_t phys = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + (j & 3));
+      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&empty[st]), ((t / ST) + 1) & 1))) {
         failed = true;
         break;
       }
-      load(t, 0, k_ring + (t % ST) * Cfg::TILE_BYTES, smem_u32(&k_full[t % ST]));
-      k_issued = t + 1;
-      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&v_empty[t % ST]), ((t / ST) + 1) & 1))) {
-        failed = true;
-        break;
-      }
-      load(t, 1, v_ring + (t % ST) * Cfg::TILE_BYTES, smem_u32(&v_full[t % ST]));
-      v_issued = t + 1;
+      const uint32_t bar = smem_u32(&full[st]);
+      if (lane == 0) mbar_arrive_expect_tx(bar, np * HALVES * SUB);
+      __syncwarp();
+      if (j < np) bulk_g2s(ring + st * Cfg::TILE_BYTES + place, src + phys * p.n_kv_heads * (2 * 16 * ROWB), size, bar);
+      issued = t + 1;
     }
     // copies still in flight must land before the CTA's shared memory goes away
-    if (lane == 0) {
-      for (int t = max(0, k_issued - ST); t < k_issued; ++t) mbar_poll(smem_u32(&k_full[t % ST]), (t / ST) & 1);
-      for (int t = max(0, v_issued - ST); t < v_issued; ++t) mbar_poll(smem_u32(&v_full[t % ST]), (t / ST) & 1);
-    }
+    if (lane == 0)
+      for (int t = max(0, issued - ST); t < issued; ++t) mbar_poll(smem_u32(&full[t % ST]), (t / ST) & 1);
   } else if (warp <= 2) {
     // ------------------------------------------------------------ MMA issuer of stream warp - 1
     const int g = warp - 1;
@@ -574,7 +568,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     constexpr uint32_t idesc_s = umma_idesc<T>(128, 64);
     constexpr uint32_t idesc_pv = umma_idesc<T>(128, HD) | (1u << 16);  // B (V) MN-major
     const uint64_t qd = sw128_desc(q_s + (pair ? g * Cfg::Q_BYTES : 0));
-    const uint64_t kd0 = sw128_desc(k_ring), vd0 = sw128_desc_mn(v_ring, V_LBO, 1024);
+    const uint64_t kd0 = sw128_desc(k_ring), vd0 = sw128_desc_mn(v_ring, SUB, 1024);
     // S of step u into the stream's buffer u & 1, whose P the stream's PV(u - 2) has read
     auto issue_s = [&](int u) -> bool {
       const int t = pair ? u : 2 * u + g, s = t % ST;
@@ -609,7 +603,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
         for (int term = 0; term < 2; ++term) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 16 positions per MMA
-            umma_ts(tbase + 128, pa + term * 32 + kk * 8, vd + ((kk * 2048) >> 4), idesc_pv, (u > 0 || term > 0 || kk > 0) ? 1u : 0u);
+            umma_ts(tbase + 128, pa + term * 32 + kk * 8, vd + ((kk * HALVES * SUB) >> 4), idesc_pv, (u > 0 || term > 0 || kk > 0) ? 1u : 0u);
         }
         tc_commit(smem_u32(&pv_done[g]));
         tc_commit(smem_u32(&v_empty[s]));
@@ -673,7 +667,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
         uint8_t* vreg = gbase + (v_ring - sbase) + (t % ST) * Cfg::TILE_BYTES;
         for (int idx = tl; idx < (64 - valid) * HALVES * 8; idx += 128) {
           const int rr = valid + idx / (HALVES * 8), rem = idx % (HALVES * 8);
-          *reinterpret_cast<uint4*>(vreg + (rem >> 3) * REGION + rr * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vreg + ((rr >> 4) * HALVES + (rem >> 3)) * SUB + (rr & 15) * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
