@@ -7,17 +7,15 @@
 // A row that sees nothing (ctx 0, or a row before position 0) gives o = 0 and lse = -inf.
 //
 // The plan cuts the work into items, each a run of score rows (query row, head of the kv head's
-// group) against a run of positions of one block-table row, for every kv head:
-//   part items   the shared positions of a group, all of the group's rows stacked, so a shared
-//                page is read once per 256 score rows; and pieces of a long own range.  They
-//                leave the state of each row in the workspace.
-//   final items  a sequence's own positions (the rest after the parts).  They join the row's
-//                part states to their own and write the output.
-// Two kernels take items of either kind: prefix_tile_kernel up to 256 score rows on the tcgen05
-// tensor cores, prefix_cols_kernel up to 8 on warp-level MMAs (eight columns cost it nothing, and
-// its CTAs need no tensor memory and a third of the registers).  The part launches come first;
-// the final launches start beside them (programmatic dependent launch), stream their own pages, and
-// wait for the parts only before they join.
+// group) against a run of positions of one block-table row, for every kv head: the shared
+// positions of a group with all of the group's rows stacked, so that a shared page is read once
+// per 256 score rows, each sequence's own positions, and pieces of long ranges.  An item that
+// covers all positions of its rows writes the output; the others leave the state of each row in
+// the workspace, and prefix_join_kernel joins a row's states.
+// Two kernels take the items: prefix_tile_kernel up to 256 score rows on the tcgen05 tensor cores,
+// prefix_cols_kernel up to 8 on warp-level MMAs (eight columns cost it nothing, and several of its
+// CTAs fit an SM).  The launches run beside one another (programmatic dependent launch); the join
+// waits for all of them.
 #pragma once
 #include "attention.cuh"
 #include "common.cuh"
@@ -31,12 +29,11 @@ struct PrefixItem {
   int rho0;        // score rows rho0 .. rho0 + n_rho - 1 counted from row0's first head
   int n_rho;
   int pos0, pos1;  // positions [pos0, pos1), cut at the last one a row of the item sees
-  int part;        // part items: the state's number; final items: states to join (0 .. part - 1)
+  int part;        // number of the rows' state in the workspace; -1: the item writes the output
 };
 
 struct PrefixParams {
   const PrefixItem* items;
-  int final;                  // the items are final items
   const void* q;
   void* out;
   float* lse;                 // [rows][n_heads] natural log, or nullptr
@@ -47,6 +44,8 @@ struct PrefixParams {
   const int* ctx;             // [n_seqs]
   const int* slots;           // [n_seqs]
   const int2* row_info;       // [n_rows] sequence, rows of the sequence from this one on
+  const int2* joins;          // [n_joins] rows with several states: row, states
+  int n_joins;
   float* ws_o;                // [parts][n_kv_heads][n_rows * group][HD] unnormalised sums
   float2* ws_ml;              // [parts][n_kv_heads][n_rows * group] (m in log2 units, l)
   int* status;
@@ -288,93 +287,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
     }
   }
   __syncthreads();
-  const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
-  const size_t rho_all = static_cast<size_t>(it.row0) * group + it.rho0;
-  if (!p.final) {
-    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
+  if (it.part >= 0) {
+    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * p.n_rows * group +
+                      static_cast<size_t>(it.row0) * group + it.rho0;
     for (int i = threadIdx.x; i < it.n_rho * HD / 4; i += kAttnWarps * 32)
       __stcg(reinterpret_cast<float4*>(p.ws_o + at * HD) + i, reinterpret_cast<const float4*>(stage)[i]);
     if (threadIdx.x < it.n_rho) __stcg(p.ws_ml + at + threadIdx.x, make_float2(s_m[threadIdx.x], s_l[threadIdx.x]));
-    griddep_wait();  // whoever waits for this launch has then waited for the ones before it
-    return;
-  }
-  griddep_wait();
-  // Join.  SUB warps share a column, each taking every SUB-th state; lane k holds the weights of
-  // states k and k + 32 (kMaxParts is 64), and a lane adds its HD / 32 dimensions of eight states at
-  // a time.
-  constexpr int V = HD / 32;
-  const int share = it.n_rho == 1 ? 4 : it.n_rho == 2 ? 2 : 1;  // warps per column
-  const int sub = warp % share;
-  float* const partial = reinterpret_cast<float*>(smem);  // [4][HD]: the page ring is idle
-  for (int c0w = 0; c0w < it.n_rho; c0w += kAttnWarps / share) {
-    const int c = c0w + warp / share;
-    const bool on = c < it.n_rho;
-    float M = -INFINITY, L = 0.f, O[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) O[e] = 0.f;
-    if (on) {
-      const size_t step = static_cast<size_t>(p.n_kv_heads) * rows_all;
-      const size_t at = static_cast<size_t>(kvh) * rows_all + rho_all + c;
-      float2 a = make_float2(-INFINITY, 0.f), b = a;
-      if (lane < it.part) a = __ldcg(p.ws_ml + at + lane * step);
-      if (lane + 32 < it.part) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
-      M = fmaxf(warp_max(fmaxf(a.x, b.x)), s_m[c]);
-      const float mu = M == -INFINITY ? 0.f : M;
-      const float wa = exp2_det_lo(a.x - mu), wb = exp2_det_lo(b.x - mu), w0 = exp2_det_lo(s_m[c] - mu);
-      L = a.y * wa + b.y * wb;
-#pragma unroll
-      for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-      L += s_l[c] * w0;
-      if (sub == 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) O[e] = stage[c * HD + lane * V + e] * w0;
-      }
-      const float* src = p.ws_o + at * HD + lane * V;
-      for (int k0 = sub; k0 < it.part; k0 += 8 * share) {
-        float v[8][V], w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = k0 + i * share;
-          w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
-          if (k >= it.part) w[i] = 0.f;
-          if (w[i] > 0.f) {  // a state without visible positions holds no sums
-            if constexpr (V == 4) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(src + k * step * HD));
-              v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-            } else {
-              const float2 x = __ldcg(reinterpret_cast<const float2*>(src + k * step * HD));
-              v[i][0] = x.x, v[i][1] = x.y;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
-      }
-    }
-    if (share > 1) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) partial[warp * HD + lane * V + e] = O[e];
-      __syncthreads();
-      if (sub == 0)
-        for (int k = 1; k < share; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) O[e] += partial[(warp + k) * HD + lane * V + e];
-    }
-    if (on && sub == 0) {
+  } else {
+    for (int i = threadIdx.x; i < it.n_rho * (HD / 2); i += kAttnWarps * 32) {
+      const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
       const int row = it.row0 + (it.rho0 + c) / group, head = kvh * group + (it.rho0 + c) % group;
-      T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
-      const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-#pragma unroll
-      for (int e = 0; e < V; e += 2)
-        *reinterpret_cast<uint32_t*>(out + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
-      if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+      const float l = s_l[c], inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + d) =
+          ActTraits<T>::pack2(stage[c * HD + d] * inv, stage[c * HD + d + 1] * inv);
+      if (p.lse && d == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(s_m[c], l);
     }
   }
+  griddep_wait();  // whoever waits for this launch has then waited for the ones before it
 }
 
 // ============================================================================ up to 256 score rows
@@ -403,8 +332,9 @@ struct PrefixTileCfg {
   static constexpr int SMEM = 2 * Q_BYTES + 2 * STAGES * TILE_BYTES + 1024;
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr float RESCALE_LOG2 = 8.0f;
-  static constexpr int HALF_PITCH = HD / 2 + 4;       // floats of a row of half the sums, staged
-  static_assert(2 * 128 * (HALF_PITCH * 4 + 8) <= 2 * STAGES * TILE_BYTES, "the ring holds both streams' half sums");
+  static constexpr int ROW_BYTES = HD * 4;            // of a row's sums, staged over Q and the rings
+  static constexpr int META = 256 * (ROW_BYTES + 16);
+  static_assert(META <= 2 * Q_BYTES + 2 * STAGES * TILE_BYTES, "Q and the rings hold both streams' sums");
 };
 constexpr int kTileThreads = 384;
 constexpr int kTileRows = 256;  // score rows of a tile item
@@ -629,14 +559,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     const bool busy = __any_sync(0xffffffffu, row_ok);  // some row of this warp is the item's
     const uint32_t trow = tmem + sg * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 
-    // Q row -> shared memory, K-major 128B-swizzled halves
-    if (pair || sg == 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head);
-      uint8_t* dst = gbase + sg * Cfg::Q_BYTES + tl * 128;
+    // The warp's 32 Q rows -> shared memory, K-major 128B-swizzled halves; consecutive lanes on the
+    // chunks of a row (one row per thread took 5 us).  Of a single tile each stream brings half.
+    {
+      constexpr int CH = HD / 8, N = CH;  // 16-byte chunks of a row; loads per lane for 32 rows
+      const long long off = row * p.q_row + head * p.q_head;
+      const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
+      const int i0 = pair || sg == 0 ? 0 : N / 2, i1 = pair || sg == 1 ? N : N / 2;
+      uint4 v[N];
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = row_ok ? src[c] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * 128 * 128 + (((c & 7) ^ (tl & 7)) << 4)) = v;
+      for (int i = 0; i < N; ++i) {
+        const int rr = (i * 32 + lane) / CH, c = lane % CH;
+        const long long o = __shfl_sync(0xffffffffu, off, rr);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (i >= i0 && i < i1 && (rows_ok >> rr & 1)) v[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + o)[c];
+      }
+      uint8_t* dst = gbase + (pair ? sg * Cfg::Q_BYTES : 0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int rr = (warp & 3) * 32 + (i * 32 + lane) / CH, c = lane % CH;
+        if (i >= i0 && i < i1)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * 128 * 128 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
       }
       fence_proxy_async_smem();
     }
@@ -766,113 +709,73 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     }
     if (l_run == 0.f) m_ref = -INFINITY;  // O of a row that saw nothing is not read
 
-    // This thread's columns of the row's sum, 32 at a time: all of them for a pair; otherwise a
-    // half, the streams having exchanged the other halves through the idle ring.
-    const int chunks = pair ? HD / 32 : HD / 64, chunk0 = pair ? 0 : sg * (HD / 64);
-    float m = m_ref, l = l_run, w_own = 1.f, w_other = 0.f;
-    float* const stage = reinterpret_cast<float*>(gbase + (k_ring - sbase));
-    float2* const s_ml = reinterpret_cast<float2*>(stage + 2 * 128 * Cfg::HALF_PITCH);  // [2][128]
-    if (!pair) {
-      float* mine = stage + (sg * 128 + tl) * Cfg::HALF_PITCH;  // the half that the other stream keeps
+    // Every MMA has completed, so Q and the rings are free: the rows' sums are staged there (16-byte
+    // chunk c of a row at c ^ row, free of bank conflicts both ways) and leave a row at a time with
+    // consecutive lanes on its columns.
+    constexpr int CH = HD / 4;  // 16-byte chunks of a row's sums
+    float4* const stage = reinterpret_cast<float4*>(gbase);
+    float2* const s_ml = reinterpret_cast<float2*>(gbase + 256 * Cfg::ROW_BYTES);  // [256]
+    long long* const s_off = reinterpret_cast<long long*>(s_ml + 256);             // [256] of the output row
+    const int mine = sg * 128 + tl;
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        uint32_t r[32];
-        tmem_ld32(trow + 128 + ((1 - sg) * (HD / 64) + c) * 32, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(mine + c * 32 + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
-                                                                      __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-      }
-      s_ml[sg * 128 + tl] = make_float2(m_ref, l_run);
-      streams_bar();
-      const float2 ml = s_ml[(1 - sg) * 128 + tl];
-      m = fmaxf(m_ref, ml.x);
-      const float mu = m == -INFINITY ? 0.f : m;
-      w_own = ex2_approx(m_ref - mu);
-      w_other = ex2_approx(ml.x - mu);
-      l = l_run * w_own + ml.y * w_other;
-    }
-    const float* theirs = stage + ((1 - sg) * 128 + tl) * Cfg::HALF_PITCH;
-    const size_t rows_all = static_cast<size_t>(p.n_rows) * group;
-    const size_t rho_all = static_cast<size_t>(it.row0) * group + rho;
-    const bool first = pair || sg == 0;  // of the threads that hold a row, the one that stores m, l, lse
-    auto sums = [&](int c, float (&o)[32]) {  // w_own * own + w_other * other of columns 32 (chunk0 + c) ..
-      uint32_t r[32];
-      tmem_ld32(trow + 128 + (chunk0 + c) * 32, r);
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t v[32];
+      tmem_ld32(trow + 128 + c * 32, v);
       tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) o[j] = w_own > 0.f && l_run > 0.f ? __uint_as_float(r[j]) * w_own : 0.f;
-      if (!pair && w_other > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(theirs + c * 32 + j);
-          o[j] += v.x * w_other;
-          o[j + 1] += v.y * w_other;
-          o[j + 2] += v.z * w_other;
-          o[j + 3] += v.w * w_other;
-        }
+      for (int j = 0; j < 8; ++j)
+        stage[mine * CH + ((c * 8 + j) ^ (lane & (CH - 1)))] =
+            make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                        __uint_as_float(v[4 * j + 3]));
+    }
+    s_ml[mine] = make_float2(m_ref, l_run);
+    s_off[mine] = row * p.o_row + head * p.o_head;
+    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * p.n_rows * group +
+                      static_cast<size_t>(it.row0) * group + it.rho0;
+    if (pair) __syncwarp();
+    else streams_bar();
+    if (pair || sg == 0) {  // the thread of a row stores its state's m and l, or its lse
+      float m = m_ref, l = l_run;
+      if (!pair) {
+        const float2 other = s_ml[128 + tl];
+        m = fmaxf(m, other.x);
+        const float mu = m == -INFINITY ? 0.f : m;
+        l = l * ex2_approx(m_ref - mu) + other.y * ex2_approx(other.x - mu);
       }
-    };
-    if (!p.final) {
-      const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * rows_all + rho_all;
-      if (row_ok && first) __stcg(p.ws_ml + at, make_float2(m, l));
-      for (int c = 0; c < chunks; ++c) {
-        float o[32];
-        sums(c, o);
-        if (!row_ok || l == 0.f) continue;
-        float4* dst = reinterpret_cast<float4*>(p.ws_o + at * HD + (chunk0 + c) * 32);
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) __stcg(dst + j / 4, make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+      if (row_ok && it.part >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
+      if (row_ok && it.part < 0 && p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
+    }
+    // rows of this warp: its own 32 of a pair; 16 of the tile, from both streams, otherwise
+    const int rows_w = pair ? 32 : 16, row_w = pair ? sg * 128 + (warp & 3) * 32 : (sg * 4 + (warp & 3)) * 16;
+    const int n_w = min(rows_w, it.n_rho - row_w);
+    constexpr int PER = 32 / CH;  // rows a warp stores at once
+    const int c = lane % CH;
+#pragma unroll 4
+    for (int r0 = 0; r0 < n_w; r0 += PER) {
+      const int rr = row_w + r0 + lane / CH;
+      if (rr >= row_w + n_w) continue;
+      const float2 a = s_ml[rr];
+      float w = 1.f, m = a.x, l = a.y;
+      float4 o = stage[rr * CH + (c ^ (rr & (CH - 1)))];
+      if (!pair) {
+        const float2 b = s_ml[128 + rr];
+        m = fmaxf(a.x, b.x);
+        const float mu = m == -INFINITY ? 0.f : m;
+        w = ex2_approx(a.x - mu);
+        const float w1 = ex2_approx(b.x - mu);
+        const float4 x = stage[(128 + rr) * CH + (c ^ (rr & (CH - 1)))];
+        l = a.y * w + b.y * w1;
+        o = w > 0.f ? make_float4(o.x * w, o.y * w, o.z * w, o.w * w) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w1 > 0.f) o = make_float4(o.x + x.x * w1, o.y + x.y * w1, o.z + x.z * w1, o.w + x.w * w1);
       }
-    } else {
-      griddep_wait();
-      float M = m;
-      if (row_ok)
-        for (int k = 0; k < it.part; ++k)
-          M = fmaxf(M, __ldcg(&p.ws_ml[(static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all].x));
-      const float mu = M == -INFINITY ? 0.f : M;
-      const float w0 = ex2_approx(m - mu);
-      float L = l * w0;
-      if (row_ok)
-        for (int k = 0; k < it.part; ++k) {
-          const float2 ml = __ldcg(p.ws_ml + (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all);
-          if (ml.x > -INFINITY) L += ml.y * ex2_approx(ml.x - mu);
-        }
-      const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-      for (int c = 0; c < chunks; ++c) {
-        float o[32];
-        sums(c, o);
-        if (!row_ok) continue;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] *= w0;
-        for (int k = 0; k < it.part; ++k) {
-          const size_t at = (static_cast<size_t>(k) * p.n_kv_heads + kvh) * rows_all + rho_all;
-          const float mk = __ldcg(&p.ws_ml[at].x);
-          if (mk == -INFINITY) continue;
-          const float w = ex2_approx(mk - mu);
-          const float4* src = reinterpret_cast<const float4*>(p.ws_o + at * HD + (chunk0 + c) * 32);
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 v = __ldcg(src + j / 4);
-            o[j] += v.x * w;
-            o[j + 1] += v.y * w;
-            o[j + 2] += v.z * w;
-            o[j + 3] += v.w * w;
-          }
-        }
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + (chunk0 + c) * 32);
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint4 v;
-          v.x = ActTraits<T>::pack2(o[j] * inv, o[j + 1] * inv);
-          v.y = ActTraits<T>::pack2(o[j + 2] * inv, o[j + 3] * inv);
-          v.z = ActTraits<T>::pack2(o[j + 4] * inv, o[j + 5] * inv);
-          v.w = ActTraits<T>::pack2(o[j + 6] * inv, o[j + 7] * inv);
-          dst[j / 8] = v;
-        }
+      if (it.part >= 0) {
+        if (l > 0.f) __stcg(reinterpret_cast<float4*>(p.ws_o + (at + rr) * HD) + c, o);  // else never read
+      } else {
+        const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+        uint2 v = make_uint2(0u, 0u);
+        if (l > 0.f) v = make_uint2(ActTraits<T>::pack2(o.x * inv, o.y * inv), ActTraits<T>::pack2(o.z * inv, o.w * inv));
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s_off[rr] + c * 4) = v;
       }
-      if (p.lse && row_ok && first) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
     }
   }
   if (failed) page_fail(p.status, kDevWaitTimeout);
@@ -883,6 +786,69 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
   }
   griddep_wait();  // whoever waits for this launch has then waited for the ones before it
+}
+
+// ============================================================================ states of a row -> output
+// One warp per (row, head).  Lane k weighs states k and k + 32 (kMaxParts is 64); then a lane adds
+// its HD / 32 dimensions of eight states at a time.
+constexpr int kMaxParts = 64;
+constexpr int kJoinWarps = 4;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixParams p) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const bool on = unit < p.n_joins * p.n_heads;
+  const int2 j = p.joins[on ? unit / p.n_heads : 0];
+  const int row = j.x, parts = on ? j.y : 0, head = unit % p.n_heads;
+  const int group = p.n_heads / p.n_kv_heads;
+  const size_t step = static_cast<size_t>(p.n_kv_heads) * p.n_rows * group;
+  const size_t at = static_cast<size_t>(head / group) * p.n_rows * group + static_cast<size_t>(row) * group + head % group;
+  griddep_wait();
+  if (!on) return;
+  float2 a = make_float2(-INFINITY, 0.f), b = a;
+  if (lane < parts) a = __ldcg(p.ws_ml + at + lane * step);
+  if (lane + 32 < parts) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
+  const float M = warp_max(fmaxf(a.x, b.x));
+  const float mu = M == -INFINITY ? 0.f : M;
+  const float wa = exp2_det_lo(a.x - mu), wb = exp2_det_lo(b.x - mu);
+  float L = a.y * wa + b.y * wb, O[V];
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+#pragma unroll
+  for (int e = 0; e < V; ++e) O[e] = 0.f;
+  const float* src = p.ws_o + at * HD + lane * V;
+  for (int k0 = 0; k0 < parts; k0 += 8) {
+    float v[8][V], w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + i;
+      w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
+      if (k >= parts) w[i] = 0.f;
+      if (w[i] > 0.f) {  // a state without visible positions holds no sums
+        if constexpr (V == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(src + k * step * HD));
+          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(src + k * step * HD));
+          v[i][0] = x.x, v[i][1] = x.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
+  }
+  T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
+  const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(out + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
+  if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
 }
 
 }  // namespace llm

@@ -213,8 +213,10 @@ struct llm_prefix_plan {
   int device = 0, dtype = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0;
   int n_seqs = 0, n_rows = 0, max_ctx = 0, top_slot = -1;
   void* block = nullptr;  // one device allocation: items, row_info, slots, states, sums
-  const PrefixItem* items[2][2] = {};  // [part, final][tile, columns]
-  int n_items[2][2] = {};
+  const PrefixItem* items[2] = {};  // [tile, columns]
+  int n_items[2] = {};
+  const int2* joins = nullptr;
+  int n_joins = 0;
   const int2* row_info = nullptr;
   const int* slots = nullptr;
   float* ws_o = nullptr;
@@ -223,8 +225,7 @@ struct llm_prefix_plan {
 
 namespace {
 
-enum { kPart = 0, kFinal = 1, kTile = 0, kCols = 1 };
-constexpr int kMaxParts = 64;    // states a row may have to join
+enum { kTile = 0, kCols = 1 };
 constexpr int kOpenEnd = 1 << 30;
 // Cost of starting and ending a CTA, in 64-position steps of its main loop.
 constexpr int kItemOverhead = 4;
@@ -235,15 +236,17 @@ struct PlanGroup {
   long long rho;  // score rows per kv head
 };
 
+long long tiles_of(long long rho) { return (rho + kTileRows - 1) / kTileRows; }
+int kind_of(long long rho) { return rho > kColRows ? kTile : kCols; }
 int kernel_slots(int kind, int head_dim) { return 148 * (kind == kTile ? 1 : head_dim == 64 ? 5 : 3); }
 
-// Positions per part item of the shared prefixes: a multiple of 64 that finishes first when every
-// CTA slot takes ceil(items / slots) items of that length.
+// Positions per item of the shared prefixes: a multiple of 64 that finishes first when every CTA
+// slot takes ceil(items / slots) items of that length.
 int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, int slots) {
   long long work = 0, longest = 0;
   for (const PlanGroup& g : groups) {
-    if (!g.shared || (g.rho > kColRows) != (kind == kTile)) continue;
-    work += ((g.rho + kTileRows - 1) / kTileRows) * n_kv_heads * ((g.prefix + 63) / 64);
+    if (!g.shared || kind_of(g.rho) != kind) continue;
+    work += tiles_of(g.rho) * n_kv_heads * ((g.prefix + 63) / 64);
     longest = std::max<long long>(longest, (g.prefix + 63) / 64);
   }
   if (work == 0) return 64;
@@ -254,8 +257,7 @@ int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, 
       if (c < 1) continue;
       long long items = 0;
       for (const PlanGroup& g : groups)
-        if (g.shared && (g.rho > kColRows) == (kind == kTile))
-          items += ((g.rho + kTileRows - 1) / kTileRows) * n_kv_heads * (((g.prefix + 63) / 64 + c - 1) / c);
+        if (g.shared && kind_of(g.rho) == kind) items += tiles_of(g.rho) * n_kv_heads * (((g.prefix + 63) / 64 + c - 1) / c);
       const long long cost = ((items + slots - 1) / slots) * (std::min(c, longest) + kItemOverhead);
       if (best_cost < 0 || cost < best_cost) best = c, best_cost = cost;
     }
@@ -263,12 +265,12 @@ int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, 
   return static_cast<int>(std::min(best, longest) * 64);
 }
 
-// The items of a batch.  Returns the number of states its rows may have.
+// The items of a batch and the rows with several states.  Returns the most states of a row.
 int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
-               int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2][2]) {
+               int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2], std::vector<int2>& joins) {
   std::vector<PlanGroup> groups;
   std::vector<int> row_start(1, 0);
-  long long final_ctas = 0;
+  long long own_ctas = 0;
   int seq = 0;
   for (int g = 0; g < n_groups; ++g) {
     PlanGroup pg{seq, group_sizes[g], prefixes[g], false, 0};
@@ -279,50 +281,50 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
       row_start.push_back(row_start.back() + rows[seq]);
       active += rho > 0;
       pg.rho += rho;
-      alone += (rho + kTileRows - 1) / kTileRows;
+      alone += (rho + 127) / 128;
+      own_ctas += tiles_of(rho) * n_kv_heads;
     }
-    final_ctas += alone * n_kv_heads;
-    // sharing pays when stacking the rows makes fewer passes over the prefix's pages
-    const long long stacked = (pg.rho + kTileRows - 1) / kTileRows;
-    pg.shared = active >= 2 && prefixes[g] > 0 && stacked * 10 <= alone * 7;
+    // sharing pays when stacking the rows leaves fewer 128-row steps over the prefix
+    pg.shared = active >= 2 && prefixes[g] > 0 && (pg.rho + 127) / 128 * 10 <= alone * 7;
     groups.push_back(pg);
   }
-  // pieces of the own ranges, when the final items alone leave most of the machine idle
-  const int pieces = final_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, final_ctas)));
+  // pieces of the own ranges, when one item a sequence leaves most of the machine idle
+  const int pieces = own_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, own_ctas)));
   const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim)),
                       part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim))};
-  int parts = 0;
+  int most = 0;
+  auto add = [&items](int row0, long long rho, int pos0, int pos1, int part) {
+    for (long long r = tiles_of(rho) - 1; r >= 0; --r)  // later rows see further: longest first
+      items[kind_of(rho)].push_back({row0, static_cast<int>(r * kTileRows),
+                                     static_cast<int>(std::min<long long>(kTileRows, rho - r * kTileRows)), pos0, pos1, part});
+  };
   for (const PlanGroup& g : groups) {
     int shared_parts = 0;
-    if (g.shared) {
-      const int kind = g.rho > kColRows ? kTile : kCols;
-      for (int pos = 0; pos < g.prefix; pos += len[kind], ++shared_parts)
-        for (long long r = 0; r < g.rho; r += kTileRows)
-          items[kPart][kind].push_back({row_start[g.seq0], static_cast<int>(r),
-                                        static_cast<int>(std::min<long long>(kTileRows, g.rho - r)), pos,
-                                        std::min(g.prefix, pos + len[kind]), shared_parts});
-    }
+    if (g.shared)
+      for (int pos = 0, c = len[kind_of(g.rho)]; pos < g.prefix; pos += c, ++shared_parts)
+        add(row_start[g.seq0], g.rho, pos, std::min(g.prefix, pos + c), shared_parts);
     const int start = g.shared ? g.prefix : 0;
     const int bound = max_ctx - start;  // most own positions
-    int n = std::max(1, std::min(pieces, bound / 512)), piece = kOpenEnd;
-    if (n > 1) piece = ((bound + n - 1) / n + 63) / 64 * 64;
+    const int n = std::max(1, std::min(pieces, bound / 512));
+    const int piece = n > 1 ? ((bound + n - 1) / n + 63) / 64 * 64 : kOpenEnd;
     for (int s = g.seq0; s < g.seq0 + g.n_seqs; ++s) {
       const long long rho = static_cast<long long>(rows[s]) * group;
-      const int kind = rho > kColRows ? kTile : kCols;
-      int own = 0;
-      for (int pos = start + piece; n > 1 && pos < max_ctx; pos += piece, ++own)
-        for (long long r = 0; r < rho; r += kTileRows)
-          items[kPart][kind].push_back({row_start[s], static_cast<int>(r), static_cast<int>(std::min<long long>(kTileRows, rho - r)),
-                                        pos, pos + piece, shared_parts + own});
-      for (long long r = (rho - 1) / kTileRows * kTileRows; rho > 0 && r >= 0; r -= kTileRows)  // longest first
-        items[kFinal][kind].push_back({row_start[s], static_cast<int>(r), static_cast<int>(std::min<long long>(kTileRows, rho - r)),
-                                       start, n > 1 ? start + piece : kOpenEnd, shared_parts + own});
-      parts = std::max(parts, shared_parts + own);
+      if (rho == 0) continue;
+      int parts = shared_parts;
+      if (n == 1) {
+        add(row_start[s], rho, start, kOpenEnd, shared_parts > 0 ? parts++ : -1);
+      } else {
+        for (int pos = start; pos < max_ctx; pos += piece) add(row_start[s], rho, pos, pos + piece, parts++);
+      }
+      for (int r = 0; parts > 0 && r < rows[s]; ++r) joins.push_back(make_int2(row_start[s] + r, parts));
+      most = std::max(most, parts);
     }
   }
-  for (auto& v : items[kPart])
-    std::stable_sort(v.begin(), v.end(), [](const PrefixItem& a, const PrefixItem& b) { return a.pos1 - a.pos0 > b.pos1 - b.pos0; });
-  return parts;
+  for (auto& v : items)
+    std::stable_sort(v.begin(), v.end(), [max_ctx](const PrefixItem& a, const PrefixItem& b) {
+      return std::min(a.pos1, max_ctx) - a.pos0 > std::min(b.pos1, max_ctx) - b.pos0;
+    });
+  return most;
 }
 
 template <typename T, int HD>
@@ -335,27 +337,31 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
     return e;
   }
   bool first = true;  // the first launch waits for the stream's earlier work as a whole
-  for (int final = 0; final < 2; ++final)
-    for (int kind = 0; kind < 2; ++kind) {
-      const int n = plan->n_items[final][kind];
-      if (n == 0) continue;
-      p.items = plan->items[final][kind];
-      p.final = final;
-      const dim3 grid(n * plan->n_kv_heads);
-      cudaError_t e;
-      if (kind == kTile) {
-        constexpr int smem = PrefixTileCfg<T, HD>::SMEM;
-        if (first) prefix_tile_kernel<T, HD><<<grid, kTileThreads, smem, s>>>(p), e = cudaGetLastError();
-        else e = launch_dependent(prefix_tile_kernel<T, HD>, grid, dim3(kTileThreads), smem, s, p);
-      } else {
-        constexpr int smem = AttnCfg<T, HD>::SMEM;
-        if (first) prefix_cols_kernel<T, HD><<<grid, kAttnWarps * 32, smem, s>>>(p), e = cudaGetLastError();
-        else e = launch_dependent(prefix_cols_kernel<T, HD>, grid, dim3(kAttnWarps * 32), smem, s, p);
-      }
-      if (e != cudaSuccess) return e;
-      first = false;
+  cudaError_t e = cudaSuccess;
+  if (plan->n_items[kTile] > 0) {
+    constexpr int smem = PrefixTileCfg<T, HD>::SMEM;
+    p.items = plan->items[kTile];
+    prefix_tile_kernel<T, HD><<<plan->n_items[kTile] * plan->n_kv_heads, kTileThreads, smem, s>>>(p);
+    e = cudaGetLastError();
+    first = false;
+  }
+  if (e == cudaSuccess && plan->n_items[kCols] > 0) {
+    constexpr int smem = AttnCfg<T, HD>::SMEM;
+    const dim3 grid(plan->n_items[kCols] * plan->n_kv_heads), block(kAttnWarps * 32);
+    p.items = plan->items[kCols];
+    if (first) {
+      prefix_cols_kernel<T, HD><<<grid, block, smem, s>>>(p);
+      e = cudaGetLastError();
+    } else {
+      e = launch_dependent(prefix_cols_kernel<T, HD>, grid, block, smem, s, p);
     }
-  return cudaSuccess;
+  }
+  if (e == cudaSuccess && plan->n_joins > 0) {
+    const long long units = static_cast<long long>(plan->n_joins) * plan->n_heads;
+    e = launch_dependent(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)),
+                         dim3(kJoinWarps * 32), 0, s, p);
+  }
+  return e;
 }
 
 cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, cudaStream_t s, bool prepare) {
@@ -409,8 +415,9 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
   llm_prefix_plan* p = nullptr;
   try {
     const int group = n_heads / n_kv_heads;
-    std::vector<PrefixItem> items[2][2];
-    const int parts = plan_items(rows, group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items);
+    std::vector<PrefixItem> items[2];
+    std::vector<int2> joins;
+    const int parts = plan_items(rows, group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins);
     std::vector<int2> info;
     info.reserve(total);
     for (int s = 0; s < n_seqs; ++s)
@@ -435,12 +442,13 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
       if (bytes) memcpy(host.data() + at, src, bytes);
       return at;
     };
-    size_t at_items[2][2];
-    for (int f = 0; f < 2; ++f)
-      for (int k = 0; k < 2; ++k) {
-        p->n_items[f][k] = static_cast<int>(items[f][k].size());
-        at_items[f][k] = place(items[f][k].data(), items[f][k].size() * sizeof(PrefixItem));
-      }
+    size_t at_items[2];
+    for (int k = 0; k < 2; ++k) {
+      p->n_items[k] = static_cast<int>(items[k].size());
+      at_items[k] = place(items[k].data(), items[k].size() * sizeof(PrefixItem));
+    }
+    p->n_joins = static_cast<int>(joins.size());
+    const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
     const size_t at_info = place(info.data(), info.size() * sizeof(int2));
     const size_t at_slots = place(slots, static_cast<size_t>(n_seqs) * 4);
     const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
@@ -460,8 +468,8 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
       return fail_fmt(LLM_ERR_CUDA, "plan set-up failed: %s", cudaGetErrorString(e));
     }
     uint8_t* base = static_cast<uint8_t*>(p->block);
-    for (int f = 0; f < 2; ++f)
-      for (int k = 0; k < 2; ++k) p->items[f][k] = reinterpret_cast<const PrefixItem*>(base + at_items[f][k]);
+    for (int k = 0; k < 2; ++k) p->items[k] = reinterpret_cast<const PrefixItem*>(base + at_items[k]);
+    p->joins = reinterpret_cast<const int2*>(base + at_joins);
     p->row_info = reinterpret_cast<const int2*>(base + at_info);
     p->slots = reinterpret_cast<const int*>(base + at_slots);
     p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
@@ -509,6 +517,8 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   p.ctx = ctx;
   p.slots = plan->slots;
   p.row_info = plan->row_info;
+  p.joins = plan->joins;
+  p.n_joins = plan->n_joins;
   p.ws_o = plan->ws_o;
   p.ws_ml = plan->ws_ml;
   p.status = c->status;
