@@ -82,12 +82,16 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
 // softmax per column, O^T += V^T . P^T with P as two terms; warp w takes pages w, w + 4, ... of
 // the item's range, and the four warps' states are joined once at the end.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix_cols_kernel(PrefixParams p) {
+constexpr int kColsSmem = kAttnWarps * AttnCfg<T, HD>::WARP_BYTES;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols_kernel(PrefixParams p) {
   using Cfg = AttnCfg<T, HD>;
   constexpr int STAGES = Cfg::STAGES;
   constexpr int PB = Cfg::PAGE_BYTES;
   constexpr int KS = HD / 16;
   constexpr int ROWB = HD * (int)sizeof(T);
+  static_assert(Cfg::FOLD_BYTES <= kColsSmem<T, HD>, "the fold area fits in the ring");
 
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kAttnWarps][STAGES];
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
   const int p_begin = it.pos0 >> 4, p_end = end > it.pos0 ? (end + 15) >> 4 : p_begin;
 
   uint8_t* wbuf = smem + warp * Cfg::WARP_BYTES;
-  float* const fold_area = reinterpret_cast<float*>(smem + kAttnWarps * Cfg::WARP_BYTES);
+  float* const fold_area = reinterpret_cast<float*>(smem);  // over the page ring, once it is idle
   float* const slot0 = fold_area;
   float* const slot1 = fold_area + Cfg::SLOT_FLOATS;
   const uint32_t wbase = smem_u32(wbuf);
@@ -258,6 +262,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
     st.l1 += __shfl_xor_sync(0xffffffffu, st.l1, off);
   }
   // (w0 + w1) + (w2 + w3), then the columns as rows [8][HD] in the fold area
+  __syncthreads();
   if (warp == 1) store_slot(slot0, st, lane);
   if (warp == 3) store_slot(slot1, st, lane);
   __syncthreads();
@@ -321,20 +326,30 @@ __global__ void __launch_bounds__(kAttnWarps * 32, attn_min_blocks<HD>()) prefix
 // Warps 0 and 11 = bulk-copy producers, warps 1 and 2 = the streams' MMA issuers (warp 1 allocates TMEM), warps
 // 3..6 stream 0, warps 7..10 stream 1.  Each stream issues PV(u), then S(u + 2) once PV(u) has read the
 // P that it overwrites; S(u + 1) is done by then, and the other stream's MMAs fill the tensor core.
-template <typename T, int HD>
+// Batches with pairs (WIDE) use the SM's shared memory whole.  Batches without use four stages (six
+// at head_dim 64) and at most 128 registers a thread, which leaves room for a CTA of
+// prefix_cols_kernel beside it: the sequences' own pages stream while the shared ones are worked on.
+// Streams that take alternate tiles use an even number of stages, so that a stage serves one stream
+// only: a stream that does not see the fill of a stage's previous tile (the other stream's) could
+// ask for the next one while that fill is still under way, and a parity wait two phases behind
+// returns at once.
+template <typename T, int HD, bool WIDE>
 struct PrefixTileCfg {
   static constexpr int HALVES = HD / 64;              // 64-element halves of a K / V row
   static constexpr int SUB = 16 * 128;                // one page's half sub-block (bytes)
   static constexpr int REGION = 4 * SUB;              // 64 positions of one half (bytes)
   static constexpr int TILE_BYTES = HALVES * REGION;  // K (or V) of one 64-position tile
-  static constexpr int STAGES = HD == 64 ? 10 : 5;    // of K and of V
+  static constexpr int STAGES = HD == 64 ? (WIDE ? 10 : 6) : (WIDE ? 5 : 4);  // of K and of V
   static constexpr int Q_BYTES = HALVES * 128 * 128;  // 128 rows x HD, K-major halves
-  static constexpr int SMEM = 2 * Q_BYTES + 2 * STAGES * TILE_BYTES + 1024;
+  static constexpr int K_RING = (WIDE ? 2 : 1) * Q_BYTES;
+  static constexpr int V_RING = K_RING + STAGES * TILE_BYTES;
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr float RESCALE_LOG2 = 8.0f;
   static constexpr int ROW_BYTES = HD * 4;            // of a row's sums, staged over Q and the rings
   static constexpr int META = 256 * (ROW_BYTES + 16);
-  static_assert(META <= 2 * Q_BYTES + 2 * STAGES * TILE_BYTES, "Q and the rings hold both streams' sums");
+  static constexpr int USED = V_RING + STAGES * TILE_BYTES;
+  static constexpr int BARS = (USED > META ? USED : META);  // the barriers lie behind the rings
+  static constexpr int SMEM = BARS + 512;
 };
 constexpr int kTileThreads = 384;
 constexpr int kTileRows = 256;  // score rows of a tile item
@@ -365,34 +380,50 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
   return p != 0;
 }
+// 32 lanes x 16 columns of 32-bit from registers (tmem_st32's half)
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void streams_bar() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixParams p) {
-  using Cfg = PrefixTileCfg<T, HD>;
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 512: at most 128 registers
+  using Cfg = PrefixTileCfg<T, HD, WIDE>;
   constexpr int ST = Cfg::STAGES;
   constexpr int HALVES = Cfg::HALVES;
   constexpr int SUB = Cfg::SUB;
   constexpr int REGION = Cfg::REGION;
   constexpr int ROWB = HD * (int)sizeof(T);
 
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2][2], p_ready[2][2],
-      pv_done[2], q_ready, drain;
-  __shared__ uint32_t s_tmem;
-  __shared__ int2 s_last[8];
+  // no static shared memory: the dynamic block starts on a 1024-byte boundary, as its alignment asks
+  extern __shared__ __align__(1024) uint8_t gbase[];
+  struct Sync {
+    uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2][2], p_ready[2][2], pv_done[2], q_ready, drain;
+    int2 s_last[8];
+    uint32_t s_tmem;
+  };
+  static_assert(sizeof(Sync) <= 512, "room behind the rings");
+  Sync& sync = *reinterpret_cast<Sync*>(gbase + Cfg::BARS);
+  auto &k_full = sync.k_full, &k_empty = sync.k_empty, &v_full = sync.v_full, &v_empty = sync.v_empty;
+  auto &s_full = sync.s_full, &p_ready = sync.p_ready;
+  auto& pv_done = sync.pv_done;
+  uint64_t &q_ready = sync.q_ready, &drain = sync.drain;
+  auto& s_last = sync.s_last;
+  uint32_t& s_tmem = sync.s_tmem;
 
-  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_s = sbase;
-  const uint32_t k_ring = q_s + 2 * Cfg::Q_BYTES;
-  const uint32_t v_ring = k_ring + ST * Cfg::TILE_BYTES;
-  uint8_t* const gbase = smem_raw + (sbase - smem_u32(smem_raw));  // generic pointer of sbase
+  const uint32_t q_s = smem_u32(gbase);
+  const uint32_t k_ring = q_s + Cfg::K_RING;
+  const uint32_t v_ring = q_s + Cfg::V_RING;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
   const int kvh = blockIdx.x % p.n_kv_heads;
   const int group = p.n_heads / p.n_kv_heads;
-  const bool pair = it.n_rho > 128;  // two row tiles; otherwise even and odd K/V tiles
+  const bool pair = WIDE && it.n_rho > 128;  // two row tiles; otherwise even and odd K/V tiles
   // warps 3..10: stream, TMEM lane, score row and the last position it sees
   const int sg = warp >= 7 ? 1 : 0;
   const int tl = (warp & 3) * 32 + lane;
@@ -449,6 +480,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
   const int n_pages_it = nkv > 0 ? ((end + 15) >> 4) - page0 : 0;
   // steps of each stream; step u of stream g works on K/V tile (pair ? u : 2 u + g)
   const int n0 = pair ? nkv : (nkv + 1) >> 1, n1 = pair ? nkv : nkv >> 1;
+  const int ring = pair ? ST : ST & ~1;  // stages in use
   bool failed = false;
 
   if (warp == 0 || warp == 11) {
@@ -457,7 +489,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     // block table 32 pages (8 tiles) per coalesced load, one batch ahead of use, and a lane issues
     // each copy: a page's half sub-block of K, both halves of V at once.
     const bool is_v = warp == 11;
-    const uint32_t ring = is_v ? v_ring : k_ring;
+    const uint32_t stages = is_v ? v_ring : k_ring;
     const uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
     const int per_page = is_v ? 1 : HALVES, size = is_v ? HALVES * SUB : SUB;
     const int j = lane / per_page, hh = lane % per_page;
@@ -469,27 +501,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
       return pg < n_pages_it ? page_entry(p, bt, pg) : 0;
     };
     int ent = entries(0), ent_next = entries(32);
-    int issued = 0;
+    int st = 0, turn = 0;  // stage, and its uses before this one
     for (int t = 0; t < nkv; ++t) {
       if (t > 0 && (t & 7) == 0) {
         ent = ent_next;
         ent_next = entries(4 * t + 32);
       }
-      const int st = t % ST, np = min(4, n_pages_it - 4 * t);
+      const int np = min(4, n_pages_it - 4 * t);
       const size_t phys = __shfl_sync(0xffffffffu, ent, ((t & 7) << 2) + (j & 3));
-      if (t >= ST && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&empty[st]), ((t / ST) + 1) & 1))) {
+      if (turn > 0 && !__all_sync(0xffffffffu, mbar_poll(smem_u32(&empty[st]), (turn + 1) & 1))) {
         failed = true;
         break;
       }
       const uint32_t bar = smem_u32(&full[st]);
       if (lane == 0) mbar_arrive_expect_tx(bar, np * HALVES * SUB);
       __syncwarp();
-      if (j < np) bulk_g2s(ring + st * Cfg::TILE_BYTES + place, src + phys * p.n_kv_heads * (2 * 16 * ROWB), size, bar);
-      issued = t + 1;
+      if (j < np) bulk_g2s(stages + st * Cfg::TILE_BYTES + place, src + phys * p.n_kv_heads * (2 * 16 * ROWB), size, bar);
+      if (++st == ring) st = 0, ++turn;
     }
     // copies still in flight must land before the CTA's shared memory goes away
     if (lane == 0)
-      for (int t = max(0, issued - ST); t < issued; ++t) mbar_poll(smem_u32(&full[t % ST]), (t / ST) & 1);
+      for (int i = 0; i < ring; ++i) {
+        const int uses = turn + (i < st ? 1 : 0);
+        if (uses > 0) mbar_poll(smem_u32(&full[i]), (uses - 1) & 1);
+      }
   } else if (warp <= 2) {
     // ------------------------------------------------------------ MMA issuer of stream warp - 1
     const int g = warp - 1;
@@ -499,11 +534,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
     constexpr uint32_t idesc_pv = umma_idesc<T>(128, HD) | (1u << 16);  // B (V) MN-major
     const uint64_t qd = sw128_desc(q_s + (pair ? g * Cfg::Q_BYTES : 0));
     const uint64_t kd0 = sw128_desc(k_ring), vd0 = sw128_desc_mn(v_ring, SUB, 1024);
+    // stage and parity of the next K and of the next V tile of this stream
+    int ks = pair ? 0 : g, kpar = 0, vs = ks, vpar = 0;
+    auto advance = [&](int& st, int& par) {
+      st += pair ? 1 : 2;
+      if (st >= ring) st -= ring, par ^= 1;
+    };
     // S of step u into the stream's buffer u & 1, whose P the stream's PV(u - 2) has read
     auto issue_s = [&](int u) -> bool {
-      const int t = pair ? u : 2 * u + g, s = t % ST;
+      const int s = ks;
       bool ok = u < 2 || mbar_poll(smem_u32(&pv_done[g]), u & 1);
-      ok = ok && mbar_poll(smem_u32(&k_full[s]), (t / ST) & 1);
+      ok = ok && mbar_poll(smem_u32(&k_full[s]), kpar);
+      advance(ks, kpar);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
       const uint64_t kd = kd0 + static_cast<uint64_t>(s * (Cfg::TILE_BYTES >> 4));
@@ -521,8 +563,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
       return true;
     };
     auto issue_pv = [&](int u) -> bool {
-      const int t = pair ? u : 2 * u + g, s = t % ST;
-      bool ok = mbar_poll(smem_u32(&v_full[s]), (t / ST) & 1);
+      const int s = vs;
+      bool ok = mbar_poll(smem_u32(&v_full[s]), vpar);
+      advance(vs, vpar);
       ok = ok && mbar_poll(smem_u32(&p_ready[g][u & 1]), (u >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
@@ -603,11 +646,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
       // Both streams of a pair do it, each before its own PV.
       const int valid = end - kbase;
       if (valid < 64) {
-        if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&v_full[t % ST]), (t / ST) & 1))) {
+        if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&v_full[t % ring]), (t / ring) & 1))) {
           ok = false;
           break;
         }
-        uint8_t* vreg = gbase + (v_ring - sbase) + (t % ST) * Cfg::TILE_BYTES;
+        uint8_t* vreg = gbase + Cfg::V_RING + (t % ring) * Cfg::TILE_BYTES;
         for (int idx = tl; idx < (64 - valid) * HALVES * 8; idx += 128) {
           const int rr = valid + idx / (HALVES * 8), rem = idx % (HALVES * 8);
           *reinterpret_cast<uint4*>(vreg + ((rr >> 4) * HALVES + (rem >> 3)) * SUB + (rr & 15) * 128 + ((rem & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -652,16 +695,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
       float2 r4[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) r4[k] = make_float2(0.f, 0.f);
-      {
-        const float2 sl22 = make_float2(sl2, sl2), nmu = make_float2(-mu, -mu);
+      const float2 sl22 = make_float2(sl2, sl2), nmu = make_float2(-mu, -mu);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 x = fma2_rn(make_float2(sv[2 * e], sv[2 * e + 1]), sl22, nmu);
+      for (int h = 0; h < 2; ++h) {  // 32 positions at a time: P as hi + lo over the S columns read
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = fma2_rn(make_float2(sv[32 * h + 2 * e], sv[32 * h + 2 * e + 1]), sl22, nmu);
           const float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-          sv[2 * e] = pe.x;
-          sv[2 * e + 1] = pe.y;
           r4[e & 3] = add2_rn(r4[e & 3], pe);
+          hi[e] = ActTraits<T>::pack2(pe.x, pe.y);
+          const float2 rest = sub2_rn(pe, ActTraits<T>::unpack2(hi[e]));
+          lo[e] = ActTraits<T>::pack2(rest.x, rest.y);
         }
+        tmem_st16(scol + 16 * h, hi);
+        tmem_st16(scol + 32 + 16 * h, lo);
       }
       l_run = l_run * alpha + (((r4[0].x + r4[0].y) + (r4[1].x + r4[1].y)) + ((r4[2].x + r4[2].y) + (r4[3].x + r4[3].y)));
       m_ref = m_new;
@@ -675,25 +723,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) prefix_tile_kernel(PrefixPara
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(trow + 128 + c * 32, r);
+          uint32_t v[32];
+          tmem_ld32(trow + 128 + c * 32, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
-          tmem_st32(trow + 128 + c * 32, r);
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+          tmem_st32(trow + 128 + c * 32, v);
         }
-      }
-      {
-        uint32_t hi[32], lo[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 pe = make_float2(sv[2 * e], sv[2 * e + 1]);
-          hi[e] = ActTraits<T>::pack2(pe.x, pe.y);
-          const float2 rest = sub2_rn(pe, ActTraits<T>::unpack2(hi[e]));
-          lo[e] = ActTraits<T>::pack2(rest.x, rest.y);
-        }
-        tmem_st32(scol, hi);
-        tmem_st32(scol + 32, lo);
       }
       tmem_wait_st();
       tc_fence_before();

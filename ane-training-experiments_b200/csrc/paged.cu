@@ -215,6 +215,7 @@ struct llm_prefix_plan {
   void* block = nullptr;  // one device allocation: items, row_info, slots, states, sums
   const PrefixItem* items[2] = {};  // [tile, columns]
   int n_items[2] = {};
+  bool pairs = false;  // some item has more than 128 score rows
   const int2* joins = nullptr;
   int n_joins = 0;
   const int2* row_info = nullptr;
@@ -322,7 +323,8 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
   }
   for (auto& v : items)
     std::stable_sort(v.begin(), v.end(), [max_ctx](const PrefixItem& a, const PrefixItem& b) {
-      return std::min(a.pos1, max_ctx) - a.pos0 > std::min(b.pos1, max_ctx) - b.pos0;
+      auto cost = [max_ctx](const PrefixItem& i) { return (std::min(i.pos1, max_ctx) - i.pos0) * (i.n_rho > 128 ? 2ll : 1ll); };
+      return cost(a) > cost(b);
     });
   return most;
 }
@@ -330,23 +332,27 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
 template <typename T, int HD>
 cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStream_t s, bool prepare) {
   if (prepare) {
-    cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         PrefixTileCfg<T, HD>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         PrefixTileCfg<T, HD, false>::SMEM);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(prefix_cols_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnCfg<T, HD>::SMEM);
+      e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               PrefixTileCfg<T, HD, true>::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(prefix_cols_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kColsSmem<T, HD>);
     return e;
   }
   bool first = true;  // the first launch waits for the stream's earlier work as a whole
   cudaError_t e = cudaSuccess;
   if (plan->n_items[kTile] > 0) {
-    constexpr int smem = PrefixTileCfg<T, HD>::SMEM;
+    const int grid = plan->n_items[kTile] * plan->n_kv_heads;
     p.items = plan->items[kTile];
-    prefix_tile_kernel<T, HD><<<plan->n_items[kTile] * plan->n_kv_heads, kTileThreads, smem, s>>>(p);
+    if (plan->pairs) prefix_tile_kernel<T, HD, true><<<grid, kTileThreads, PrefixTileCfg<T, HD, true>::SMEM, s>>>(p);
+    else prefix_tile_kernel<T, HD, false><<<grid, kTileThreads, PrefixTileCfg<T, HD, false>::SMEM, s>>>(p);
     e = cudaGetLastError();
     first = false;
   }
   if (e == cudaSuccess && plan->n_items[kCols] > 0) {
-    constexpr int smem = AttnCfg<T, HD>::SMEM;
+    constexpr int smem = kColsSmem<T, HD>;
     const dim3 grid(plan->n_items[kCols] * plan->n_kv_heads), block(kAttnWarps * 32);
     p.items = plan->items[kCols];
     if (first) {
@@ -447,6 +453,7 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
       p->n_items[k] = static_cast<int>(items[k].size());
       at_items[k] = place(items[k].data(), items[k].size() * sizeof(PrefixItem));
     }
+    for (const PrefixItem& it : items[kTile]) p->pairs = p->pairs || it.n_rho > 128;
     p->n_joins = static_cast<int>(joins.size());
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
     const size_t at_info = place(info.data(), info.size() * sizeof(int2));
