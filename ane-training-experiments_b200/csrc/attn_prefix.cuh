@@ -308,7 +308,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
       if (p.lse && d == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(s_m[c], l);
     }
   }
-  griddep_wait();  // whoever waits for this launch has then waited for the ones before it
+  // the launch ends after the one before it, so that whoever waits for it has waited for both; one
+  // CTA sees to that, the others make room
+  if (blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 // ============================================================================ up to 256 score rows
@@ -346,7 +348,7 @@ struct PrefixTileCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr float RESCALE_LOG2 = 8.0f;
   static constexpr int ROW_BYTES = HD * 4;            // of a row's sums, staged over Q and the rings
-  static constexpr int META = 256 * (ROW_BYTES + 16);
+  static constexpr int META = 256 * (ROW_BYTES + 20);
   static constexpr int USED = V_RING + STAGES * TILE_BYTES;
   static constexpr int BARS = (USED > META ? USED : META);  // the barriers lie behind the rings
   static constexpr int SMEM = BARS + 512;
@@ -752,6 +754,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     float4* const stage = reinterpret_cast<float4*>(gbase);
     float2* const s_ml = reinterpret_cast<float2*>(gbase + 256 * Cfg::ROW_BYTES);  // [256]
     long long* const s_off = reinterpret_cast<long long*>(s_ml + 256);             // [256] of the output row
+    float* const s_w = reinterpret_cast<float*>(s_off + 256);                      // [256]
     const int mine = sg * 128 + tl;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
@@ -768,49 +771,54 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     s_off[mine] = row * p.o_row + head * p.o_head;
     const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * p.n_rows * group +
                       static_cast<size_t>(it.row0) * group + it.rho0;
+    if (!pair) streams_bar();
+    float m = m_ref, l = l_run, w = l_run > 0.f ? 1.f : 0.f;  // the row's state, and this stream's weight in it
+    if (!pair) {
+      const float2 other = s_ml[(1 - sg) * 128 + tl];
+      m = fmaxf(m_ref, other.x);
+      const float mu = m == -INFINITY ? 0.f : m;
+      w = ex2_approx(m_ref - mu);  // 0 where this stream saw nothing
+      l = l_run * w + other.y * ex2_approx(other.x - mu);
+    }
+    if (row_ok && (pair || sg == 0)) {
+      if (it.part >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
+      else if (p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
+    }
+    s_w[mine] = it.part < 0 && l > 0.f ? __fdiv_rn(w, l) : w;
     if (pair) __syncwarp();
     else streams_bar();
-    if (pair || sg == 0) {  // the thread of a row stores its state's m and l, or its lse
-      float m = m_ref, l = l_run;
-      if (!pair) {
-        const float2 other = s_ml[128 + tl];
-        m = fmaxf(m, other.x);
-        const float mu = m == -INFINITY ? 0.f : m;
-        l = l * ex2_approx(m_ref - mu) + other.y * ex2_approx(other.x - mu);
-      }
-      if (row_ok && it.part >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
-      if (row_ok && it.part < 0 && p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
-    }
     // rows of this warp: its own 32 of a pair; 16 of the tile, from both streams, otherwise
     const int rows_w = pair ? 32 : 16, row_w = pair ? sg * 128 + (warp & 3) * 32 : (sg * 4 + (warp & 3)) * 16;
     const int n_w = min(rows_w, it.n_rho - row_w);
     constexpr int PER = 32 / CH;  // rows a warp stores at once
     const int c = lane % CH;
-#pragma unroll 4
-    for (int r0 = 0; r0 < n_w; r0 += PER) {
-      const int rr = row_w + r0 + lane / CH;
-      if (rr >= row_w + n_w) continue;
-      const float2 a = s_ml[rr];
-      float w = 1.f, m = a.x, l = a.y;
-      float4 o = stage[rr * CH + (c ^ (rr & (CH - 1)))];
-      if (!pair) {
-        const float2 b = s_ml[128 + rr];
-        m = fmaxf(a.x, b.x);
-        const float mu = m == -INFINITY ? 0.f : m;
-        w = ex2_approx(a.x - mu);
-        const float w1 = ex2_approx(b.x - mu);
-        const float4 x = stage[(128 + rr) * CH + (c ^ (rr & (CH - 1)))];
-        l = a.y * w + b.y * w1;
-        o = w > 0.f ? make_float4(o.x * w, o.y * w, o.z * w, o.w * w) : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w1 > 0.f) o = make_float4(o.x + x.x * w1, o.y + x.y * w1, o.z + x.z * w1, o.w + x.w * w1);
+    for (int r0 = 0; r0 < n_w; r0 += 8 * PER) {
+      float4 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = r0 + i * PER + lane / CH, rr = row_w + (k < n_w ? k : 0);
+        const float wa = s_w[rr];
+        const float4 x = stage[rr * CH + (c ^ (rr & (CH - 1)))];  // not finite where the row saw nothing
+        o[i] = wa > 0.f ? make_float4(x.x * wa, x.y * wa, x.z * wa, x.w * wa) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!pair) {
+          const float wb = s_w[128 + rr];
+          const float4 y = stage[(128 + rr) * CH + (c ^ (rr & (CH - 1)))];
+          if (wb > 0.f) o[i] = make_float4(o[i].x + y.x * wb, o[i].y + y.y * wb, o[i].z + y.z * wb, o[i].w + y.w * wb);
+        }
       }
       if (it.part >= 0) {
-        if (l > 0.f) __stcg(reinterpret_cast<float4*>(p.ws_o + (at + rr) * HD) + c, o);  // else never read
+        float4* dst = reinterpret_cast<float4*>(p.ws_o + (at + row_w + r0 + lane / CH) * HD) + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r0 + i * PER + lane / CH < n_w) __stcg(dst + i * PER * CH, o[i]);
       } else {
-        const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
-        uint2 v = make_uint2(0u, 0u);
-        if (l > 0.f) v = make_uint2(ActTraits<T>::pack2(o.x * inv, o.y * inv), ActTraits<T>::pack2(o.z * inv, o.w * inv));
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s_off[rr] + c * 4) = v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = r0 + i * PER + lane / CH;
+          if (k < n_w)
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s_off[row_w + k] + c * 4) =
+                make_uint2(ActTraits<T>::pack2(o[i].x, o[i].y), ActTraits<T>::pack2(o[i].z, o[i].w));
+        }
       }
     }
   }
@@ -821,16 +829,17 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
   }
-  griddep_wait();  // whoever waits for this launch has then waited for the ones before it
 }
 
 // ============================================================================ states of a row -> output
 // One warp per (row, head).  Lane k weighs states k and k + 32 (kMaxParts is 64); then a lane adds
-// its HD / 32 dimensions of eight states at a time.
+// its HD / 32 dimensions of BATCH states at a time: 8, or 20 where rows have more (18 states of 64
+// rows: 2.5 us after the last item against 4; but 152 registers, which costs 4 us where 4096 rows and
+// heads have four states each).
 constexpr int kMaxParts = 64;
 constexpr int kJoinWarps = 4;
 
-template <typename T, int HD>
+template <typename T, int HD, int BATCH>
 __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixParams p) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x & 31;
@@ -855,10 +864,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
 #pragma unroll
   for (int e = 0; e < V; ++e) O[e] = 0.f;
   const float* src = p.ws_o + at * HD + lane * V;
-  for (int k0 = 0; k0 < parts; k0 += 8) {
-    float v[8][V], w[8];
+  for (int k0 = 0; k0 < parts; k0 += BATCH) {
+    float v[BATCH][V], w[BATCH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       const int k = k0 + i;
       w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
       if (k >= parts) w[i] = 0.f;
@@ -876,7 +885,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < BATCH; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
   }

@@ -217,7 +217,7 @@ struct llm_prefix_plan {
   int n_items[2] = {};
   bool pairs = false;  // some item has more than 128 score rows
   const int2* joins = nullptr;
-  int n_joins = 0;
+  int n_joins = 0, parts = 0;
   const int2* row_info = nullptr;
   const int* slots = nullptr;
   float* ws_o = nullptr;
@@ -332,13 +332,15 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
 template <typename T, int HD>
 cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStream_t s, bool prepare) {
   if (prepare) {
-    cudaError_t e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         PrefixTileCfg<T, HD, false>::SMEM);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(prefix_tile_kernel<T, HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               PrefixTileCfg<T, HD, true>::SMEM);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(prefix_cols_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kColsSmem<T, HD>);
+    // the whole carve-out for shared memory, so that CTAs of both kernels fit an SM together
+    auto set = [](auto kernel, int smem) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                                         cudaSharedmemCarveoutMaxShared);
+    };
+    cudaError_t e = set(prefix_tile_kernel<T, HD, false>, PrefixTileCfg<T, HD, false>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, true>, PrefixTileCfg<T, HD, true>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_cols_kernel<T, HD>, kColsSmem<T, HD>);
     return e;
   }
   bool first = true;  // the first launch waits for the stream's earlier work as a whole
@@ -364,8 +366,9 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
   }
   if (e == cudaSuccess && plan->n_joins > 0) {
     const long long units = static_cast<long long>(plan->n_joins) * plan->n_heads;
-    e = launch_dependent(prefix_join_kernel<T, HD>, dim3(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)),
-                         dim3(kJoinWarps * 32), 0, s, p);
+    const dim3 grid(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
+    e = plan->parts > 8 ? launch_dependent(prefix_join_kernel<T, HD, 20>, grid, block, 0, s, p)
+                        : launch_dependent(prefix_join_kernel<T, HD, 8>, grid, block, 0, s, p);
   }
   return e;
 }
@@ -455,6 +458,7 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     }
     for (const PrefixItem& it : items[kTile]) p->pairs = p->pairs || it.n_rho > 128;
     p->n_joins = static_cast<int>(joins.size());
+    p->parts = parts;
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
     const size_t at_info = place(info.data(), info.size() * sizeof(int2));
     const size_t at_slots = place(slots, static_cast<size_t>(n_seqs) * 4);
