@@ -121,7 +121,7 @@ PageTables tables(const llm_page_cache* c) {
 // CTAs of a launch that copies up to `moves` pages of every layer.
 int copy_grid(const PageTables& t, long long moves) {
   const long long chunks = moves * t.n_layers * (t.block_bytes / kCopyChunk);
-  return static_cast<int>(std::max(1ll, std::min(chunks, 148ll * 8)));
+  return static_cast<int>(std::max(1ll, std::min((chunks + kCopyBatch - 1) / kCopyBatch, 148ll * 5)));
 }
 
 }  // namespace
@@ -191,7 +191,7 @@ extern "C" int llm_pages_free(int device, const llm_page_cache* c, const int32_t
   if (n == 0) return LLM_OK;
   DeviceScope dev;
   RC(dev.enter(device));
-  pages_free_kernel<<<std::min(n, 148), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(tables(c), slots, n);
+  pages_free_kernel<<<std::min(n, 148 * 4), kFreeThreads, 0, static_cast<cudaStream_t>(stream)>>>(tables(c), slots, n);
   CU(cudaGetLastError());
   return LLM_OK;
 }

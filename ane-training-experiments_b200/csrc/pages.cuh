@@ -43,7 +43,7 @@ struct PageTables {
 
 // Layout of the work area.  ticket, marks and bits are zero between calls.
 struct PageWork {
-  enum { kTicket = 0, kValid = 1, kCount = 2, kLive = 3, kHeader = 16 };
+  enum { kTicket = 0, kValid = 1, kCount = 2, kLive = 3, kMoves = 4, kHeader = 16 };
   static __host__ __device__ size_t marks() { return kHeader; }                                  // [max_seqs]
   static __host__ __device__ size_t first(int seqs) { return marks() + seqs; }                   // [max_seqs]
   static __host__ __device__ size_t bits(int seqs) { return first(seqs) + seqs; }                // [n_pages / 32]
@@ -53,12 +53,14 @@ struct PageWork {
 };
 
 constexpr int kPlanThreads = 1024;
+constexpr int kFreeThreads = 256;
 constexpr int kCopyThreads = 256;
-constexpr int kCopyChunk = 4096;  // bytes one CTA copies per turn: 16 per thread
+constexpr int kCopyChunk = 4096;  // bytes of a chunk: 16 per thread; a block of any geometry is whole chunks
+constexpr int kCopyBatch = 4;     // chunks a CTA has in flight
 
 __device__ __forceinline__ void page_fail(int* status, int code) { atomicCAS(status, 0, code); }
 
-// Exclusive prefix sum over the CTA's kPlanThreads values; `total` is their sum.  `s` holds 33 ints.
+// Exclusive prefix sum over the CTA's values (at most 1024); `total` is their sum.  `s` holds 33 ints.
 __device__ __forceinline__ int block_exclusive(int v, int* s, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
@@ -71,7 +73,7 @@ __device__ __forceinline__ int block_exclusive(int v, int* s, int& total) {
   if (lane == 31) s[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    const int w = s[lane];
+    const int w = lane < static_cast<int>(blockDim.x >> 5) ? s[lane] : 0;
     int y = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -86,30 +88,47 @@ __device__ __forceinline__ int block_exclusive(int v, int* s, int& total) {
   return s[warp] + x - v;
 }
 
-// Chunk `c` of page move src -> dst: chunks run over (move, layer, offset in the block).
-__device__ __forceinline__ void copy_chunk(const uint8_t* from, int from_pages, uint8_t* to, int to_pages,
-                                           int block_bytes, int src, int dst, int layer, int offset) {
-  const size_t a = (static_cast<size_t>(layer) * from_pages + src) * block_bytes + offset;
-  const size_t b = (static_cast<size_t>(layer) * to_pages + dst) * block_bytes + offset;
-  const uint4 v = *reinterpret_cast<const uint4*>(from + a + threadIdx.x * 16);
-  *reinterpret_cast<uint4*>(to + b + threadIdx.x * 16) = v;
+// Copies page src[i] -> dst[i] in every layer, i < n, over all CTAs of the grid.  Moving a page is
+// its bytes read and written once, so what counts is bytes in flight: a CTA takes kCopyBatch
+// consecutive chunks (16 KB) at a time, every load before the first store, five CTAs to an SM.
+// Chunks run over (move, layer, offset in the block).
+__device__ __forceinline__ void copy_pages(const uint8_t* from, int from_pages, uint8_t* to, int to_pages, int n_layers,
+                                           int block_bytes, const int* src, const int* dst, int n, int* status) {
+  const unsigned chunks = block_bytes / kCopyChunk;
+  const long long all = static_cast<long long>(n) * n_layers * chunks;
+  for (long long w = static_cast<long long>(blockIdx.x) * kCopyBatch; w < all; w += static_cast<long long>(gridDim.x) * kCopyBatch) {
+    const long long blk = w / chunks;
+    unsigned chunk = static_cast<unsigned>(w - blk * chunks);
+    int i = static_cast<int>(blk / n_layers), layer = static_cast<int>(blk - static_cast<long long>(i) * n_layers);
+    uint4 v[kCopyBatch];
+    uint8_t* out[kCopyBatch];
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u) {
+      out[u] = nullptr;
+      if (w + u < all) {
+        const int a = src[i], b = dst[i];
+        if (a < 0 || a >= from_pages || b < 0 || b >= to_pages) {
+          if (threadIdx.x == 0) page_fail(status, kPageBadRequest);
+        } else {
+          const size_t at = static_cast<size_t>(chunk) * kCopyChunk + threadIdx.x * 16;
+          v[u] = *reinterpret_cast<const uint4*>(from + (static_cast<size_t>(layer) * from_pages + a) * block_bytes + at);
+          out[u] = to + (static_cast<size_t>(layer) * to_pages + b) * block_bytes + at;
+        }
+        if (++chunk == chunks) {
+          chunk = 0;
+          if (++layer == n_layers) layer = 0, ++i;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u)
+      if (out[u]) *reinterpret_cast<uint4*>(out[u]) = v[u];
+  }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(PageTables from, PageTables to, const int* src,
-                                                                  const int* dst, int n) {
-  const int chunks = from.block_bytes / kCopyChunk;
-  const long long all = static_cast<long long>(n) * from.n_layers * chunks;
-  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
-    const int chunk = static_cast<int>(w % chunks);
-    const int layer = static_cast<int>((w / chunks) % from.n_layers);
-    const int i = static_cast<int>(w / chunks / from.n_layers);
-    const int a = src[i], b = dst[i];
-    if (a < 0 || a >= from.n_pages || b < 0 || b >= to.n_pages) {
-      if (threadIdx.x == 0) page_fail(from.status, kPageBadRequest);
-      continue;
-    }
-    copy_chunk(from.pool, from.n_pages, to.pool, to.n_pages, from.block_bytes, a, b, layer, chunk * kCopyChunk);
-  }
+__global__ void __launch_bounds__(kCopyThreads, 5) pages_copy_kernel(PageTables from, PageTables to, const int* src,
+                                                                     const int* dst, int n) {
+  copy_pages(from.pool, from.n_pages, to.pool, to.n_pages, from.n_layers, from.block_bytes, src, dst, n, from.status);
 }
 
 // ----------------------------------------------------------------------------- fork
@@ -149,9 +168,12 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParam
   int* const work = p.t.work;
   int* const mark = work + PageWork::marks();
   int* const first = work + PageWork::first(p.t.max_seqs);
+  int* const src = work + PageWork::src(p.t.max_seqs, p.t.n_pages);
+  int* const dst = work + PageWork::dst(p.t.max_seqs, p.t.n_pages);
+  const int have = *p.t.n_free;
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
-  int base = 0;
+  int base = 0, moves = 0;
   for (int i0 = 0; i0 < p.n; i0 += kPlanThreads) {
     const int i = i0 + threadIdx.x;
     ForkShape f{0, 0, false, false};
@@ -162,6 +184,15 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParam
     int total;
     const int off = block_exclusive(f.fresh, s_scan, total);
     if (i < p.n) first[i] = base + off;
+    // the copies of partly filled pages; a request that needs one takes a new page, so the list
+    // is no longer than the pool when the request is served
+    int tails;
+    const int at = moves + block_exclusive(f.tail ? 1 : 0, s_scan, tails);
+    if (f.tail && base + off < have && at < p.t.n_pages) {
+      src[at] = p.t.table[static_cast<size_t>(p.parents[i]) * p.t.max_pages + f.keep];
+      dst[at] = p.t.free_pages[have - 1 - base - off];
+    }
+    moves += tails;
     base += total;
     if (base > p.t.n_pages) break;  // more than the pool has: refused below; also keeps the sum small
   }
@@ -171,19 +202,19 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParam
     if (c >= 0 && c < p.t.max_seqs) mark[c] = 0;
   }
   if (threadIdx.x == 0) {
-    const int have = *p.t.n_free;
     const bool bad = s_bad != 0, out = base > have;
     if (bad) page_fail(p.t.status, kPageBadRequest);
     else if (out) page_fail(p.t.status, kPageExhausted);
     work[PageWork::kValid] = !bad && !out;
     work[PageWork::kCount] = have;
+    work[PageWork::kMoves] = moves;
     if (!bad && !out) *p.t.n_free = have - base;
   }
 }
 
 // Rows, reference counts and the copies of partly filled pages.  The rows are read while npages
 // still holds the old counts; the last CTA stores the new ones.
-__global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(ForkParams p) {
+__global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams p) {
   __shared__ int s_last;
   griddep_wait();
   int* const work = p.t.work;
@@ -211,23 +242,9 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(ForkParams p) 
       }
     }
   }
-  const int chunks = p.t.block_bytes / kCopyChunk;
-  const long long all = static_cast<long long>(p.n) * p.t.n_layers * chunks;
-  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
-    const int i = static_cast<int>(w / chunks / p.t.n_layers);
-    ForkShape f;
-    fork_shape(p, i, f);
-    if (!f.tail) continue;
-    const int a = p.t.table[static_cast<size_t>(p.parents[i]) * p.t.max_pages + f.keep];
-    const int b = p.t.free_pages[top - 1 - first[i]];
-    if (a < 0 || a >= p.t.n_pages || b < 0 || b >= p.t.n_pages) {
-      if (threadIdx.x == 0) page_fail(p.t.status, kDevBadPage);
-      continue;
-    }
-    const int chunk = static_cast<int>(w % chunks);
-    copy_chunk(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.block_bytes, a, b,
-               static_cast<int>((w / chunks) % p.t.n_layers), chunk * kCopyChunk);
-  }
+  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes,
+             work + PageWork::src(p.t.max_seqs, p.t.n_pages), work + PageWork::dst(p.t.max_seqs, p.t.n_pages),
+             work[PageWork::kMoves], p.t.status);
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
@@ -245,7 +262,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(ForkParams p) 
 }
 
 // ----------------------------------------------------------------------------- free
-__global__ void __launch_bounds__(kPlanThreads) pages_free_kernel(PageTables t, const int* slots, int n) {
+__global__ void __launch_bounds__(kFreeThreads) pages_free_kernel(PageTables t, const int* slots, int n) {
   __shared__ int s_scan[33];
   __shared__ int s_held, s_last;
   int* const work = t.work;
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_free_kernel(PageTables t, 
     if (threadIdx.x == 0) s_held = min(atomicExch(t.npages + slot, 0), t.max_pages);
     __syncthreads();
     int* row = t.table + static_cast<size_t>(slot) * t.max_pages;
-    for (int j = threadIdx.x; j < s_held; j += kPlanThreads) {
+    for (int j = threadIdx.x; j < s_held; j += kFreeThreads) {
       const int e = row[j];
       row[j] = -1;
       if (e < 0 || e >= t.n_pages) {
@@ -287,7 +304,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_free_kernel(PageTables t, 
   __threadfence();
   // the emptied pages in ascending order on the stack: each thread a run of words
   const int words = (t.n_pages + 31) / 32;
-  const int per = (words + kPlanThreads - 1) / kPlanThreads;
+  const int per = (words + kFreeThreads - 1) / kFreeThreads;
   const int w0 = min(words, static_cast<int>(threadIdx.x) * per), w1 = min(words, w0 + per);
   int mine = 0;
   for (int w = w0; w < w1; ++w) mine += __popc(__ldcg(bits + w));
@@ -363,7 +380,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTa
   __syncthreads();
   for (int w = w0; w < w1; ++w) bits[w] = 0;
   if (threadIdx.x == 0) {
-    work[PageWork::kCount] = moves;
+    work[PageWork::kMoves] = moves;
     work[PageWork::kLive] = n_live;
     work[PageWork::kTicket] = 0;
     *t.n_free = t.n_pages - n_live;
@@ -372,10 +389,10 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTa
 
 // The moves (sources are at or above n_live, destinations below it, so they never overlap), the
 // renamed counts and table entries, and the free stack.
-__global__ void __launch_bounds__(kCopyThreads) pages_compact_kernel(PageTables t) {
+__global__ void __launch_bounds__(kCopyThreads, 5) pages_compact_kernel(PageTables t) {
   griddep_wait();
   const int* work = t.work;
-  const int moves = work[PageWork::kCount], n_live = work[PageWork::kLive];
+  const int moves = work[PageWork::kMoves], n_live = work[PageWork::kLive];
   const int* src = work + PageWork::src(t.max_seqs, t.n_pages);
   const int* dst = work + PageWork::dst(t.max_seqs, t.n_pages);
   const long long tid = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x;
@@ -399,13 +416,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_compact_kernel(PageTables 
     t.refs[src[k]] = 0;
   }
   for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
-  const int chunks = t.block_bytes / kCopyChunk;
-  const long long all = static_cast<long long>(moves) * t.n_layers * chunks;
-  for (long long w = blockIdx.x; w < all; w += gridDim.x) {
-    const int i = static_cast<int>(w / chunks / t.n_layers);
-    copy_chunk(t.pool, t.n_pages, t.pool, t.n_pages, t.block_bytes, src[i], dst[i],
-               static_cast<int>((w / chunks) % t.n_layers), static_cast<int>(w % chunks) * kCopyChunk);
-  }
+  copy_pages(t.pool, t.n_pages, t.pool, t.n_pages, t.n_layers, t.block_bytes, src, dst, moves, t.status);
 }
 
 }  // namespace llm
