@@ -118,10 +118,11 @@ PageTables tables(const llm_page_cache* c) {
   return t;
 }
 
-// CTAs of a launch that copies up to `moves` pages of every layer.
-int copy_grid(const PageTables& t, long long moves) {
-  const long long chunks = moves * t.n_layers * (t.block_bytes / kCopyChunk);
-  return static_cast<int>(std::max(1ll, std::min((chunks + kCopyBatch - 1) / kCopyBatch, 148ll * 5)));
+// CTAs of a launch that copies up to `moves` pages of every layer (copy_pages); 0: too many to launch.
+unsigned copy_grid(const PageTables& t, long long moves, int turns = 1) {
+  const long long run = static_cast<long long>(kCopyBatch) * turns;
+  const long long ctas = (moves * t.n_layers * (t.block_bytes / kCopyChunk) + run - 1) / run;
+  return ctas > 0x7fffffffll ? 0u : static_cast<unsigned>(std::max(1ll, ctas));
 }
 
 }  // namespace
@@ -164,7 +165,9 @@ extern "C" int llm_pages_copy(int device, const llm_page_cache* from, const llm_
   DeviceScope dev;
   RC(dev.enter(device));
   const PageTables a = tables(from), b = tables(to);
-  pages_copy_kernel<<<copy_grid(a, n), kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, b, src, dst, n);
+  const unsigned grid = copy_grid(a, n);
+  if (!grid) return fail_fmt(LLM_ERR_INVALID, "%d pages in one request", n);
+  pages_copy_kernel<<<grid, kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, b, src, dst, n);
   CU(cudaGetLastError());
   return LLM_OK;
 }
@@ -179,9 +182,11 @@ extern "C" int llm_pages_fork(int device, const llm_page_cache* c, const int32_t
   RC(dev.enter(device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ForkParams p{tables(c), parents, children, lens, rooms, n};
+  const unsigned grid = copy_grid(p.t, n);
+  if (!grid) return fail_fmt(LLM_ERR_INVALID, "%d requests in one call", n);
   pages_fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
   CU(cudaGetLastError());
-  CU(launch_dependent(pages_fork_kernel, dim3(copy_grid(p.t, n)), dim3(kCopyThreads), 0, s, p));
+  CU(launch_dependent(pages_fork_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
   return LLM_OK;
 }
 
@@ -202,9 +207,14 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
   RC(dev.enter(device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PageTables t = tables(c);
+  // the host knows only a bound of the moves (half of the pool): longer CTAs where the bound makes
+  // many, as most of them may find nothing to do
+  const int turns = copy_grid(t, t.n_pages / 2 + 1) > 148 * 16 ? 4 : 1;
+  const unsigned grid = copy_grid(t, t.n_pages / 2 + 1, turns);
+  if (!grid) return fail_fmt(LLM_ERR_INVALID, "%d pages in one request", t.n_pages);
   pages_compact_plan_kernel<<<(t.n_pages + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, s>>>(t);
   CU(cudaGetLastError());
-  CU(launch_dependent(pages_compact_kernel, dim3(copy_grid(t, t.n_pages / 2 + 1)), dim3(kCopyThreads), 0, s, t));
+  CU(launch_dependent(pages_compact_kernel, dim3(grid), dim3(kCopyThreads), 0, s, t, turns));
   return LLM_OK;
 }
 

@@ -88,15 +88,19 @@ __device__ __forceinline__ int block_exclusive(int v, int* s, int& total) {
   return s[warp] + x - v;
 }
 
-// Copies page src[i] -> dst[i] in every layer, i < n, over all CTAs of the grid.  Moving a page is
-// its bytes read and written once, so what counts is bytes in flight: a CTA takes kCopyBatch
-// consecutive chunks (16 KB) at a time, every load before the first store, five CTAs to an SM.
-// Chunks run over (move, layer, offset in the block).
+// Copies page src[i] -> dst[i] in every layer, i < n, over the CTAs of the grid.  Moving a page is
+// its bytes read and written once, so what counts is bytes in flight in an order that memory likes: a
+// CTA takes `turns` runs of kCopyBatch consecutive chunks (16 KB), every load of a run before its
+// first store, and the hardware hands out CTAs in order.  Chunks run over (move, layer, offset in the
+// block).  2048 pages of 4 x 64 KiB: 167 us (6430 GB/s, 0.98 of a plain copy); CTAs that stay and stride over
+// the list 171 to 202 us depending on the stride, bulk copies through shared memory 169 to 222 us.
 __device__ __forceinline__ void copy_pages(const uint8_t* from, int from_pages, uint8_t* to, int to_pages, int n_layers,
-                                           int block_bytes, const int* src, const int* dst, int n, int* status) {
+                                           int block_bytes, const int* src, const int* dst, int n, int turns, int* status) {
   const unsigned chunks = block_bytes / kCopyChunk;
   const long long all = static_cast<long long>(n) * n_layers * chunks;
-  for (long long w = static_cast<long long>(blockIdx.x) * kCopyBatch; w < all; w += static_cast<long long>(gridDim.x) * kCopyBatch) {
+  for (int turn = 0; turn < turns; ++turn) {
+    const long long w = (static_cast<long long>(blockIdx.x) * turns + turn) * kCopyBatch;
+    if (w >= all) break;
     const long long blk = w / chunks;
     unsigned chunk = static_cast<unsigned>(w - blk * chunks);
     int i = static_cast<int>(blk / n_layers), layer = static_cast<int>(blk - static_cast<long long>(i) * n_layers);
@@ -111,7 +115,7 @@ __device__ __forceinline__ void copy_pages(const uint8_t* from, int from_pages, 
           if (threadIdx.x == 0) page_fail(status, kPageBadRequest);
         } else {
           const size_t at = static_cast<size_t>(chunk) * kCopyChunk + threadIdx.x * 16;
-          v[u] = *reinterpret_cast<const uint4*>(from + (static_cast<size_t>(layer) * from_pages + a) * block_bytes + at);
+          v[u] = __ldcs(reinterpret_cast<const uint4*>(from + (static_cast<size_t>(layer) * from_pages + a) * block_bytes + at));
           out[u] = to + (static_cast<size_t>(layer) * to_pages + b) * block_bytes + at;
         }
         if (++chunk == chunks) {
@@ -122,13 +126,13 @@ __device__ __forceinline__ void copy_pages(const uint8_t* from, int from_pages, 
     }
 #pragma unroll
     for (int u = 0; u < kCopyBatch; ++u)
-      if (out[u]) *reinterpret_cast<uint4*>(out[u]) = v[u];
+      if (out[u]) __stcs(reinterpret_cast<uint4*>(out[u]), v[u]);
   }
 }
 
 __global__ void __launch_bounds__(kCopyThreads, 5) pages_copy_kernel(PageTables from, PageTables to, const int* src,
                                                                      const int* dst, int n) {
-  copy_pages(from.pool, from.n_pages, to.pool, to.n_pages, from.n_layers, from.block_bytes, src, dst, n, from.status);
+  copy_pages(from.pool, from.n_pages, to.pool, to.n_pages, from.n_layers, from.block_bytes, src, dst, n, 1, from.status);
 }
 
 // ----------------------------------------------------------------------------- fork
@@ -221,7 +225,12 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams 
   if (!work[PageWork::kValid]) return;
   const int* first = work + PageWork::first(p.t.max_seqs);
   const int top = work[PageWork::kCount];  // the stack before this call
-  for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
+  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes,
+             work + PageWork::src(p.t.max_seqs, p.t.n_pages), work + PageWork::dst(p.t.max_seqs, p.t.n_pages),
+             work[PageWork::kMoves], 1, p.t.status);
+  const int rows = min(static_cast<int>(min(gridDim.x, 0x7fffffffu)), p.n);  // the CTAs that fill rows
+  if (static_cast<int>(blockIdx.x) >= rows) return;
+  for (int i = blockIdx.x; i < p.n; i += rows) {
     ForkShape f;
     fork_shape(p, i, f);
     const int par = p.parents[i];
@@ -242,13 +251,10 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams 
       }
     }
   }
-  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes,
-             work + PageWork::src(p.t.max_seqs, p.t.n_pages), work + PageWork::dst(p.t.max_seqs, p.t.n_pages),
-             work[PageWork::kMoves], p.t.status);
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    s_last = atomicAdd(work + PageWork::kTicket, 1) == static_cast<int>(gridDim.x) - 1;
+    s_last = atomicAdd(work + PageWork::kTicket, 1) == rows - 1;
   }
   __syncthreads();
   if (!s_last) return;
@@ -389,7 +395,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTa
 
 // The moves (sources are at or above n_live, destinations below it, so they never overlap), the
 // renamed counts and table entries, and the free stack.
-__global__ void __launch_bounds__(kCopyThreads, 5) pages_compact_kernel(PageTables t) {
+__global__ void __launch_bounds__(kCopyThreads, 4) pages_compact_kernel(PageTables t, int turns) {
   griddep_wait();
   const int* work = t.work;
   const int moves = work[PageWork::kMoves], n_live = work[PageWork::kLive];
@@ -416,7 +422,7 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_compact_kernel(PageTabl
     t.refs[src[k]] = 0;
   }
   for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
-  copy_pages(t.pool, t.n_pages, t.pool, t.n_pages, t.n_layers, t.block_bytes, src, dst, moves, t.status);
+  copy_pages(t.pool, t.n_pages, t.pool, t.n_pages, t.n_layers, t.block_bytes, src, dst, moves, turns, t.status);
 }
 
 }  // namespace llm
