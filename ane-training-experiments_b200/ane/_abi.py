@@ -54,7 +54,7 @@ EXPORTS = [
     "llm_debug_gemm_f16", "llm_debug_read_kv", "llm_gemm_i8_splitk_noalloc", "llm_set_option", "llm_set_sampling", "llm_sample_uniform", "llm_debug_sample", "llm_debug_wait_timeout",
     "llm_eval_window", "llm_debug_exp2", "llm_shard_range", "llm_comm_unique_id", "llm_comm_create",
     "llm_comm_destroy", "llm_gather_tokens", "llm_comm_last_gather_ms", "llm_linear_create", "llm_linear_eval_cf", "llm_linear_destroy",
-    "llm_pages_work_words", "llm_pages_status", "llm_pages_copy", "llm_pages_fork", "llm_pages_free",
+    "llm_seq_fork", "llm_pages_work_words", "llm_pages_status", "llm_pages_copy", "llm_pages_fork", "llm_pages_free",
     "llm_pages_compact", "llm_prefix_plan_create", "llm_prefix_attend", "llm_prefix_plan_destroy",
 ]
 
@@ -75,6 +75,7 @@ LLM_OPT_PREFILL_BN = 14
 LLM_OPT_PREFILL_TC = 15
 LLM_OPT_PREFILL_PERSIST = 16
 LLM_OPT_DECODE_SPLITK = 17
+LLM_OPT_SHARED_PREFIX = 18
 
 
 class LLMError(RuntimeError):
@@ -131,6 +132,7 @@ def lib() -> C.CDLL:
         "llm_synth_stream": (C.c_uint64, [C.c_int, C.c_int]),
         "llm_kv_alloc": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
         "llm_seq_release": (C.c_int, [C.c_void_p, C.c_int]),
+        "llm_seq_fork": (C.c_int, [C.c_void_p, C.c_int, i32p, C.c_int, C.c_int]),
         "llm_prefill": (C.c_int, [C.c_void_p, i32p, i32p, i32p, i32p, C.c_int, i32p, _FP]),
         "llm_decode_step": (C.c_int, [C.c_void_p, i32p, i32p, i32p, C.c_int, i32p, _FP]),
         "llm_generate_begin": (C.c_int, [C.c_void_p, i32p, i32p, i32p, C.c_int, C.c_int]),

@@ -385,6 +385,12 @@ class Engine:
     def release(self, seq: int) -> None:
         _abi.check(_abi.lib().llm_seq_release(self.h, seq))
 
+    def fork(self, parent: int, children, length: int) -> None:
+        """Make the empty slots `children` copies of slot `parent`'s first `length` positions, sharing
+        its complete pages (llm_seq_fork)."""
+        ch = _abi.i32(children)
+        _abi.check(_abi.lib().llm_seq_fork(self.h, parent, _abi.ptr(ch, C.c_int32), len(ch), int(length)))
+
     def prefill(self, seq_ids, prompts: List[List[int]], start_pos=None, want_logits=False):
         seq = _abi.i32(seq_ids)
         lens = _abi.i32([len(p) for p in prompts])

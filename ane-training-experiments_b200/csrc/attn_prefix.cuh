@@ -35,14 +35,17 @@ struct PrefixItem {
 struct PrefixParams {
   const PrefixItem* items;
   const void* q;
-  void* out;
+  void* out;                  // T, or f32 when out_f32
+  int out_f32;
   float* lse;                 // [rows][n_heads] natural log, or nullptr
   long long q_row, q_head;    // strides in elements
   long long o_row, o_head;
   const uint8_t* pool;        // the layer's pages
   const int* table;
-  const int* ctx;             // [n_seqs]
+  const int* ctx;             // [n_seqs] positions, less ctx_add
+  int ctx_add;
   const int* slots;           // [n_seqs]
+  const int* row_map;         // [n_rows] the row of q, out and lse; nullptr: the same
   const int2* row_info;       // [n_rows] sequence, rows of the sequence from this one on
   const int2* joins;          // [n_joins] rows with several states: row, states
   int n_joins;
@@ -55,7 +58,7 @@ struct PrefixParams {
 
 // Positions sequence s has, at most what its table row and the plan cover.
 __device__ __forceinline__ int seq_ctx(const PrefixParams& p, int s) {
-  const int c = p.ctx[s], most = min(p.max_ctx, p.max_pages * 16);
+  const int c = p.ctx[s] + p.ctx_add, most = min(p.max_ctx, p.max_pages * 16);
   if (c > most) page_fail(p.status, kPageBadRequest);
   return max(0, min(c, most));
 }
@@ -65,6 +68,7 @@ __device__ __forceinline__ int row_last(const PrefixParams& p, int row, int& seq
   seq = ri.x;
   return seq_ctx(p, ri.x) - ri.y;
 }
+__device__ __forceinline__ int outer_row(const PrefixParams& p, int row) { return p.row_map ? p.row_map[row] : row; }
 __device__ __forceinline__ int page_entry(const PrefixParams& p, const int* bt, int lp) {
   int e = bt[lp];
   if (e < 0 || e >= p.n_pages) {
@@ -146,7 +150,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   {
     const bool ok = g < it.n_rho;
     const int rho = it.rho0 + (ok ? g : 0);
-    const T* qrow = static_cast<const T*>(p.q) + (it.row0 + rho / group) * p.q_row + (kvh * group + rho % group) * p.q_head;
+    const T* qrow = static_cast<const T*>(p.q) + outer_row(p, it.row0 + rho / group) * p.q_row +
+                    (kvh * group + rho % group) * p.q_head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qb[ks][0] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t) : 0u;
@@ -301,10 +306,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   } else {
     for (int i = threadIdx.x; i < it.n_rho * (HD / 2); i += kAttnWarps * 32) {
       const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
-      const int row = it.row0 + (it.rho0 + c) / group, head = kvh * group + (it.rho0 + c) % group;
+      const int row = outer_row(p, it.row0 + (it.rho0 + c) / group), head = kvh * group + (it.rho0 + c) % group;
       const float l = s_l[c], inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + d) =
-          ActTraits<T>::pack2(stage[c * HD + d] * inv, stage[c * HD + d + 1] * inv);
+      const float x = stage[c * HD + d] * inv, y = stage[c * HD + d + 1] * inv;
+      const long long at = row * p.o_row + head * p.o_head + d;
+      if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = make_float2(x, y);
+      else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at) = ActTraits<T>::pack2(x, y);
       if (p.lse && d == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(s_m[c], l);
     }
   }
@@ -433,9 +440,10 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
   const bool softmax_warp = warp >= 3 && warp <= 10;
   const bool row_ok = softmax_warp && local < it.n_rho;
   const int rho = it.rho0 + (row_ok ? local : 0);
-  const int row = it.row0 + rho / group, head = kvh * group + rho % group;
+  const int head = kvh * group + rho % group;
   int seq = 0;
-  const int lim_row = row_ok ? row_last(p, row, seq) : -1;
+  const int lim_row = row_ok ? row_last(p, it.row0 + rho / group, seq) : -1;
+  const int row = softmax_warp ? outer_row(p, it.row0 + rho / group) : 0;
   if (softmax_warp) {
     const int m = __reduce_max_sync(0xffffffffu, lim_row);
     const int from = __ffs(__ballot_sync(0xffffffffu, lim_row == m)) - 1;
@@ -815,8 +823,11 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int k = r0 + i * PER + lane / CH;
-          if (k < n_w)
-            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s_off[row_w + k] + c * 4) =
+          if (k >= n_w) continue;
+          const long long to = s_off[row_w + k] + c * 4;
+          if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to) = o[i];
+          else
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + to) =
                 make_uint2(ActTraits<T>::pack2(o[i].x, o[i].y), ActTraits<T>::pack2(o[i].z, o[i].w));
         }
       }
@@ -889,11 +900,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
 #pragma unroll
       for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
   }
-  T* out = static_cast<T*>(p.out) + row * p.o_row + head * p.o_head + lane * V;
+  const int to_row = outer_row(p, row);
+  const long long to = to_row * p.o_row + head * p.o_head + lane * V;
   const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
 #pragma unroll
-  for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(out + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(M, L);
+  for (int e = 0; e < V; e += 2) {
+    if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + e) = make_float2(O[e] * inv, O[e + 1] * inv);
+    else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
+  }
+  if (p.lse && lane == 0) p.lse[static_cast<size_t>(to_row) * p.n_heads + head] = natural_lse(M, L);
 }
 
 }  // namespace llm

@@ -12,6 +12,7 @@
 
 #include "../../include/llm_cuda.h"
 #include "attn_prefix.cuh"
+#include "paged.h"
 #include "pages.cuh"
 
 using namespace llm;
@@ -229,7 +230,7 @@ struct llm_prefix_plan {
   const int2* joins = nullptr;
   int n_joins = 0, parts = 0;
   const int2* row_info = nullptr;
-  const int* slots = nullptr;
+  const int *slots = nullptr, *row_map = nullptr;
   float* ws_o = nullptr;
   float2* ws_ml = nullptr;
 };
@@ -390,7 +391,48 @@ cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, cudaS
   return bf ? prefix_launch<__nv_bfloat16, 128>(plan, p, s, prepare) : prefix_launch<__half, 128>(plan, p, s, prepare);
 }
 
+// What a plan fixes of its launches.
+PrefixParams plan_params(const llm_prefix_plan* plan) {
+  PrefixParams p{};
+  p.slots = plan->slots;
+  p.row_info = plan->row_info;
+  p.row_map = plan->row_map;
+  p.joins = plan->joins;
+  p.n_joins = plan->n_joins;
+  p.ws_o = plan->ws_o;
+  p.ws_ml = plan->ws_ml;
+  p.n_rows = plan->n_rows;
+  p.n_heads = plan->n_heads;
+  p.n_kv_heads = plan->n_kv_heads;
+  p.max_ctx = plan->max_ctx;
+  return p;
+}
+
+float scale_log2(double scale) { return static_cast<float>(scale * 1.4426950408889634); }
+
 }  // namespace
+
+cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_rows& r, cudaStream_t s) {
+  PrefixParams p = plan_params(plan);
+  p.q = r.q;
+  p.out = r.out;
+  p.out_f32 = r.out_f32;
+  p.q_row = p.o_row = static_cast<long long>(plan->n_heads) * plan->head_dim;
+  p.q_head = p.o_head = plan->head_dim;
+  p.pool = static_cast<const uint8_t*>(r.layer_pool);
+  p.table = r.table;
+  p.ctx = r.positions;
+  p.ctx_add = 1;
+  p.status = r.status;
+  p.n_pages = r.n_pages;
+  p.max_pages = r.max_pages;
+  p.scale_log2 = scale_log2(1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
+  return prefix_any(plan, p, s, false);
+}
+
+int llm_detail_prefix_launches(const llm_prefix_plan* plan) {
+  return (plan->n_items[kTile] > 0) + (plan->n_items[kCols] > 0) + (plan->n_joins > 0);
+}
 
 extern "C" int llm_prefix_plan_destroy(llm_prefix_plan* plan) {
   if (!plan) return fail_fmt(LLM_ERR_INVALID, "nil plan");
@@ -405,6 +447,13 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
                                       const int32_t* slots, const int32_t* rows, int n_seqs,
                                       const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
                                       llm_prefix_plan** out) {
+  return llm_detail_prefix_create(device, dtype, n_heads, n_kv_heads, head_dim, slots, rows, n_seqs, nullptr, group_sizes,
+                                  prefixes, n_groups, max_ctx, out);
+}
+
+int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads, int head_dim, const int* slots,
+                             const int* rows, int n_seqs, const int* order, const int* group_sizes, const int* prefixes,
+                             int n_groups, int max_ctx, llm_prefix_plan** out) {
   if (!out) return fail_fmt(LLM_ERR_INVALID, "nil output handle");
   *out = nullptr;
   if (dtype != LLM_DTYPE_F16 && dtype != LLM_DTYPE_BF16)
@@ -436,11 +485,20 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     const int group = n_heads / n_kv_heads;
     std::vector<PrefixItem> items[2];
     std::vector<int2> joins;
-    const int parts = plan_items(rows, group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins);
+    // rows in plan order: sequence by sequence as listed; outer[r] is the caller's row
+    std::vector<int> listed(n_seqs), start(1, 0), outer;
+    for (int s = 0; s < n_seqs; ++s) start.push_back(start.back() + rows[s]);
     std::vector<int2> info;
     info.reserve(total);
-    for (int s = 0; s < n_seqs; ++s)
-      for (int r = 0; r < rows[s]; ++r) info.push_back(make_int2(s, rows[s] - r));
+    for (int i = 0; i < n_seqs; ++i) {
+      const int s = order ? order[i] : i;
+      listed[i] = rows[s];
+      for (int r = 0; r < rows[s]; ++r) {
+        info.push_back(make_int2(s, rows[s] - r));
+        if (order) outer.push_back(start[s] + r);
+      }
+    }
+    const int parts = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins);
     DeviceScope dev;
     RC(dev.enter(device));
     p = new llm_prefix_plan;
@@ -472,6 +530,7 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
     const size_t at_info = place(info.data(), info.size() * sizeof(int2));
     const size_t at_slots = place(slots, static_cast<size_t>(n_seqs) * 4);
+    const size_t at_outer = place(outer.data(), outer.size() * 4);
     const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
     const size_t at_ml = (host.size() + 255) / 256 * 256, at_o = (at_ml + states * 8 + 255) / 256 * 256;
     const size_t bytes = at_o + states * head_dim * 4;
@@ -493,6 +552,7 @@ extern "C" int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_
     p->joins = reinterpret_cast<const int2*>(base + at_joins);
     p->row_info = reinterpret_cast<const int2*>(base + at_info);
     p->slots = reinterpret_cast<const int*>(base + at_slots);
+    p->row_map = order ? reinterpret_cast<const int*>(base + at_outer) : nullptr;
     p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
     p->ws_o = reinterpret_cast<float*>(base + at_o);
     *out = p;
@@ -524,7 +584,7 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   if (!std::isfinite(scale)) return fail_fmt(LLM_ERR_INVALID, "scale is not finite");
   DeviceScope dev;
   RC(dev.enter(plan->device));
-  PrefixParams p{};
+  PrefixParams p = plan_params(plan);
   p.q = q;
   p.out = out;
   p.lse = lse;
@@ -536,21 +596,10 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
            static_cast<size_t>(layer) * c->n_pages * c->n_kv_heads * (2 * 16 * 2) * c->head_dim;
   p.table = c->table;
   p.ctx = ctx;
-  p.slots = plan->slots;
-  p.row_info = plan->row_info;
-  p.joins = plan->joins;
-  p.n_joins = plan->n_joins;
-  p.ws_o = plan->ws_o;
-  p.ws_ml = plan->ws_ml;
   p.status = c->status;
-  p.n_rows = plan->n_rows;
-  p.n_heads = plan->n_heads;
-  p.n_kv_heads = plan->n_kv_heads;
   p.n_pages = c->n_pages;
   p.max_pages = c->max_pages;
-  p.max_ctx = plan->max_ctx;
-  const double sc = scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim));
-  p.scale_log2 = static_cast<float>(sc * 1.4426950408889634);
+  p.scale_log2 = scale_log2(scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
   CU(prefix_any(plan, p, static_cast<cudaStream_t>(stream), false));
   return LLM_OK;
 }

@@ -130,6 +130,14 @@ int llm_kv_alloc(llm_ctx *ctx, int max_seqs, int max_pos, int page_tokens);
 /* Return a sequence slot's pages to the pool.  Replaces Decoder.ResetCache
  * (ane/stories/infer.go:62-71) for one slot. */
 int llm_seq_release(llm_ctx *ctx, int seq);
+/* Make each of the n empty slots children[i] a copy of the first `len` positions of slot `parent`
+ * (several samples of one prompt, a common system prompt): complete pages are shared and counted, a
+ * partly filled last page is copied.  Shared pages are read-only: a call that would write a position
+ * inside one fails with LLM_ERR_STATE, so parent and children continue at `len` or later.  A page
+ * returns to the pool when the last slot that holds it is released.  Decode steps read shared pages
+ * once per group of sequences (LLM_OPT_SHARED_PREFIX).  All children are made or none.  No
+ * counterpart in the reference (one cache per decoder, ane/stories/infer.go:113-114). */
+int llm_seq_fork(llm_ctx *ctx, int parent, const int32_t *children, int n, int len);
 
 /* ---------------------------------------------------------------- token loop */
 /* Prefill: for each of `nseq` sequences, run its `lens[i]` prompt tokens (concatenated in
@@ -250,6 +258,10 @@ int llm_debug_sample(int device, const float *logits, int rows, int vocab, float
                                     (default 1; the split per projection is fixed by its shape,
                                     so results do not depend on the batch; the rounding differs
                                     from 0; int8 models never split) */
+#define LLM_OPT_SHARED_PREFIX 18 /* decode steps whose sequences share pages (llm_seq_fork) read them once
+                                    per group: 0 never, 1 when that saves more K/V time than its
+                                    extra launches take (default), 2 always.  Attention sums in
+                                    another order than per sequence; tests bound the difference */
 #define LLM_OPT_ATTN_CHAIN 7   /* overlap mode: a micro-batch's attention launch starts once every CTA of
                                   the other's has started (1, default) or once it completed (0)  */
 /* Set an execution option (0/1 switches; sizes and counts where noted).  Results do not depend
