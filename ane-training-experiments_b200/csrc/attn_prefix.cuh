@@ -44,9 +44,7 @@ struct PrefixParams {
   const int* table;
   const int* ctx;             // [n_seqs] positions, less ctx_add
   int ctx_add;
-  const int* slots;           // [n_seqs]
-  const int* row_map;         // [n_rows] the row of q, out and lse; nullptr: the same
-  const int2* row_info;       // [n_rows] sequence, rows of the sequence from this one on
+  const int4* row_info;       // [n_rows] sequence, its rows from this one on, its slot, the row of q, out and lse
   const int2* joins;          // [n_joins] rows with several states: row, states
   int n_joins;
   float* ws_o;                // [parts][n_kv_heads][n_rows * group][HD] unnormalised sums
@@ -62,13 +60,8 @@ __device__ __forceinline__ int seq_ctx(const PrefixParams& p, int s) {
   if (c > most) page_fail(p.status, kPageBadRequest);
   return max(0, min(c, most));
 }
-// Last position that query row `row` sees (negative: none), and its sequence.
-__device__ __forceinline__ int row_last(const PrefixParams& p, int row, int& seq) {
-  const int2 ri = p.row_info[row];
-  seq = ri.x;
-  return seq_ctx(p, ri.x) - ri.y;
-}
-__device__ __forceinline__ int outer_row(const PrefixParams& p, int row) { return p.row_map ? p.row_map[row] : row; }
+// Last position that a query row sees (negative: none).
+__device__ __forceinline__ int row_last(const PrefixParams& p, const int4& info) { return seq_ctx(p, info.x) - info.y; }
 __device__ __forceinline__ int page_entry(const PrefixParams& p, const int* bt, int lp) {
   int e = bt[lp];
   if (e < 0 || e >= p.n_pages) {
@@ -110,13 +103,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
 
   // last visible position of this lane's two score columns; none for columns past the item
   const int c0 = 2 * t, c1 = 2 * t + 1;
-  int seq = 0, seq1 = 0;
-  const int lim0 = c0 < it.n_rho ? row_last(p, it.row0 + (it.rho0 + c0) / group, seq) : -1;
-  const int lim1 = c1 < it.n_rho ? row_last(p, it.row0 + (it.rho0 + c1) / group, seq1) : -1;
-  if (lim1 > lim0) seq = seq1;
+  const int4 i0 = p.row_info[it.row0 + (it.rho0 + (c0 < it.n_rho ? c0 : 0)) / group];
+  const int4 i1 = p.row_info[it.row0 + (it.rho0 + (c1 < it.n_rho ? c1 : 0)) / group];
+  const int4 ig = p.row_info[it.row0 + (it.rho0 + (g < it.n_rho ? g : 0)) / group];
+  // Q^T fragments: column g of the B operand is score row rho0 + g
+  uint32_t qb[KS][2];
+  {
+    const bool ok = g < it.n_rho;
+    const T* qrow = static_cast<const T*>(p.q) + ig.w * p.q_row + (kvh * group + (it.rho0 + (ok ? g : 0)) % group) * p.q_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qb[ks][0] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t) : 0u;
+      qb[ks][1] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * t) : 0u;
+    }
+  }
+  const int lim0 = c0 < it.n_rho ? row_last(p, i0) : -1;
+  const int lim1 = c1 < it.n_rho ? row_last(p, i1) : -1;
+  int slot = lim1 > lim0 ? i1.z : i0.z;
   const int last = __reduce_max_sync(0xffffffffu, max(lim0, lim1));
   // the sequence that sees furthest names the pages (an idle one's row may be empty)
-  seq = __shfl_sync(0xffffffffu, seq, __ffs(__ballot_sync(0xffffffffu, max(lim0, lim1) == last)) - 1);
+  slot = __shfl_sync(0xffffffffu, slot, __ffs(__ballot_sync(0xffffffffu, max(lim0, lim1) == last)) - 1);
   const int end = min(it.pos1, last + 1);  // positions [it.pos0, end) are read
   const int p_begin = it.pos0 >> 4, p_end = end > it.pos0 ? (end + 15) >> 4 : p_begin;
 
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   float* const slot1 = fold_area + Cfg::SLOT_FLOATS;
   const uint32_t wbase = smem_u32(wbuf);
   const uint32_t bar0 = smem_u32(&bars[warp][0]);
-  const int* bt = p.table + static_cast<size_t>(p.slots[seq]) * p.max_pages;
+  const int* bt = p.table + static_cast<size_t>(slot) * p.max_pages;
   auto page_src = [&](int lp) -> const uint8_t* {
     return p.pool + (static_cast<size_t>(page_entry(p, bt, lp)) * p.n_kv_heads + kvh) * PB;
   };
@@ -145,20 +151,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
     }
   }
   __syncwarp();
-  // Q^T fragments: column g of the B operand is score row rho0 + g.
-  uint32_t qb[KS][2];
-  {
-    const bool ok = g < it.n_rho;
-    const int rho = it.rho0 + (ok ? g : 0);
-    const T* qrow = static_cast<const T*>(p.q) + outer_row(p, it.row0 + rho / group) * p.q_row +
-                    (kvh * group + rho % group) * p.q_head;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qb[ks][0] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t) : 0u;
-      qb[ks][1] = ok ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * t) : 0u;
-    }
-  }
-
   WarpState<KS> st;
   st.clear();
   int seen = 0;       // pages this warp has consumed (ring position)
@@ -306,7 +298,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   } else {
     for (int i = threadIdx.x; i < it.n_rho * (HD / 2); i += kAttnWarps * 32) {
       const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
-      const int row = outer_row(p, it.row0 + (it.rho0 + c) / group), head = kvh * group + (it.rho0 + c) % group;
+      const int row = p.row_info[it.row0 + (it.rho0 + c) / group].w, head = kvh * group + (it.rho0 + c) % group;
       const float l = s_l[c], inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
       const float x = stage[c * HD + d] * inv, y = stage[c * HD + d + 1] * inv;
       const long long at = row * p.o_row + head * p.o_head + d;
@@ -441,13 +433,13 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
   const bool row_ok = softmax_warp && local < it.n_rho;
   const int rho = it.rho0 + (row_ok ? local : 0);
   const int head = kvh * group + rho % group;
-  int seq = 0;
-  const int lim_row = row_ok ? row_last(p, it.row0 + rho / group, seq) : -1;
-  const int row = softmax_warp ? outer_row(p, it.row0 + rho / group) : 0;
+  const int4 info = p.row_info[it.row0 + rho / group];
+  const int row = info.w;
+  const int lim_row = row_ok ? row_last(p, info) : -1;
   if (softmax_warp) {
     const int m = __reduce_max_sync(0xffffffffu, lim_row);
     const int from = __ffs(__ballot_sync(0xffffffffu, lim_row == m)) - 1;
-    if (lane == from) s_last[warp - 3] = make_int2(m, seq);
+    if (lane == from) s_last[warp - 3] = make_int2(m, info.z);
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -505,7 +497,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     const int j = lane / per_page, hh = lane % per_page;
     const uint32_t place = is_v ? j * HALVES * SUB : hh * REGION + j * SUB;
     const uint8_t* const src = p.pool + static_cast<size_t>(kvh) * (2 * 16 * ROWB) + (is_v ? 16 * ROWB : hh * SUB);
-    const int* bt = p.table + static_cast<size_t>(p.slots[far.y]) * p.max_pages + page0;
+    const int* bt = p.table + static_cast<size_t>(far.y) * p.max_pages + page0;
     auto entries = [&](int first_page) -> int {
       const int pg = first_page + lane;
       return pg < n_pages_it ? page_entry(p, bt, pg) : 0;
@@ -858,6 +850,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
   const bool on = unit < p.n_joins * p.n_heads;
   const int2 j = p.joins[on ? unit / p.n_heads : 0];
   const int row = j.x, parts = on ? j.y : 0, head = unit % p.n_heads;
+  const int to_row = p.row_info[row].w;
   const int group = p.n_heads / p.n_kv_heads;
   const size_t step = static_cast<size_t>(p.n_kv_heads) * p.n_rows * group;
   const size_t at = static_cast<size_t>(head / group) * p.n_rows * group + static_cast<size_t>(row) * group + head % group;
@@ -900,7 +893,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
 #pragma unroll
       for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
   }
-  const int to_row = outer_row(p, row);
   const long long to = to_row * p.o_row + head * p.o_head + lane * V;
   const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
 #pragma unroll

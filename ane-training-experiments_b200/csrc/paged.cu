@@ -229,8 +229,7 @@ struct llm_prefix_plan {
   bool pairs = false;  // some item has more than 128 score rows
   const int2* joins = nullptr;
   int n_joins = 0, parts = 0;
-  const int2* row_info = nullptr;
-  const int *slots = nullptr, *row_map = nullptr;
+  const int4* row_info = nullptr;
   float* ws_o = nullptr;
   float2* ws_ml = nullptr;
 };
@@ -394,9 +393,7 @@ cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, cudaS
 // What a plan fixes of its launches.
 PrefixParams plan_params(const llm_prefix_plan* plan) {
   PrefixParams p{};
-  p.slots = plan->slots;
   p.row_info = plan->row_info;
-  p.row_map = plan->row_map;
   p.joins = plan->joins;
   p.n_joins = plan->n_joins;
   p.ws_o = plan->ws_o;
@@ -485,18 +482,15 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     const int group = n_heads / n_kv_heads;
     std::vector<PrefixItem> items[2];
     std::vector<int2> joins;
-    // rows in plan order: sequence by sequence as listed; outer[r] is the caller's row
-    std::vector<int> listed(n_seqs), start(1, 0), outer;
+    // rows in plan order: sequence by sequence as listed
+    std::vector<int> listed(n_seqs), start(1, 0);
     for (int s = 0; s < n_seqs; ++s) start.push_back(start.back() + rows[s]);
-    std::vector<int2> info;
+    std::vector<int4> info;
     info.reserve(total);
     for (int i = 0; i < n_seqs; ++i) {
       const int s = order ? order[i] : i;
       listed[i] = rows[s];
-      for (int r = 0; r < rows[s]; ++r) {
-        info.push_back(make_int2(s, rows[s] - r));
-        if (order) outer.push_back(start[s] + r);
-      }
+      for (int r = 0; r < rows[s]; ++r) info.push_back(make_int4(s, rows[s] - r, slots[s], start[s] + r));
     }
     const int parts = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins);
     DeviceScope dev;
@@ -528,9 +522,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     p->n_joins = static_cast<int>(joins.size());
     p->parts = parts;
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
-    const size_t at_info = place(info.data(), info.size() * sizeof(int2));
-    const size_t at_slots = place(slots, static_cast<size_t>(n_seqs) * 4);
-    const size_t at_outer = place(outer.data(), outer.size() * 4);
+    const size_t at_info = place(info.data(), info.size() * sizeof(int4));
     const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
     const size_t at_ml = (host.size() + 255) / 256 * 256, at_o = (at_ml + states * 8 + 255) / 256 * 256;
     const size_t bytes = at_o + states * head_dim * 4;
@@ -550,9 +542,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     uint8_t* base = static_cast<uint8_t*>(p->block);
     for (int k = 0; k < 2; ++k) p->items[k] = reinterpret_cast<const PrefixItem*>(base + at_items[k]);
     p->joins = reinterpret_cast<const int2*>(base + at_joins);
-    p->row_info = reinterpret_cast<const int2*>(base + at_info);
-    p->slots = reinterpret_cast<const int*>(base + at_slots);
-    p->row_map = order ? reinterpret_cast<const int*>(base + at_outer) : nullptr;
+    p->row_info = reinterpret_cast<const int4*>(base + at_info);
     p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
     p->ws_o = reinterpret_cast<float*>(base + at_o);
     *out = p;
