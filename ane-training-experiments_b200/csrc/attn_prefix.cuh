@@ -47,6 +47,7 @@ struct PrefixParams {
   const int4* row_info;       // [n_rows] sequence, its rows from this one on, its slot, the row of q, out and lse
   const int2* joins;          // [n_joins] rows with several states: row, states
   int n_joins;
+  int* tickets;               // [n_kv_heads], zero between calls: the columns' last CTA of a kv head joins; or nullptr
   float* ws_o;                // [parts][n_kv_heads][n_rows * group][HD] unnormalised sums
   float2* ws_ml;              // [parts][n_kv_heads][n_rows * group] (m in log2 units, l)
   int* status;
@@ -74,6 +75,66 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
   return l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
+// One warp joins the states of (row, head) and writes the output.  Lane k weighs states k and k + 32
+// (kMaxParts is 64); then a lane adds its HD / 32 dimensions of BATCH states at a time: 8, or 20 where
+// rows have more (18 states of 64 rows: 2.5 us after the last item against 4; but 152 registers, which
+// costs 4 us where 4096 rows and heads have four states each).
+constexpr int kMaxParts = 64;
+
+template <typename T, int HD, int BATCH>
+__device__ __forceinline__ void join_states(const PrefixParams& p, int row, int parts, int to_row, int head) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int group = p.n_heads / p.n_kv_heads;
+  const size_t step = static_cast<size_t>(p.n_kv_heads) * p.n_rows * group;
+  const size_t at = static_cast<size_t>(head / group) * p.n_rows * group + static_cast<size_t>(row) * group + head % group;
+  float2 a = make_float2(-INFINITY, 0.f), b = a;
+  if (lane < parts) a = __ldcg(p.ws_ml + at + lane * step);
+  if (lane + 32 < parts) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
+  const float M = warp_max(fmaxf(a.x, b.x));
+  const float mu = M == -INFINITY ? 0.f : M;
+  const float wa = exp2_det_lo(a.x - mu), wb = exp2_det_lo(b.x - mu);
+  float L = a.y * wa + b.y * wb, O[V];
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+#pragma unroll
+  for (int e = 0; e < V; ++e) O[e] = 0.f;
+  const float* src = p.ws_o + at * HD + lane * V;
+  for (int k0 = 0; k0 < parts; k0 += BATCH) {
+    float v[BATCH][V], w[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int k = k0 + i;
+      w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
+      if (k >= parts) w[i] = 0.f;
+      if (w[i] > 0.f) {  // a state without visible positions holds no sums
+        if constexpr (V == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(src + k * step * HD));
+          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(src + k * step * HD));
+          v[i][0] = x.x, v[i][1] = x.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
+  }
+  const long long to = to_row * p.o_row + head * p.o_head + lane * V;
+  const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + e) = make_float2(O[e] * inv, O[e + 1] * inv);
+    else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
+  }
+  if (p.lse && lane == 0) p.lse[static_cast<size_t>(to_row) * p.n_heads + head] = natural_lse(M, L);
+}
+
 // ============================================================================ up to 8 score rows
 // The arithmetic of attn_kernel (attention.cuh): S^T[16 positions x 8 columns] = K . Q^T, online
 // softmax per column, O^T += V^T . P^T with P as two terms; warp w takes pages w, w + 4, ... of
@@ -93,6 +154,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kAttnWarps][STAGES];
   __shared__ float s_m[8], s_l[8];
+  __shared__ int s_last;
 
   griddep_launch_dependents();
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
@@ -306,6 +368,27 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
       else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at) = ActTraits<T>::pack2(x, y);
       if (p.lse && d == 0) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(s_m[c], l);
     }
+  }
+  if (p.tickets) {  // small batches: no join launch; which CTA comes last does not change a sum's order
+    const int units = p.n_joins * group;
+    int2 j = p.joins[min(warp, units - 1) / group];  // the warp's first pair, fetched before it is known to be needed
+    int to_row = p.row_info[j.x].w;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      const int n = gridDim.x / p.n_kv_heads;
+      s_last = atomicAdd(p.tickets + kvh, 1) == n - 1;
+      if (s_last) p.tickets[kvh] = 0;
+    }
+    __syncthreads();
+    if (s_last) {
+      __threadfence();
+      for (int u = warp; u < units; u += kAttnWarps) {
+        if (u != warp) j = p.joins[u / group], to_row = p.row_info[j.x].w;
+        join_states<T, HD, 8>(p, j.x, j.y, to_row, kvh * group + u % group);
+      }
+    }
+    return;
   }
   // the launch ends after the one before it, so that whoever waits for it has waited for both; one
   // CTA sees to that, the others make room
@@ -835,72 +918,16 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
 }
 
 // ============================================================================ states of a row -> output
-// One warp per (row, head).  Lane k weighs states k and k + 32 (kMaxParts is 64); then a lane adds
-// its HD / 32 dimensions of BATCH states at a time: 8, or 20 where rows have more (18 states of 64
-// rows: 2.5 us after the last item against 4; but 152 registers, which costs 4 us where 4096 rows and
-// heads have four states each).
-constexpr int kMaxParts = 64;
 constexpr int kJoinWarps = 4;
 
 template <typename T, int HD, int BATCH>
 __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixParams p) {
-  constexpr int V = HD / 32;
-  const int lane = threadIdx.x & 31;
   const int unit = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const bool on = unit < p.n_joins * p.n_heads;
   const int2 j = p.joins[on ? unit / p.n_heads : 0];
-  const int row = j.x, parts = on ? j.y : 0, head = unit % p.n_heads;
-  const int to_row = p.row_info[row].w;
-  const int group = p.n_heads / p.n_kv_heads;
-  const size_t step = static_cast<size_t>(p.n_kv_heads) * p.n_rows * group;
-  const size_t at = static_cast<size_t>(head / group) * p.n_rows * group + static_cast<size_t>(row) * group + head % group;
+  const int to_row = p.row_info[j.x].w;
   griddep_wait();
-  if (!on) return;
-  float2 a = make_float2(-INFINITY, 0.f), b = a;
-  if (lane < parts) a = __ldcg(p.ws_ml + at + lane * step);
-  if (lane + 32 < parts) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
-  const float M = warp_max(fmaxf(a.x, b.x));
-  const float mu = M == -INFINITY ? 0.f : M;
-  const float wa = exp2_det_lo(a.x - mu), wb = exp2_det_lo(b.x - mu);
-  float L = a.y * wa + b.y * wb, O[V];
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-#pragma unroll
-  for (int e = 0; e < V; ++e) O[e] = 0.f;
-  const float* src = p.ws_o + at * HD + lane * V;
-  for (int k0 = 0; k0 < parts; k0 += BATCH) {
-    float v[BATCH][V], w[BATCH];
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int k = k0 + i;
-      w[i] = __shfl_sync(0xffffffffu, k < 32 ? wa : wb, k & 31);
-      if (k >= parts) w[i] = 0.f;
-      if (w[i] > 0.f) {  // a state without visible positions holds no sums
-        if constexpr (V == 4) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(src + k * step * HD));
-          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-        } else {
-          const float2 x = __ldcg(reinterpret_cast<const float2*>(src + k * step * HD));
-          v[i][0] = x.x, v[i][1] = x.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
-  }
-  const long long to = to_row * p.o_row + head * p.o_head + lane * V;
-  const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
-#pragma unroll
-  for (int e = 0; e < V; e += 2) {
-    if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + e) = make_float2(O[e] * inv, O[e + 1] * inv);
-    else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
-  }
-  if (p.lse && lane == 0) p.lse[static_cast<size_t>(to_row) * p.n_heads + head] = natural_lse(M, L);
+  if (on) join_states<T, HD, BATCH>(p, j.x, j.y, to_row, unit % p.n_heads);
 }
 
 }  // namespace llm

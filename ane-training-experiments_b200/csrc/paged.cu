@@ -88,7 +88,7 @@ int check_geometry(const llm_page_cache* c) {
     return fail_fmt(LLM_ERR_UNSUPPORTED, "head_dim=%d (supported: 64, 128)", c->head_dim);
   if (c->n_layers <= 0 || c->n_pages <= 0 || c->n_kv_heads <= 0 || c->max_seqs <= 0 || c->max_pages <= 0)
     return fail_fmt(LLM_ERR_INVALID, "cache sizes must be positive");
-  if (c->n_kv_heads > 1024 || c->n_pages > (1 << 28) || c->max_seqs > (1 << 24) || c->max_pages > (1 << 24))
+  if (c->n_kv_heads > 1024 || c->n_pages > (1 << 26) || c->max_seqs > (1 << 24) || c->max_pages > (1 << 20))
     return fail_fmt(LLM_ERR_INVALID, "cache sizes out of range");
   if (!c->pool || !aligned(c->pool, 128)) return fail_fmt(LLM_ERR_INVALID, "the pool must be device memory aligned to 128 bytes");
   return LLM_OK;
@@ -129,7 +129,7 @@ unsigned copy_grid(const PageTables& t, long long moves, int turns = 1) {
 }  // namespace
 
 extern "C" size_t llm_pages_work_words(int n_pages, int max_seqs) {
-  if (n_pages <= 0 || max_seqs <= 0 || n_pages > (1 << 28) || max_seqs > (1 << 24)) return 0;
+  if (n_pages <= 0 || max_seqs <= 0 || n_pages > (1 << 26) || max_seqs > (1 << 24)) return 0;
   return PageWork::words(max_seqs, n_pages);
 }
 
@@ -185,6 +185,13 @@ extern "C" int llm_pages_fork(int device, const llm_page_cache* c, const int32_t
   ForkParams p{tables(c), parents, children, lens, rooms, n};
   const unsigned grid = copy_grid(p.t, n);
   if (!grid) return fail_fmt(LLM_ERR_INVALID, "%d requests in one call", n);
+  // one launch where few requests copy little (one sequence into four: 6 us on the device against 8,
+  // and 3 us less on the host)
+  if (n <= kCopyThreads && grid <= 148 * 4) {
+    pages_fork_small_kernel<<<grid, kCopyThreads, 0, s>>>(p);
+    CU(cudaGetLastError());
+    return LLM_OK;
+  }
   pages_fork_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
   CU(cudaGetLastError());
   CU(launch_dependent(pages_fork_kernel, dim3(grid), dim3(kCopyThreads), 0, s, p));
@@ -208,6 +215,13 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
   RC(dev.enter(device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PageTables t = tables(c);
+  const int few = static_cast<int>((copy_grid(t, t.n_pages / 2 + 1) + 148 * 4 - 1) / (148 * 4));
+  // one launch of at most four CTAs an SM (96 pages: as long on the device as two, 3 us less on the host)
+  if (t.n_pages <= kSmallPool && few <= 8) {
+    pages_compact_small_kernel<<<copy_grid(t, t.n_pages / 2 + 1, few), kCopyThreads, 0, s>>>(t, few);
+    CU(cudaGetLastError());
+    return LLM_OK;
+  }
   // the host knows only a bound of the moves (half of the pool): longer CTAs where the bound makes
   // many, as most of them may find nothing to do
   const int turns = copy_grid(t, t.n_pages / 2 + 1) > 148 * 16 ? 4 : 1;
@@ -229,6 +243,7 @@ struct llm_prefix_plan {
   bool pairs = false;  // some item has more than 128 score rows
   const int2* joins = nullptr;
   int n_joins = 0, parts = 0;
+  int* tickets = nullptr;  // [n_kv_heads], where the columns' last CTA joins
   const int4* row_info = nullptr;
   float* ws_o = nullptr;
   float2* ws_ml = nullptr;
@@ -240,6 +255,8 @@ enum { kTile = 0, kCols = 1 };
 constexpr int kOpenEnd = 1 << 30;
 // Cost of starting and ending a CTA, in 64-position steps of its main loop.
 constexpr int kItemOverhead = 4;
+// (row, head) pairs that a warp of a column CTA joins itself before a launch of its own is faster.
+constexpr int kInlineJoins = 4;
 
 struct PlanGroup {
   int seq0, n_seqs, prefix;
@@ -374,7 +391,7 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
       e = launch_dependent(prefix_cols_kernel<T, HD>, grid, block, smem, s, p);
     }
   }
-  if (e == cudaSuccess && plan->n_joins > 0) {
+  if (e == cudaSuccess && plan->n_joins > 0 && !plan->tickets) {
     const long long units = static_cast<long long>(plan->n_joins) * plan->n_heads;
     const dim3 grid(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
     e = plan->parts > 8 ? launch_dependent(prefix_join_kernel<T, HD, 20>, grid, block, 0, s, p)
@@ -396,6 +413,7 @@ PrefixParams plan_params(const llm_prefix_plan* plan) {
   p.row_info = plan->row_info;
   p.joins = plan->joins;
   p.n_joins = plan->n_joins;
+  p.tickets = plan->tickets;
   p.ws_o = plan->ws_o;
   p.ws_ml = plan->ws_ml;
   p.n_rows = plan->n_rows;
@@ -428,7 +446,7 @@ cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_
 }
 
 int llm_detail_prefix_launches(const llm_prefix_plan* plan) {
-  return (plan->n_items[kTile] > 0) + (plan->n_items[kCols] > 0) + (plan->n_joins > 0);
+  return (plan->n_items[kTile] > 0) + (plan->n_items[kCols] > 0) + (plan->n_joins > 0 && !plan->tickets);
 }
 
 extern "C" int llm_prefix_plan_destroy(llm_prefix_plan* plan) {
@@ -523,6 +541,12 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     p->parts = parts;
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
     const size_t at_info = place(info.data(), info.size() * sizeof(int4));
+    // Few rows of column items only: the last CTA of a kv head joins them, at most kInlineJoins
+    // (row, head) pairs a warp.  Four samples: 13.4 us a call, which the host bounds, against 17.8
+    // with a join launch; on the device alone 7.4 us against 5.8 (a fence and a ticket).
+    const std::vector<int> zeros(n_kv_heads, 0);
+    const bool join_inline = items[kTile].empty() && joins.size() * group <= static_cast<size_t>(kInlineJoins * kAttnWarps);
+    const size_t at_tickets = place(zeros.data(), join_inline ? zeros.size() * 4 : 0);
     const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
     const size_t at_ml = (host.size() + 255) / 256 * 256, at_o = (at_ml + states * 8 + 255) / 256 * 256;
     const size_t bytes = at_o + states * head_dim * 4;
@@ -542,6 +566,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     uint8_t* base = static_cast<uint8_t*>(p->block);
     for (int k = 0; k < 2; ++k) p->items[k] = reinterpret_cast<const PrefixItem*>(base + at_items[k]);
     p->joins = reinterpret_cast<const int2*>(base + at_joins);
+    if (join_inline && p->n_joins > 0) p->tickets = reinterpret_cast<int*>(base + at_tickets);
     p->row_info = reinterpret_cast<const int4*>(base + at_info);
     p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
     p->ws_o = reinterpret_cast<float*>(base + at_o);

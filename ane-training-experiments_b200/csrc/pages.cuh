@@ -216,21 +216,17 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParam
   }
 }
 
-// Rows, reference counts and the copies of partly filled pages.  The rows are read while npages
-// still holds the old counts; the last CTA stores the new ones.
-__global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams p) {
-  __shared__ int s_last;
-  griddep_wait();
-  int* const work = p.t.work;
-  if (!work[PageWork::kValid]) return;
-  const int* first = work + PageWork::first(p.t.max_seqs);
-  const int top = work[PageWork::kCount];  // the stack before this call
-  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes,
-             work + PageWork::src(p.t.max_seqs, p.t.n_pages), work + PageWork::dst(p.t.max_seqs, p.t.n_pages),
-             work[PageWork::kMoves], 1, p.t.status);
-  const int rows = min(static_cast<int>(min(gridDim.x, 0x7fffffffu)), p.n);  // the CTAs that fill rows
-  if (static_cast<int>(blockIdx.x) >= rows) return;
-  for (int i = blockIdx.x; i < p.n; i += rows) {
+// Rows and reference counts of a checked request, by the first CTAs of the grid, and the pages per
+// slot by the last of `waits` CTAs to arrive (0: of those that fill rows): the others still read them.
+// *s_last tells the CTA whether it was the last.
+__device__ __forceinline__ void fork_rows(const ForkParams& p, const int* first, int top, int* s_last, int waits = 0) {
+  const int rows = min(static_cast<int>(min(gridDim.x, 0x7fffffffu)), p.n);
+  if (threadIdx.x == 0) *s_last = 0;
+  if (waits == 0 && static_cast<int>(blockIdx.x) >= rows) {
+    __syncthreads();
+    return;
+  }
+  for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
     ForkShape f;
     fork_shape(p, i, f);
     const int par = p.parents[i];
@@ -254,17 +250,68 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams 
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    s_last = atomicAdd(work + PageWork::kTicket, 1) == rows - 1;
+    *s_last = atomicAdd(p.t.work + PageWork::kTicket, 1) == (waits ? waits : rows) - 1;
   }
   __syncthreads();
-  if (!s_last) return;
+  if (!*s_last) return;
   __threadfence();
   for (int i = threadIdx.x; i < p.n; i += kCopyThreads) {
     const int par = p.parents[i], child = p.children[i];
     const int keep = par == child ? p.t.npages[child] : p.lens[i] >> 4;
     p.t.npages[child] = max(keep, (p.rooms[i] + 15) / 16);
   }
-  if (threadIdx.x == 0) work[PageWork::kTicket] = 0;
+}
+
+// Rows, reference counts and the copies of partly filled pages.  The rows are read while npages
+// still holds the old counts; the last CTA stores the new ones.
+__global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_kernel(ForkParams p) {
+  __shared__ int s_last;
+  griddep_wait();
+  int* const work = p.t.work;
+  if (!work[PageWork::kValid]) return;
+  const int* first = work + PageWork::first(p.t.max_seqs);
+  const int top = work[PageWork::kCount];  // the stack before this call
+  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes,
+             work + PageWork::src(p.t.max_seqs, p.t.n_pages), work + PageWork::dst(p.t.max_seqs, p.t.n_pages),
+             work[PageWork::kMoves], 1, p.t.status);
+  fork_rows(p, first, top, &s_last);
+  if (s_last) work[PageWork::kTicket] = 0;
+}
+
+// The same in one launch for at most kCopyThreads requests: every CTA checks and numbers the requests
+// itself (they are few, and a second launch costs more than a CTA's 2 us), so nothing that the
+// checks read may change before the last CTA is done with them.
+__global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_small_kernel(ForkParams p) {
+  __shared__ int s_scan[33], s_first[kCopyThreads], s_child[kCopyThreads], s_src[kCopyThreads], s_dst[kCopyThreads];
+  __shared__ int s_last, s_bad;
+  const int i = threadIdx.x;
+  const int have = *p.t.n_free;
+  ForkShape f{0, 0, false, false};
+  bool bad = i < p.n && !fork_shape(p, i, f);
+  s_child[i] = i < p.n ? p.children[i] : -1 - i;
+  if (i == 0) s_bad = 0;
+  __syncthreads();
+  for (int k = 0; k < i && i < p.n; ++k) bad = bad || s_child[k] == s_child[i];
+  if (bad) s_bad = 1;
+  int total, moves;
+  const int off = block_exclusive(bad ? 0 : f.fresh, s_scan, total);
+  const int at = block_exclusive(!bad && f.tail ? 1 : 0, s_scan, moves);
+  s_first[i] = off;
+  if (!bad && f.tail && off < have) {
+    s_src[at] = p.t.table[static_cast<size_t>(p.parents[i]) * p.t.max_pages + f.keep];
+    s_dst[at] = p.t.free_pages[have - 1 - off];
+  }
+  __syncthreads();
+  if (s_bad || total > have) {  // alike in every CTA
+    if (i == 0 && blockIdx.x == 0) page_fail(p.t.status, s_bad ? kPageBadRequest : kPageExhausted);
+    return;
+  }
+  copy_pages(p.t.pool, p.t.n_pages, p.t.pool, p.t.n_pages, p.t.n_layers, p.t.block_bytes, s_src, s_dst, moves, 1, p.t.status);
+  fork_rows(p, s_first, have, &s_last, gridDim.x);
+  if (s_last && i == 0) {
+    *p.t.n_free = have - total;
+    p.t.work[PageWork::kTicket] = 0;
+  }
 }
 
 // ----------------------------------------------------------------------------- free
@@ -335,6 +382,26 @@ __global__ void __launch_bounds__(kFreeThreads) pages_free_kernel(PageTables t, 
 }
 
 // ----------------------------------------------------------------------------- compact
+// Block-table entries of moved pages renamed (src is ascending), and the new free stack.
+__device__ __forceinline__ void compact_tables(const PageTables& t, const int* src, const int* dst, int moves, int n_live) {
+  const long long tid = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x;
+  const long long step = static_cast<long long>(gridDim.x) * kCopyThreads;
+  const long long entries = static_cast<long long>(t.max_seqs) * t.max_pages;
+  for (long long k = tid; k < entries; k += step) {
+    const int e = t.table[k];
+    if (e < n_live) continue;
+    int lo = 0, hi = moves;  // the rank of e among the sources
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (src[mid] < e) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo < moves && src[lo] == e) t.table[k] = dst[lo];
+    else page_fail(t.status, kDevBadPage);  // an entry whose page has no references
+  }
+  for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
+}
+
 // Live pages as a bit mask; the last CTA lists the moves and the new name of every moved page.
 __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTables t) {
   __shared__ int s_scan[33];
@@ -393,6 +460,54 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTa
   }
 }
 
+// The same as the two kernels above and below in one launch, for pools of at most kSmallPool pages:
+// every CTA lists the moves itself, and the counts, which they all read, change when the last is done.
+constexpr int kSmallPool = 2048;
+__global__ void __launch_bounds__(kCopyThreads, 4) pages_compact_small_kernel(PageTables t, int turns) {
+  __shared__ int s_scan[33], s_src[kSmallPool / 2 + 1], s_dst[kSmallPool / 2 + 1];
+  __shared__ unsigned s_bits[kSmallPool / 32];
+  __shared__ int s_last;
+  constexpr int PER = kSmallPool / kCopyThreads;
+  const int words = (t.n_pages + 31) / 32;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int q = k * kCopyThreads + threadIdx.x;
+    const unsigned live = __ballot_sync(0xffffffffu, q < t.n_pages && t.refs[q] > 0);
+    if ((threadIdx.x & 31) == 0) s_bits[q >> 5] = live;
+  }
+  __syncthreads();
+  const int w = threadIdx.x;
+  const unsigned mine = w < words ? s_bits[w] : 0u;
+  int n_live, moves, same;
+  block_exclusive(__popc(mine), s_scan, n_live);
+  const int lo = n_live - w * 32;  // ids below n_live in this word
+  const unsigned below = lo <= 0 ? 0u : (lo >= 32 ? 0xffffffffu : ~(0xffffffffu << lo));
+  unsigned above = mine & ~below, holes = w < words ? ~mine & below : 0u;
+  int a = block_exclusive(__popc(above), s_scan, moves);
+  int b = block_exclusive(__popc(holes), s_scan, same);
+  for (; above != 0; above &= above - 1) s_src[a++] = w * 32 + __ffs(above) - 1;
+  for (; holes != 0; holes &= holes - 1) s_dst[b++] = w * 32 + __ffs(holes) - 1;
+  __syncthreads();
+  compact_tables(t, s_src, s_dst, moves, n_live);
+  copy_pages(t.pool, t.n_pages, t.pool, t.n_pages, t.n_layers, t.block_bytes, s_src, s_dst, moves, turns, t.status);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(t.work + PageWork::kTicket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int k = threadIdx.x; k < moves; k += kCopyThreads) {
+    t.refs[s_dst[k]] = t.refs[s_src[k]];
+    t.refs[s_src[k]] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *t.n_free = t.n_pages - n_live;
+    t.work[PageWork::kTicket] = 0;
+  }
+}
+
 // The moves (sources are at or above n_live, destinations below it, so they never overlap), the
 // renamed counts and table entries, and the free stack.
 __global__ void __launch_bounds__(kCopyThreads, 4) pages_compact_kernel(PageTables t, int turns) {
@@ -401,27 +516,11 @@ __global__ void __launch_bounds__(kCopyThreads, 4) pages_compact_kernel(PageTabl
   const int moves = work[PageWork::kMoves], n_live = work[PageWork::kLive];
   const int* src = work + PageWork::src(t.max_seqs, t.n_pages);
   const int* dst = work + PageWork::dst(t.max_seqs, t.n_pages);
-  const long long tid = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x;
-  const long long step = static_cast<long long>(gridDim.x) * kCopyThreads;
-  const long long entries = static_cast<long long>(t.max_seqs) * t.max_pages;
-  for (long long k = tid; k < entries; k += step) {
-    const int e = t.table[k];
-    if (e < n_live) continue;
-    // the rank of e among the sources: src is ascending
-    int lo = 0, hi = moves;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (src[mid] < e) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo < moves && src[lo] == e) t.table[k] = dst[lo];
-    else page_fail(t.status, kDevBadPage);  // an entry whose page has no references
-  }
-  for (long long k = tid; k < moves; k += step) {
+  compact_tables(t, src, dst, moves, n_live);
+  for (int k = blockIdx.x * kCopyThreads + threadIdx.x; k < moves; k += gridDim.x * kCopyThreads) {
     t.refs[dst[k]] = t.refs[src[k]];
     t.refs[src[k]] = 0;
   }
-  for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
   copy_pages(t.pool, t.n_pages, t.pool, t.n_pages, t.n_layers, t.block_bytes, src, dst, moves, turns, t.status);
 }
 
