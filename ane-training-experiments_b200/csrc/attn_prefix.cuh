@@ -29,7 +29,15 @@ struct PrefixItem {
   int rho0;        // score rows rho0 .. rho0 + n_rho - 1 counted from row0's first head
   int n_rho;
   int pos0, pos1;  // positions [pos0, pos1), cut at the last one a row of the item sees
-  int part;        // number of the rows' state in the workspace; -1: the item writes the output
+  int span;        // states between one kv head's and the next
+  long long state; // of score row 0 and kv head 0 in the workspace; -1: the item writes the output
+};
+
+// A query row with several states: of head h of kv head k's group, `parts` of them, from
+// state + k * span + h on, span * n_kv_heads apart.
+struct PrefixJoin {
+  int row, parts, span, outer;  // outer: the row of out and lse
+  long long state;
 };
 
 struct PrefixParams {
@@ -45,11 +53,11 @@ struct PrefixParams {
   const int* ctx;             // [n_seqs] positions, less ctx_add
   int ctx_add;
   const int4* row_info;       // [n_rows] sequence, its rows from this one on, its slot, the row of q, out and lse
-  const int2* joins;          // [n_joins] rows with several states: row, states
+  const PrefixJoin* joins;    // [n_joins]
   int n_joins;
   int* tickets;               // [n_kv_heads], zero between calls: the columns' last CTA of a kv head joins; or nullptr
-  float* ws_o;                // [parts][n_kv_heads][n_rows * group][HD] unnormalised sums
-  float2* ws_ml;              // [parts][n_kv_heads][n_rows * group] (m in log2 units, l)
+  float* ws_o;                // [states][HD] unnormalised sums
+  float2* ws_ml;              // [states] (m in log2 units, l)
   int* status;
   int n_rows, n_heads, n_kv_heads, n_pages, max_pages, max_ctx;
   float scale_log2;
@@ -82,12 +90,13 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
 constexpr int kMaxParts = 64;
 
 template <typename T, int HD, int BATCH>
-__device__ __forceinline__ void join_states(const PrefixParams& p, int row, int parts, int to_row, int head) {
+__device__ __forceinline__ void join_states(const PrefixParams& p, const PrefixJoin& j, int head) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x & 31;
   const int group = p.n_heads / p.n_kv_heads;
-  const size_t step = static_cast<size_t>(p.n_kv_heads) * p.n_rows * group;
-  const size_t at = static_cast<size_t>(head / group) * p.n_rows * group + static_cast<size_t>(row) * group + head % group;
+  const int parts = j.parts;
+  const size_t step = static_cast<size_t>(p.n_kv_heads) * j.span;
+  const size_t at = j.state + static_cast<size_t>(head / group) * j.span + head % group;
   float2 a = make_float2(-INFINITY, 0.f), b = a;
   if (lane < parts) a = __ldcg(p.ws_ml + at + lane * step);
   if (lane + 32 < parts) b = __ldcg(p.ws_ml + at + (lane + 32) * step);
@@ -125,14 +134,14 @@ __device__ __forceinline__ void join_states(const PrefixParams& p, int row, int 
 #pragma unroll
       for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
   }
-  const long long to = to_row * p.o_row + head * p.o_head + lane * V;
+  const long long to = j.outer * p.o_row + head * p.o_head + lane * V;
   const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
 #pragma unroll
   for (int e = 0; e < V; e += 2) {
     if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + e) = make_float2(O[e] * inv, O[e + 1] * inv);
     else *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + e) = ActTraits<T>::pack2(O[e] * inv, O[e + 1] * inv);
   }
-  if (p.lse && lane == 0) p.lse[static_cast<size_t>(to_row) * p.n_heads + head] = natural_lse(M, L);
+  if (p.lse && lane == 0) p.lse[static_cast<size_t>(j.outer) * p.n_heads + head] = natural_lse(M, L);
 }
 
 // ============================================================================ up to 8 score rows
@@ -351,9 +360,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
     }
   }
   __syncthreads();
-  if (it.part >= 0) {
-    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * p.n_rows * group +
-                      static_cast<size_t>(it.row0) * group + it.rho0;
+  if (it.state >= 0) {
+    const size_t at = it.state + static_cast<size_t>(kvh) * it.span;
     for (int i = threadIdx.x; i < it.n_rho * HD / 4; i += kAttnWarps * 32)
       __stcg(reinterpret_cast<float4*>(p.ws_o + at * HD) + i, reinterpret_cast<const float4*>(stage)[i]);
     if (threadIdx.x < it.n_rho) __stcg(p.ws_ml + at + threadIdx.x, make_float2(s_m[threadIdx.x], s_l[threadIdx.x]));
@@ -371,8 +379,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   }
   if (p.tickets) {  // small batches: no join launch; which CTA comes last does not change a sum's order
     const int units = p.n_joins * group;
-    int2 j = p.joins[min(warp, units - 1) / group];  // the warp's first pair, fetched before it is known to be needed
-    int to_row = p.row_info[j.x].w;
+    PrefixJoin j = p.joins[min(warp, units - 1) / group];  // the warp's first pair, fetched before it is known to be needed
     __syncthreads();
     if (threadIdx.x == 0) {
       __threadfence();
@@ -384,8 +391,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
     if (s_last) {
       __threadfence();
       for (int u = warp; u < units; u += kAttnWarps) {
-        if (u != warp) j = p.joins[u / group], to_row = p.row_info[j.x].w;
-        join_states<T, HD, 8>(p, j.x, j.y, to_row, kvh * group + u % group);
+        if (u != warp) j = p.joins[u / group];
+        join_states<T, HD, 8>(p, j, kvh * group + u % group);
       }
     }
     return;
@@ -852,8 +859,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     }
     s_ml[mine] = make_float2(m_ref, l_run);
     s_off[mine] = row * p.o_row + head * p.o_head;
-    const size_t at = (static_cast<size_t>(it.part) * p.n_kv_heads + kvh) * p.n_rows * group +
-                      static_cast<size_t>(it.row0) * group + it.rho0;
+    const size_t at = it.state + static_cast<size_t>(kvh) * it.span;  // of the item's score row 0
     if (!pair) streams_bar();
     float m = m_ref, l = l_run, w = l_run > 0.f ? 1.f : 0.f;  // the row's state, and this stream's weight in it
     if (!pair) {
@@ -864,10 +870,10 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
       l = l_run * w + other.y * ex2_approx(other.x - mu);
     }
     if (row_ok && (pair || sg == 0)) {
-      if (it.part >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
+      if (it.state >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
       else if (p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
     }
-    s_w[mine] = it.part < 0 && l > 0.f ? __fdiv_rn(w, l) : w;
+    s_w[mine] = it.state < 0 && l > 0.f ? __fdiv_rn(w, l) : w;
     if (pair) __syncwarp();
     else streams_bar();
     // rows of this warp: its own 32 of a pair; 16 of the tile, from both streams, otherwise
@@ -889,7 +895,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
           if (wb > 0.f) o[i] = make_float4(o[i].x + y.x * wb, o[i].y + y.y * wb, o[i].z + y.z * wb, o[i].w + y.w * wb);
         }
       }
-      if (it.part >= 0) {
+      if (it.state >= 0) {
         float4* dst = reinterpret_cast<float4*>(p.ws_o + (at + row_w + r0 + lane / CH) * HD) + c;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -924,10 +930,9 @@ template <typename T, int HD, int BATCH>
 __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixParams p) {
   const int unit = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const bool on = unit < p.n_joins * p.n_heads;
-  const int2 j = p.joins[on ? unit / p.n_heads : 0];
-  const int to_row = p.row_info[j.x].w;
+  const PrefixJoin j = p.joins[on ? unit / p.n_heads : 0];
   griddep_wait();
-  if (on) join_states<T, HD, BATCH>(p, j.x, j.y, to_row, unit % p.n_heads);
+  if (on) join_states<T, HD, BATCH>(p, j, unit % p.n_heads);
 }
 
 }  // namespace llm

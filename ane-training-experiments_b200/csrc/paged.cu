@@ -241,7 +241,7 @@ struct llm_prefix_plan {
   const PrefixItem* items[2] = {};  // [tile, columns]
   int n_items[2] = {};
   bool pairs = false;  // some item has more than 128 score rows
-  const int2* joins = nullptr;
+  const PrefixJoin* joins = nullptr;
   int n_joins = 0, parts = 0;
   int* tickets = nullptr;  // [n_kv_heads], where the columns' last CTA joins
   const int4* row_info = nullptr;
@@ -293,9 +293,11 @@ int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, 
   return static_cast<int>(std::min(best, longest) * 64);
 }
 
-// The items of a batch and the rows with several states.  Returns the most states of a row.
-int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
-               int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2], std::vector<int2>& joins) {
+// The items of a batch and the rows with several states (the caller fills in their outer rows).
+// Returns the number of states in all; *most is a row's most.
+long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
+                     int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2],
+                     std::vector<PrefixJoin>& joins, int* most) {
   std::vector<PlanGroup> groups;
   std::vector<int> row_start(1, 0);
   long long own_ctas = 0;
@@ -320,14 +322,18 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
   const int pieces = own_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, own_ctas)));
   const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim)),
                       part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim))};
-  int most = 0;
-  auto add = [&items](int row0, long long rho, int pos0, int pos1, int part) {
-    for (long long r = tiles_of(rho) - 1; r >= 0; --r)  // later rows see further: longest first
-      items[kind_of(rho)].push_back({row0, static_cast<int>(r * kTileRows),
-                                     static_cast<int>(std::min<long long>(kTileRows, rho - r * kTileRows)), pos0, pos1, part});
-  };
+  *most = 0;
+  // A group's states lie together: [parts][n_kv_heads][the group's score rows], from `states` on.
+  long long states = 0;
   for (const PlanGroup& g : groups) {
-    int shared_parts = 0;
+    auto add = [&](int row0, long long rho, int pos0, int pos1, int part) {
+      const long long at = part < 0 ? -1 : states + part * n_kv_heads * g.rho + (row0 - row_start[g.seq0]) * static_cast<long long>(group);
+      for (long long r = tiles_of(rho) - 1; r >= 0; --r)  // later rows see further: longest first
+        items[kind_of(rho)].push_back({row0, static_cast<int>(r * kTileRows),
+                                       static_cast<int>(std::min<long long>(kTileRows, rho - r * kTileRows)), pos0, pos1,
+                                       static_cast<int>(g.rho), at < 0 ? -1 : at + r * kTileRows});
+    };
+    int shared_parts = 0, group_parts = 0;
     if (g.shared)
       for (int pos = 0, c = len[kind_of(g.rho)]; pos < g.prefix; pos += c, ++shared_parts)
         add(row_start[g.seq0], g.rho, pos, std::min(g.prefix, pos + c), shared_parts);
@@ -344,16 +350,20 @@ int plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* p
       } else {
         for (int pos = start; pos < max_ctx; pos += piece) add(row_start[s], rho, pos, pos + piece, parts++);
       }
-      for (int r = 0; parts > 0 && r < rows[s]; ++r) joins.push_back(make_int2(row_start[s] + r, parts));
-      most = std::max(most, parts);
+      for (int r = 0; parts > 0 && r < rows[s]; ++r)
+        joins.push_back({row_start[s] + r, parts, static_cast<int>(g.rho), 0,
+                         states + (row_start[s] + r - row_start[g.seq0]) * static_cast<long long>(group)});
+      group_parts = std::max(group_parts, parts);
     }
+    *most = std::max(*most, group_parts);
+    states += group_parts * n_kv_heads * g.rho;
   }
   for (auto& v : items)
     std::stable_sort(v.begin(), v.end(), [max_ctx](const PrefixItem& a, const PrefixItem& b) {
       auto cost = [max_ctx](const PrefixItem& i) { return (std::min(i.pos1, max_ctx) - i.pos0) * (i.n_rho > 128 ? 2ll : 1ll); };
       return cost(a) > cost(b);
     });
-  return most;
+  return states;
 }
 
 template <typename T, int HD>
@@ -499,7 +509,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
   try {
     const int group = n_heads / n_kv_heads;
     std::vector<PrefixItem> items[2];
-    std::vector<int2> joins;
+    std::vector<PrefixJoin> joins;
     // rows in plan order: sequence by sequence as listed
     std::vector<int> listed(n_seqs), start(1, 0);
     for (int s = 0; s < n_seqs; ++s) start.push_back(start.back() + rows[s]);
@@ -510,7 +520,9 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
       listed[i] = rows[s];
       for (int r = 0; r < rows[s]; ++r) info.push_back(make_int4(s, rows[s] - r, slots[s], start[s] + r));
     }
-    const int parts = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins);
+    int parts = 0;
+    const long long n_states = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins, &parts);
+    for (PrefixJoin& j : joins) j.outer = info[j.row].w;
     DeviceScope dev;
     RC(dev.enter(device));
     p = new llm_prefix_plan;
@@ -539,7 +551,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     for (const PrefixItem& it : items[kTile]) p->pairs = p->pairs || it.n_rho > 128;
     p->n_joins = static_cast<int>(joins.size());
     p->parts = parts;
-    const size_t at_joins = place(joins.data(), joins.size() * sizeof(int2));
+    const size_t at_joins = place(joins.data(), joins.size() * sizeof(PrefixJoin));
     const size_t at_info = place(info.data(), info.size() * sizeof(int4));
     // Few rows of column items only: the last CTA of a kv head joins them, at most kInlineJoins
     // (row, head) pairs a warp.  Four samples: 13.4 us a call, which the host bounds, against 17.8
@@ -547,7 +559,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     const std::vector<int> zeros(n_kv_heads, 0);
     const bool join_inline = items[kTile].empty() && joins.size() * group <= static_cast<size_t>(kInlineJoins * kAttnWarps);
     const size_t at_tickets = place(zeros.data(), join_inline ? zeros.size() * 4 : 0);
-    const size_t states = static_cast<size_t>(parts) * n_kv_heads * p->n_rows * group;
+    const size_t states = static_cast<size_t>(n_states);
     const size_t at_ml = (host.size() + 255) / 256 * 256, at_o = (at_ml + states * 8 + 255) / 256 * 256;
     const size_t bytes = at_o + states * head_dim * 4;
     cudaError_t e = cudaMalloc(&p->block, bytes);
@@ -565,7 +577,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     }
     uint8_t* base = static_cast<uint8_t*>(p->block);
     for (int k = 0; k < 2; ++k) p->items[k] = reinterpret_cast<const PrefixItem*>(base + at_items[k]);
-    p->joins = reinterpret_cast<const int2*>(base + at_joins);
+    p->joins = reinterpret_cast<const PrefixJoin*>(base + at_joins);
     if (join_inline && p->n_joins > 0) p->tickets = reinterpret_cast<int*>(base + at_tickets);
     p->row_info = reinterpret_cast<const int4*>(base + at_info);
     p->ws_ml = reinterpret_cast<float2*>(base + at_ml);
