@@ -424,27 +424,28 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
 // only: a stream that does not see the fill of a stage's previous tile (the other stream's) could
 // ask for the next one while that fill is still under way, and a parity wait two phases behind
 // returns at once.
-template <typename T, int HD, bool WIDE>
+// Batches of many short ranges take one stream a CTA (STREAMS = 1, 128 rows) and two CTAs an SM: what
+// they wait for is a CTA's start and end, about 7 us, which then overlap.
+template <typename T, int HD, int STREAMS, bool WIDE>
 struct PrefixTileCfg {
   static constexpr int HALVES = HD / 64;              // 64-element halves of a K / V row
   static constexpr int SUB = 16 * 128;                // one page's half sub-block (bytes)
   static constexpr int REGION = 4 * SUB;              // 64 positions of one half (bytes)
   static constexpr int TILE_BYTES = HALVES * REGION;  // K (or V) of one 64-position tile
-  static constexpr int STAGES = HD == 64 ? (WIDE ? 10 : 6) : (WIDE ? 5 : 4);  // of K and of V
+  static constexpr int STAGES = STREAMS == 1 ? (HD == 64 ? 5 : 2) : HD == 64 ? (WIDE ? 10 : 6) : (WIDE ? 5 : 4);  // of K and of V
   static constexpr int Q_BYTES = HALVES * 128 * 128;  // 128 rows x HD, K-major halves
   static constexpr int K_RING = (WIDE ? 2 : 1) * Q_BYTES;
   static constexpr int V_RING = K_RING + STAGES * TILE_BYTES;
-  static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr uint32_t TMEM_COLS = 256 * STREAMS;
+  static constexpr int THREADS = STREAMS == 1 ? 256 : 384;
   static constexpr float RESCALE_LOG2 = 8.0f;
   static constexpr int ROW_BYTES = HD * 4;            // of a row's sums, staged over Q and the rings
-  static constexpr int META = 256 * (ROW_BYTES + 20);
+  static constexpr int META = 128 * STREAMS * (ROW_BYTES + 20);
   static constexpr int USED = V_RING + STAGES * TILE_BYTES;
   static constexpr int BARS = (USED > META ? USED : META);  // the barriers lie behind the rings
   static constexpr int SMEM = BARS + 512;
 };
-constexpr int kTileThreads = 384;
-constexpr int kTileRows = 256;  // score rows of a tile item
-constexpr int kColRows = 8;     // score rows of a column item
+constexpr int kColRows = 8;  // score rows of a column item
 
 __device__ __forceinline__ float ex2_approx(float x) {  // 2 ulp; 0 for -inf
   float y;
@@ -481,9 +482,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void streams_bar() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
 
-template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 512: at most 128 registers
-  using Cfg = PrefixTileCfg<T, HD, WIDE>;
+template <typename T, int HD, int STREAMS, bool WIDE>
+__global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1)  // both: at most 128 registers
+    prefix_tile_kernel(PrefixParams p) {
+  using Cfg = PrefixTileCfg<T, HD, STREAMS, WIDE>;
+  constexpr int V_WARP = STREAMS == 1 ? 7 : 11;  // fetches V
   constexpr int ST = Cfg::STAGES;
   constexpr int HALVES = Cfg::HALVES;
   constexpr int SUB = Cfg::SUB;
@@ -514,12 +517,13 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
   const int kvh = blockIdx.x % p.n_kv_heads;
   const int group = p.n_heads / p.n_kv_heads;
-  const bool pair = WIDE && it.n_rho > 128;  // two row tiles; otherwise even and odd K/V tiles
+  const bool pair = WIDE && it.n_rho > 128;    // two row tiles
+  const bool apart = pair || STREAMS == 1;     // a stream has every K/V tile; otherwise the even or the odd ones
   // warps 3..10: stream, TMEM lane, score row and the last position it sees
-  const int sg = warp >= 7 ? 1 : 0;
+  const int sg = STREAMS == 2 && warp >= 7 ? 1 : 0;
   const int tl = (warp & 3) * 32 + lane;
   const int local = pair ? sg * 128 + tl : tl;
-  const bool softmax_warp = warp >= 3 && warp <= 10;
+  const bool softmax_warp = warp >= 3 && warp < 3 + 4 * STREAMS;
   const bool row_ok = softmax_warp && local < it.n_rho;
   const int rho = it.rho0 + (row_ok ? local : 0);
   const int head = kvh * group + rho % group;
@@ -545,8 +549,8 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
       }
       mbar_init(smem_u32(&pv_done[g]), 1);
     }
-    mbar_init(smem_u32(&q_ready), 256);
-    mbar_init(smem_u32(&drain), 2);
+    mbar_init(smem_u32(&q_ready), 128 * STREAMS);
+    mbar_init(smem_u32(&drain), STREAMS);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -563,24 +567,24 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
   // the sequence that sees furthest names the pages (an idle one's row may be empty)
   int2 far = s_last[0];
 #pragma unroll
-  for (int w = 1; w < 8; ++w)
+  for (int w = 1; w < 4 * STREAMS; ++w)
     if (s_last[w].x > far.x) far = s_last[w];
   const int last = far.x;
   const int end = min(it.pos1, last + 1);  // positions [it.pos0, end) are read
   const int nkv = end > it.pos0 ? (end - it.pos0 + 63) >> 6 : 0;
   const int page0 = it.pos0 >> 4;
   const int n_pages_it = nkv > 0 ? ((end + 15) >> 4) - page0 : 0;
-  // steps of each stream; step u of stream g works on K/V tile (pair ? u : 2 u + g)
-  const int n0 = pair ? nkv : (nkv + 1) >> 1, n1 = pair ? nkv : nkv >> 1;
-  const int ring = pair ? ST : ST & ~1;  // stages in use
+  // steps of each stream; step u of stream g works on K/V tile (apart ? u : 2 u + g)
+  const int n0 = apart ? nkv : (nkv + 1) >> 1, n1 = apart ? nkv : nkv >> 1;
+  const int ring = apart ? ST : ST & ~1;  // stages in use
   bool failed = false;
 
-  if (warp == 0 || warp == 11) {
+  if (warp == 0 || warp == V_WARP) {
     // ------------------------------------------------------------ bulk-copy producers
     // Warp 0 fetches K, warp 11 V (one warp issues a copy each 50 to 80 clocks).  A warp reads the
     // block table 32 pages (8 tiles) per coalesced load, one batch ahead of use, and a lane issues
     // each copy: a page's half sub-block of K, both halves of V at once.
-    const bool is_v = warp == 11;
+    const bool is_v = warp == V_WARP;
     const uint32_t stages = is_v ? v_ring : k_ring;
     const uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
     const int per_page = is_v ? 1 : HALVES, size = is_v ? HALVES * SUB : SUB;
@@ -617,7 +621,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
         const int uses = turn + (i < st ? 1 : 0);
         if (uses > 0) mbar_poll(smem_u32(&full[i]), (uses - 1) & 1);
       }
-  } else if (warp <= 2) {
+  } else if (warp <= STREAMS) {
     // ------------------------------------------------------------ MMA issuer of stream warp - 1
     const int g = warp - 1;
     const int steps = __shfl_sync(0xffffffffu, g ? n1 : n0, 0);
@@ -627,9 +631,9 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     const uint64_t qd = sw128_desc(q_s + (pair ? g * Cfg::Q_BYTES : 0));
     const uint64_t kd0 = sw128_desc(k_ring), vd0 = sw128_desc_mn(v_ring, SUB, 1024);
     // stage and parity of the next K and of the next V tile of this stream
-    int ks = pair ? 0 : g, kpar = 0, vs = ks, vpar = 0;
+    int ks = apart ? 0 : g, kpar = 0, vs = ks, vpar = 0;
     auto advance = [&](int& st, int& par) {
-      st += pair ? 1 : 2;
+      st += apart ? 1 : 2;
       if (st >= ring) st -= ring, par ^= 1;
     };
     // S of step u into the stream's buffer u & 1, whose P the stream's PV(u - 2) has read
@@ -688,7 +692,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     if (elect_one()) tc_commit(smem_u32(&drain));
     __syncwarp();
     mbar_poll(smem_u32(&drain), 0);
-  } else {
+  } else if (softmax_warp) {
     // ------------------------------------------------------------ softmax / epilogue warps
     const int lim = min(lim_row, end - 1);     // last visible position of this row in the range
     const bool busy = __any_sync(0xffffffffu, row_ok);  // some row of this warp is the item's
@@ -700,7 +704,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
       constexpr int CH = HD / 8, N = CH;  // 16-byte chunks of a row; loads per lane for 32 rows
       const long long off = row * p.q_row + head * p.q_head;
       const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
-      const int i0 = pair || sg == 0 ? 0 : N / 2, i1 = pair || sg == 1 ? N : N / 2;
+      const int i0 = apart || sg == 0 ? 0 : N / 2, i1 = apart || sg == 1 ? N : N / 2;
       uint4 v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -725,7 +729,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     bool ok = true;
     const int steps = sg ? n1 : n0;
     for (int u = 0; u < steps; ++u) {
-      const int t = pair ? u : 2 * u + sg;
+      const int t = apart ? u : 2 * u + sg;
       // wait results are made warp-uniform: the TMEM accesses below are warp-collective
       if (!__all_sync(0xffffffffu, mbar_poll(smem_u32(&s_full[sg][u & 1]), (u >> 1) & 1))) {
         ok = false;
@@ -842,9 +846,9 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     // consecutive lanes on its columns.
     constexpr int CH = HD / 4;  // 16-byte chunks of a row's sums
     float4* const stage = reinterpret_cast<float4*>(gbase);
-    float2* const s_ml = reinterpret_cast<float2*>(gbase + 256 * Cfg::ROW_BYTES);  // [256]
-    long long* const s_off = reinterpret_cast<long long*>(s_ml + 256);             // [256] of the output row
-    float* const s_w = reinterpret_cast<float*>(s_off + 256);                      // [256]
+    float2* const s_ml = reinterpret_cast<float2*>(gbase + 128 * STREAMS * Cfg::ROW_BYTES);  // [128 STREAMS]
+    long long* const s_off = reinterpret_cast<long long*>(s_ml + 128 * STREAMS);  // [128 STREAMS] of the output row
+    float* const s_w = reinterpret_cast<float*>(s_off + 128 * STREAMS);            // [128 STREAMS]
     const int mine = sg * 128 + tl;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
@@ -860,24 +864,24 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
     s_ml[mine] = make_float2(m_ref, l_run);
     s_off[mine] = row * p.o_row + head * p.o_head;
     const size_t at = it.state + static_cast<size_t>(kvh) * it.span;  // of the item's score row 0
-    if (!pair) streams_bar();
+    if (!apart) streams_bar();
     float m = m_ref, l = l_run, w = l_run > 0.f ? 1.f : 0.f;  // the row's state, and this stream's weight in it
-    if (!pair) {
+    if (!apart) {
       const float2 other = s_ml[(1 - sg) * 128 + tl];
       m = fmaxf(m_ref, other.x);
       const float mu = m == -INFINITY ? 0.f : m;
       w = ex2_approx(m_ref - mu);  // 0 where this stream saw nothing
       l = l_run * w + other.y * ex2_approx(other.x - mu);
     }
-    if (row_ok && (pair || sg == 0)) {
+    if (row_ok && (apart || sg == 0)) {
       if (it.state >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
       else if (p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
     }
     s_w[mine] = it.state < 0 && l > 0.f ? __fdiv_rn(w, l) : w;
-    if (pair) __syncwarp();
+    if (apart) __syncwarp();
     else streams_bar();
-    // rows of this warp: its own 32 of a pair; 16 of the tile, from both streams, otherwise
-    const int rows_w = pair ? 32 : 16, row_w = pair ? sg * 128 + (warp & 3) * 32 : (sg * 4 + (warp & 3)) * 16;
+    // rows of this warp: its own 32; or 16 of the tile, from both streams
+    const int rows_w = apart ? 32 : 16, row_w = apart ? sg * 128 + (warp & 3) * 32 : (sg * 4 + (warp & 3)) * 16;
     const int n_w = min(rows_w, it.n_rho - row_w);
     constexpr int PER = 32 / CH;  // rows a warp stores at once
     const int c = lane % CH;
@@ -889,7 +893,7 @@ __global__ void __launch_bounds__(512) prefix_tile_kernel(PrefixParams p) {  // 
         const float wa = s_w[rr];
         const float4 x = stage[rr * CH + (c ^ (rr & (CH - 1)))];  // not finite where the row saw nothing
         o[i] = wa > 0.f ? make_float4(x.x * wa, x.y * wa, x.z * wa, x.w * wa) : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!pair) {
+        if (!apart) {
           const float wb = s_w[128 + rr];
           const float4 y = stage[(128 + rr) * CH + (c ^ (rr & (CH - 1)))];
           if (wb > 0.f) o[i] = make_float4(o[i].x + y.x * wb, o[i].y + y.y * wb, o[i].z + y.z * wb, o[i].w + y.w * wb);

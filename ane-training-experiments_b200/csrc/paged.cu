@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -240,7 +241,7 @@ struct llm_prefix_plan {
   void* block = nullptr;  // one device allocation: items, row_info, slots, states, sums
   const PrefixItem* items[2] = {};  // [tile, columns]
   int n_items[2] = {};
-  bool pairs = false;  // some item has more than 128 score rows
+  int variant = 0;  // of the tile kernel: kWide, kNarrow, kSingle
   const PrefixJoin* joins = nullptr;
   int n_joins = 0, parts = 0;
   int* tickets = nullptr;  // [n_kv_heads], where the columns' last CTA joins
@@ -252,6 +253,7 @@ struct llm_prefix_plan {
 namespace {
 
 enum { kTile = 0, kCols = 1 };
+enum { kWide, kNarrow, kSingle };  // two streams with pairs, two without, one
 constexpr int kOpenEnd = 1 << 30;
 // Cost of starting and ending a CTA, in 64-position steps of its main loop.
 constexpr int kItemOverhead = 4;
@@ -264,17 +266,17 @@ struct PlanGroup {
   long long rho;  // score rows per kv head
 };
 
-long long tiles_of(long long rho) { return (rho + kTileRows - 1) / kTileRows; }
+long long tiles_of(long long rho, int rows) { return (rho + rows - 1) / rows; }
 int kind_of(long long rho) { return rho > kColRows ? kTile : kCols; }
 int kernel_slots(int kind, int head_dim) { return 148 * (kind == kTile ? 1 : head_dim == 64 ? 5 : 3); }
 
 // Positions per item of the shared prefixes: a multiple of 64 that finishes first when every CTA
 // slot takes ceil(items / slots) items of that length.
-int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, int slots) {
+int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, int slots, int tile_rows) {
   long long work = 0, longest = 0;
   for (const PlanGroup& g : groups) {
     if (!g.shared || kind_of(g.rho) != kind) continue;
-    work += tiles_of(g.rho) * n_kv_heads * ((g.prefix + 63) / 64);
+    work += tiles_of(g.rho, tile_rows) * n_kv_heads * ((g.prefix + 63) / 64);
     longest = std::max<long long>(longest, (g.prefix + 63) / 64);
   }
   if (work == 0) return 64;
@@ -285,7 +287,7 @@ int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, 
       if (c < 1) continue;
       long long items = 0;
       for (const PlanGroup& g : groups)
-        if (g.shared && kind_of(g.rho) == kind) items += tiles_of(g.rho) * n_kv_heads * (((g.prefix + 63) / 64 + c - 1) / c);
+        if (g.shared && kind_of(g.rho) == kind) items += tiles_of(g.rho, tile_rows) * n_kv_heads * (((g.prefix + 63) / 64 + c - 1) / c);
       const long long cost = ((items + slots - 1) / slots) * (std::min(c, longest) + kItemOverhead);
       if (best_cost < 0 || cost < best_cost) best = c, best_cost = cost;
     }
@@ -296,7 +298,7 @@ int part_length(const std::vector<PlanGroup>& groups, int kind, int n_kv_heads, 
 // The items of a batch and the rows with several states (the caller fills in their outer rows).
 // Returns the number of states in all; *most is a row's most.
 long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int32_t* prefixes, int n_groups, int max_ctx,
-                     int group, int n_kv_heads, int head_dim, std::vector<PrefixItem> (&items)[2],
+                     int group, int n_kv_heads, int head_dim, int tile_rows, std::vector<PrefixItem> (&items)[2],
                      std::vector<PrefixJoin>& joins, int* most) {
   std::vector<PlanGroup> groups;
   std::vector<int> row_start(1, 0);
@@ -312,7 +314,7 @@ long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int3
       active += rho > 0;
       pg.rho += rho;
       alone += (rho + 127) / 128;
-      own_ctas += tiles_of(rho) * n_kv_heads;
+      own_ctas += tiles_of(rho, tile_rows) * n_kv_heads;
     }
     // sharing pays when stacking the rows leaves fewer 128-row steps over the prefix
     pg.shared = active >= 2 && prefixes[g] > 0 && (pg.rho + 127) / 128 * 10 <= alone * 7;
@@ -320,18 +322,18 @@ long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int3
   }
   // pieces of the own ranges, when one item a sequence leaves most of the machine idle
   const int pieces = own_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, own_ctas)));
-  const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim)),
-                      part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim))};
+  const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim), tile_rows),
+                      part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim), tile_rows)};
   *most = 0;
   // A group's states lie together: [parts][n_kv_heads][the group's score rows], from `states` on.
   long long states = 0;
   for (const PlanGroup& g : groups) {
     auto add = [&](int row0, long long rho, int pos0, int pos1, int part) {
       const long long at = part < 0 ? -1 : states + part * n_kv_heads * g.rho + (row0 - row_start[g.seq0]) * static_cast<long long>(group);
-      for (long long r = tiles_of(rho) - 1; r >= 0; --r)  // later rows see further: longest first
-        items[kind_of(rho)].push_back({row0, static_cast<int>(r * kTileRows),
-                                       static_cast<int>(std::min<long long>(kTileRows, rho - r * kTileRows)), pos0, pos1,
-                                       static_cast<int>(g.rho), at < 0 ? -1 : at + r * kTileRows});
+      for (long long r = tiles_of(rho, tile_rows) - 1; r >= 0; --r)  // later rows see further: longest first
+        items[kind_of(rho)].push_back({row0, static_cast<int>(r * tile_rows),
+                                       static_cast<int>(std::min<long long>(tile_rows, rho - r * tile_rows)), pos0, pos1,
+                                       static_cast<int>(g.rho), at < 0 ? -1 : at + r * tile_rows});
     };
     int shared_parts = 0, group_parts = 0;
     if (g.shared)
@@ -366,6 +368,30 @@ long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int3
   return states;
 }
 
+// Time, in clocks, of a batch's tile items in one variant of the kernel: items in list order, each on
+// the CTA slot that is free first.  A CTA's clocks a 64-position step and its start and end are
+// measured (24 prompts of 51..203 rows after 2048 positions; two CTAs of the single variant share an
+// SM's tensor core, so each takes longer): 113 us wide, 100 us single; five groups of 79 rows and
+// eight heads on 14960 positions: 67 us wide, 76 us single.
+double tile_clocks(const std::vector<PrefixItem>& items, int n_kv_heads, int max_ctx, int variant) {
+  const int slots = variant == kSingle ? 296 : 148;
+  std::vector<double> free_at(slots, 0.0);  // a heap, earliest first
+  double sum = 0, longest = 0;
+  const size_t ctas = items.size() * n_kv_heads;
+  for (const PrefixItem& it : items) {
+    const double steps = (std::min(it.pos1, max_ctx) - it.pos0 + 63) / 64;
+    const double clocks = variant == kSingle ? 9000 + 2280 * steps : it.n_rho > 128 ? 13000 + 1950 * steps : 9000 + 1270 * steps;
+    sum += clocks * n_kv_heads;
+    longest = std::max(longest, clocks);
+    for (int k = 0; ctas <= 4096 && k < n_kv_heads; ++k) {
+      std::pop_heap(free_at.begin(), free_at.end(), std::greater<double>());
+      free_at.back() += clocks;
+      std::push_heap(free_at.begin(), free_at.end(), std::greater<double>());
+    }
+  }
+  return ctas <= 4096 ? *std::max_element(free_at.begin(), free_at.end()) : sum / slots + longest / 2;
+}
+
 template <typename T, int HD>
 cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStream_t s, bool prepare) {
   if (prepare) {
@@ -375,8 +401,9 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
       return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                                          cudaSharedmemCarveoutMaxShared);
     };
-    cudaError_t e = set(prefix_tile_kernel<T, HD, false>, PrefixTileCfg<T, HD, false>::SMEM);
-    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, true>, PrefixTileCfg<T, HD, true>::SMEM);
+    cudaError_t e = set(prefix_tile_kernel<T, HD, 2, false>, PrefixTileCfg<T, HD, 2, false>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 2, true>, PrefixTileCfg<T, HD, 2, true>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 1, false>, PrefixTileCfg<T, HD, 1, false>::SMEM);
     if (e == cudaSuccess) e = set(prefix_cols_kernel<T, HD>, kColsSmem<T, HD>);
     return e;
   }
@@ -385,8 +412,13 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
   if (plan->n_items[kTile] > 0) {
     const int grid = plan->n_items[kTile] * plan->n_kv_heads;
     p.items = plan->items[kTile];
-    if (plan->pairs) prefix_tile_kernel<T, HD, true><<<grid, kTileThreads, PrefixTileCfg<T, HD, true>::SMEM, s>>>(p);
-    else prefix_tile_kernel<T, HD, false><<<grid, kTileThreads, PrefixTileCfg<T, HD, false>::SMEM, s>>>(p);
+    auto launch = [&](auto kernel, int threads, int smem) { kernel<<<grid, threads, smem, s>>>(p); };
+    using Wide = PrefixTileCfg<T, HD, 2, true>;
+    using Narrow = PrefixTileCfg<T, HD, 2, false>;
+    using Single = PrefixTileCfg<T, HD, 1, false>;
+    if (plan->variant == kWide) launch(prefix_tile_kernel<T, HD, 2, true>, Wide::THREADS, Wide::SMEM);
+    else if (plan->variant == kNarrow) launch(prefix_tile_kernel<T, HD, 2, false>, Narrow::THREADS, Narrow::SMEM);
+    else launch(prefix_tile_kernel<T, HD, 1, false>, Single::THREADS, Single::SMEM);
     e = cudaGetLastError();
     first = false;
   }
@@ -521,7 +553,28 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
       for (int r = 0; r < rows[s]; ++r) info.push_back(make_int4(s, rows[s] - r, slots[s], start[s] + r));
     }
     int parts = 0;
-    const long long n_states = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim, items, joins, &parts);
+    // Rows in pairs of 128-row tiles read each K/V tile once for both; single tiles spread better and
+    // start and end beside one another.  Without pairs, one stream a CTA once the CTAs are more than
+    // one and a half to an SM.
+    long long n_states = 0;
+    int variant = kNarrow;
+    for (int v : {kWide, kSingle}) {
+      std::vector<PrefixItem> it[2];
+      std::vector<PrefixJoin> jo;
+      int most = 0;
+      const long long st = plan_items(listed.data(), group_sizes, prefixes, n_groups, max_ctx, group, n_kv_heads, head_dim,
+                                      v == kWide ? 256 : 128, it, jo, &most);
+      const bool pairs = std::any_of(it[kTile].begin(), it[kTile].end(), [](const PrefixItem& i) { return i.n_rho > 128; });
+      if (v == kSingle && variant == kWide &&
+          tile_clocks(items[kTile], n_kv_heads, max_ctx, kWide) <= tile_clocks(it[kTile], n_kv_heads, max_ctx, kSingle))
+        break;
+      if (v == kSingle && variant != kWide) break;
+      for (int k = 0; k < 2; ++k) items[k] = std::move(it[k]);
+      joins = std::move(jo);
+      parts = most;
+      n_states = st;
+      variant = v == kSingle ? kSingle : pairs ? kWide : items[kTile].size() * n_kv_heads > 222 ? kSingle : kNarrow;
+    }
     for (PrefixJoin& j : joins) j.outer = info[j.row].w;
     DeviceScope dev;
     RC(dev.enter(device));
@@ -548,7 +601,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
       p->n_items[k] = static_cast<int>(items[k].size());
       at_items[k] = place(items[k].data(), items[k].size() * sizeof(PrefixItem));
     }
-    for (const PrefixItem& it : items[kTile]) p->pairs = p->pairs || it.n_rho > 128;
+    p->variant = variant;
     p->n_joins = static_cast<int>(joins.size());
     p->parts = parts;
     const size_t at_joins = place(joins.data(), joins.size() * sizeof(PrefixJoin));
