@@ -408,10 +408,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
 // runs S = Q . K^T, softmax, P back over the S columns as hi + lo terms, O += P . V with P from
 // TMEM; the reference max of a row moves only when a tile exceeds it by 2^8 (the pipeline of
 // attn_prefill_tc_kernel, whose header explains it).
-//   more than 128 rows  the streams are two row tiles that share every K/V tile.  One SM streams
-//                       about 25 bytes a clock into shared memory, 1300 clocks for the 32 KB of a
-//                       64-position tile of head_dim 128; 128 rows would give the tensor core 770
-//                       clocks of work for it, 256 rows give 1540.
+//   more than 128 rows  the streams are two row tiles that share every K/V tile.  At the memory's rate
+//                       an SM gets 24 bytes a clock, 1300 clocks for the 32 KB of a 64-position tile
+//                       of head_dim 128; a row tile takes the tensor core 900 clocks for it (S 384,
+//                       bound by re-reading Q from shared memory, P hi and lo 512): 1950 measured
+//                       for two.
 //   up to 128 rows      the streams take the even and the odd K/V tiles of the same rows, and are
 //                       joined at the end.
 // Warps 0 and 11 = bulk-copy producers, warps 1 and 2 = the streams' MMA issuers (warp 1 allocates TMEM), warps

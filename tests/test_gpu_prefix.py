@@ -172,6 +172,22 @@ def test_several_rows_each(dtype, heads, kv, hd, rows):
     b.check(*b.run())
 
 
+@pytest.mark.parametrize("dtype,heads,kv,hd", [("bf16", 8, 4, 128), ("fp16", 8, 4, 64)])
+def test_long_ranges_of_many_rows(dtype, heads, kv, hd):
+    # enough work an item that two row tiles share a CTA: more than 128 score rows a kv head, 28 steps
+    rng = np.random.default_rng(hd)
+    rows = [int(r) for r in rng.integers(65, 129, 38)]
+    b = Batch(dtype, kv, hd, [1] * 38, [0] * 38, [int(c) for c in rng.integers(1700, 1800, 38)], rows, heads, layers=1, seed=hd)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("prefix", [1040, 6160])
+def test_many_rows_on_one_long_prefix(prefix):
+    rng = np.random.default_rng(prefix)
+    b = Batch("bf16", 8, 64, [20], [prefix], lengths(rng, [prefix], [20], 90, 40), [40] * 20, 16, layers=1, seed=prefix)
+    b.check(*b.run())
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_rows_that_see_nothing_or_little(rows):
     # idle places, a context shorter than the rows, one inside the prefix, one of a single position
