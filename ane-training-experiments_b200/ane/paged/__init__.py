@@ -33,7 +33,7 @@ def meta_words(n_pages: int, max_seqs: int, max_pages: int) -> int:
 
 
 def _need(t, what: str, dtype, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or not t.is_contiguous():
         raise LLMError(_abi.LLM_ERR_INVALID, f"{what} must be a contiguous {dtype} tensor on {device}")
     return t.data_ptr()
 
@@ -141,6 +141,7 @@ class PrefixPlan:
         if len(slots) != len(rows) or len(sizes) != len(prefixes):
             raise LLMError(_abi.LLM_ERR_INVALID, "slots and rows, group_sizes and prefixes must have one length")
         self.n_seqs, self.n_rows = len(slots), int(rows.sum())
+        self._shape = torch.Size((self.n_rows, n_heads, cache.head_dim))
         h = C.c_void_p()
         self.h = None
         _abi.check(self._lib.llm_prefix_plan_create(
@@ -151,8 +152,8 @@ class PrefixPlan:
 
     def _rows(self, t, what: str):
         c = self.cache
-        if not isinstance(t, torch.Tensor) or t.dtype != c.torch_dtype or t.device != c.device or \
-                t.shape != (self.n_rows, self.n_heads, c.head_dim) or t.stride(2) != 1:
+        if not isinstance(t, torch.Tensor) or t.dtype is not c.torch_dtype or t.device != c.device or \
+                t.shape != self._shape or t.stride(2) != 1:
             raise LLMError(_abi.LLM_ERR_INVALID, f"{what} must be a {c.torch_dtype} tensor [{self.n_rows}, {self.n_heads}, "
                                                  f"{c.head_dim}] on {c.device} with contiguous rows of a head")
         return t.data_ptr(), t.stride(0), t.stride(1)
@@ -165,8 +166,7 @@ class PrefixPlan:
         qp, qr, qh = self._rows(q, "q")
         if out is None:
             out = torch.empty_like(q)
-        op, orow, oh = (out.data_ptr(), qr, qh) if out.stride() == q.stride() and out.shape == q.shape and \
-            out.dtype == q.dtype and out.device == q.device else self._rows(out, "out")
+        op, orow, oh = self._rows(out, "out")
         if lse is not None:
             lp = _need(lse, "lse", torch.float32, c.device)
             if lse.shape != (self.n_rows, self.n_heads):

@@ -216,7 +216,9 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
   RC(dev.enter(device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PageTables t = tables(c);
-  const int few = static_cast<int>((copy_grid(t, t.n_pages / 2 + 1) + 148 * 4 - 1) / (148 * 4));
+  const unsigned all = copy_grid(t, t.n_pages / 2 + 1);
+  if (!all) return fail_fmt(LLM_ERR_INVALID, "%d pages in one request", t.n_pages);
+  const int few = static_cast<int>((all + 148 * 4 - 1) / (148 * 4));
   // one launch of at most four CTAs an SM (96 pages: as long on the device as two, 3 us less on the host)
   if (t.n_pages <= kSmallPool && few <= 8) {
     pages_compact_small_kernel<<<copy_grid(t, t.n_pages / 2 + 1, few), kCopyThreads, 0, s>>>(t, few);
@@ -225,9 +227,8 @@ extern "C" int llm_pages_compact(int device, const llm_page_cache* c, void* stre
   }
   // the host knows only a bound of the moves (half of the pool): longer CTAs where the bound makes
   // many, as most of them may find nothing to do
-  const int turns = copy_grid(t, t.n_pages / 2 + 1) > 148 * 16 ? 4 : 1;
+  const int turns = all > 148 * 16 ? 4 : 1;
   const unsigned grid = copy_grid(t, t.n_pages / 2 + 1, turns);
-  if (!grid) return fail_fmt(LLM_ERR_INVALID, "%d pages in one request", t.n_pages);
   pages_compact_plan_kernel<<<(t.n_pages + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, s>>>(t);
   CU(cudaGetLastError());
   CU(launch_dependent(pages_compact_kernel, dim3(grid), dim3(kCopyThreads), 0, s, t, turns));

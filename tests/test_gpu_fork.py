@@ -61,6 +61,28 @@ def test_forks_equal_separate_prefills(cfg, dtype, length):
     a.close()
 
 
+@pytest.mark.parametrize("cfg,dtype", [(MHA, "w8a8_fp16"), (CFG, "w8a8_bf16"), (MHA, "fp16")])
+def test_groups_and_lone_sequences_in_one_step(cfg, dtype):
+    # a group of four, a group of two and two sequences that share with nobody
+    rng = np.random.default_rng(8)
+    prompts = {s: rng.integers(3, cfg.vocab, n).tolist() for s, n in ((0, 100), (1, 64), (2, 45), (3, 5))}
+    seqs = [6, 2, 0, 8, 1, 7, 3, 5]
+    owner = {6: 0, 7: 0, 8: 0, 5: 1}
+    runs = []
+    for mode in (0, 2):
+        eng = engine(cfg, dtype)
+        eng.set_option(_abi.LLM_OPT_SHARED_PREFIX, mode)
+        eng.prefill(list(prompts), list(prompts.values()))
+        eng.fork(0, [6, 7, 8], 100)
+        eng.fork(1, [5], 64)
+        pos = np.array([len(prompts[owner.get(s, s)]) for s in seqs], np.int32)
+        tok = np.random.default_rng(9).integers(3, cfg.vocab, (20, len(seqs)))
+        runs.append([eng.decode_step(seqs, tok[i], pos + i, want_logits=True)[1] for i in range(20)])
+        eng.close()
+    for x, y in zip(*runs):
+        assert float(np.abs(x - y).max()) <= REF_ORDER_TOL[dtype]
+
+
 def test_generate_over_shared_prefixes_follows_the_step_loop():
     rng = np.random.default_rng(3)
     prompts = [rng.integers(3, CFG.vocab, n).tolist() for n in (70, 33)]
