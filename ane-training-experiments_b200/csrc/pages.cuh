@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(ForkParam
   int* const first = work + PageWork::first(p.t.max_seqs);
   int* const src = work + PageWork::src(p.t.max_seqs, p.t.n_pages);
   int* const dst = work + PageWork::dst(p.t.max_seqs, p.t.n_pages);
-  const int have = *p.t.n_free;
+  const int have = min(*p.t.n_free, p.t.n_pages);
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
   int base = 0, moves = 0;
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kCopyThreads, 5) pages_fork_small_kernel(ForkP
   __shared__ int s_scan[33], s_first[kCopyThreads], s_child[kCopyThreads], s_src[kCopyThreads], s_dst[kCopyThreads];
   __shared__ int s_last, s_bad;
   const int i = threadIdx.x;
-  const int have = *p.t.n_free;
+  const int have = min(*p.t.n_free, p.t.n_pages);
   ForkShape f{0, 0, false, false};
   bool bad = i < p.n && !fork_shape(p, i, f);
   s_child[i] = i < p.n ? p.children[i] : -1 - i;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kFreeThreads) pages_free_kernel(PageTables t, 
   int mine = 0;
   for (int w = w0; w < w1; ++w) mine += __popc(__ldcg(bits + w));
   int total;
-  const int base = *t.n_free;
+  const int base = min(max(*t.n_free, 0), t.n_pages);
   int at = base + block_exclusive(mine, s_scan, total);
   for (int w = w0; w < w1; ++w) {
     unsigned b = __ldcg(bits + w);
