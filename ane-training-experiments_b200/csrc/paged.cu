@@ -623,7 +623,10 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
       llm_prefix_plan_destroy(p);
       return fail_fmt(LLM_ERR_OOM, "cudaMalloc(%zu) failed: %s", bytes, cudaGetErrorString(e));
     }
+    // A copy from pageable memory may return with its last bytes still on the way, and the first call
+    // may come on a stream that is not ordered with the null stream: wait for them here.
     e = cudaMemcpy(p->block, host.data(), host.size(), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (e == cudaSuccess) e = prefix_any(p, PrefixParams{}, nullptr, true);
     if (e != cudaSuccess) {
       llm_prefix_plan_destroy(p);
