@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstring>
 #include <functional>
+#include <initializer_list>
 #include <new>
 #include <vector>
 
@@ -95,11 +96,16 @@ int check_geometry(const llm_page_cache* c) {
   return LLM_OK;
 }
 
+// Device arrays of n int32 arguments: there, and aligned for the kernels' loads.
+int check_lists(std::initializer_list<const int32_t*> lists, const char* what) {
+  for (const int32_t* p : lists)
+    if (!p || !aligned(p, 4)) return fail_fmt(LLM_ERR_INVALID, "nil or misaligned %s", what);
+  return LLM_OK;
+}
+
 int check_tables(const llm_page_cache* c) {
   RC(check_geometry(c));
-  for (const int32_t* p : {c->n_free, c->status, c->npages, c->refs, c->free_pages, c->table, c->work})
-    if (!p || !aligned(p, 4)) return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
-  return LLM_OK;
+  return check_lists({c->n_free, c->status, c->npages, c->refs, c->free_pages, c->table, c->work}, "cache table");
 }
 
 PageTables tables(const llm_page_cache* c) {
@@ -158,12 +164,13 @@ extern "C" int llm_pages_copy(int device, const llm_page_cache* from, const llm_
                               const int32_t* dst, int n, void* stream) {
   RC(check_geometry(from));
   RC(check_geometry(to));
-  if (!from->status) return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
+  RC(check_lists({from->status}, "cache table"));
   if (from->dtype != to->dtype || from->n_layers != to->n_layers || from->n_kv_heads != to->n_kv_heads ||
       from->head_dim != to->head_dim)
     return fail_fmt(LLM_ERR_INVALID, "the caches have different layers, heads, head_dim or dtype");
-  if (n < 0 || (n > 0 && (!src || !dst))) return fail_fmt(LLM_ERR_INVALID, "nil page list or negative count");
+  if (n < 0) return fail_fmt(LLM_ERR_INVALID, "negative count");
   if (n == 0) return LLM_OK;
+  RC(check_lists({src, dst}, "page list"));
   DeviceScope dev;
   RC(dev.enter(device));
   const PageTables a = tables(from), b = tables(to);
@@ -179,7 +186,7 @@ extern "C" int llm_pages_fork(int device, const llm_page_cache* c, const int32_t
   RC(check_tables(c));
   if (n < 0 || n > c->max_seqs) return fail_fmt(LLM_ERR_INVALID, "%d requests for %d slots", n, c->max_seqs);
   if (n == 0) return LLM_OK;
-  if (!parents || !children || !lens || !rooms) return fail_fmt(LLM_ERR_INVALID, "nil request array");
+  RC(check_lists({parents, children, lens, rooms}, "request array"));
   DeviceScope dev;
   RC(dev.enter(device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -201,8 +208,9 @@ extern "C" int llm_pages_fork(int device, const llm_page_cache* c, const int32_t
 
 extern "C" int llm_pages_free(int device, const llm_page_cache* c, const int32_t* slots, int n, void* stream) {
   RC(check_tables(c));
-  if (n < 0 || (n > 0 && !slots)) return fail_fmt(LLM_ERR_INVALID, "nil slot list or negative count");
+  if (n < 0) return fail_fmt(LLM_ERR_INVALID, "negative count");
   if (n == 0) return LLM_OK;
+  RC(check_lists({slots}, "slot list"));
   DeviceScope dev;
   RC(dev.enter(device));
   pages_free_kernel<<<std::min(n, 148 * 4), kFreeThreads, 0, static_cast<cudaStream_t>(stream)>>>(tables(c), slots, n);
@@ -652,8 +660,7 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
                                  int64_t o_head, float* lse, void* stream) {
   if (!plan) return fail_fmt(LLM_ERR_INVALID, "nil plan");
   RC(check_geometry(c));
-  if (!c->table || !c->status || !aligned(c->table, 4) || !aligned(c->status, 4))
-    return fail_fmt(LLM_ERR_INVALID, "nil or misaligned cache table");
+  RC(check_lists({c->table, c->status}, "cache table"));
   if (c->dtype != plan->dtype || c->n_kv_heads != plan->n_kv_heads || c->head_dim != plan->head_dim)
     return fail_fmt(LLM_ERR_INVALID, "the cache's dtype, heads or head_dim are not the plan's");
   if (plan->top_slot >= c->max_seqs) return fail_fmt(LLM_ERR_INVALID, "sequence %d out of range", plan->top_slot);

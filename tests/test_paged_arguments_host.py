@@ -1,0 +1,31 @@
+"""Argument checks of the paged caches that need no GPU: what would fault on the device, or race there,
+is refused on the host before any launch.  Addresses are host numbers that no entry may touch."""
+import ctypes as C
+
+import pytest
+
+from ane import _abi
+from test_pages_host import cache
+
+INVALID = _abi.LLM_ERR_INVALID
+X = 1 << 20
+
+
+@pytest.mark.parametrize("odd", [X + 1, X + 2, X + 3])
+def test_misaligned_lists_are_refused(odd):
+    L, good = _abi.lib(), cache()
+    p = C.addressof(good)
+    calls = [lambda a, b, c, d: L.llm_pages_copy(0, p, p, a, b, 1, None), lambda a, b, c, d: L.llm_pages_fork(0, p, a, b, c, d, 1, None),
+             lambda a, b, c, d: L.llm_pages_free(0, p, a, 1, None)]
+    for call, n in zip(calls, (2, 4, 1)):
+        for i in range(n):
+            args = [X] * 4
+            args[i] = odd
+            assert call(*args) == INVALID and "misaligned" in _abi.last_error()
+
+
+def test_a_copy_with_a_misaligned_status_word_is_refused():
+    L, good = _abi.lib(), cache()
+    for odd in (None, X + 1, X + 2):
+        bad = cache(status=odd)
+        assert L.llm_pages_copy(0, C.addressof(bad), C.addressof(good), X, X, 1, None) == INVALID and "table" in _abi.last_error()
