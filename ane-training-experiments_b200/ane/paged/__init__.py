@@ -93,9 +93,12 @@ class PagedCache:
         return p
 
     def copy(self, src, dst, to: "PagedCache | None" = None) -> None:
-        """Page src[i] of this cache to page dst[i] of `to` (default: this cache) in every layer."""
-        n = src.numel()
+        """Page src[i] of this cache to page dst[i] of `to` (default: this cache; on the same GPU) in
+        every layer."""
         to = self if to is None else to
+        if not isinstance(to, PagedCache) or to.device != self.device:
+            raise LLMError(_abi.LLM_ERR_INVALID, f"`to` must be a PagedCache on {self.device}, not {getattr(to, 'device', to)}")
+        n = src.numel()
         _abi.check(self._lib.llm_pages_copy(self.device.index, self._ref, to._ref, self._ints(src, "src"),
                                             self._ints(dst, "dst", n), n, self._stream()))
 

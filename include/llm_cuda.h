@@ -401,8 +401,8 @@ size_t llm_pages_work_words(int n_pages, int max_seqs);
  * returns the matching LLM_ERR_* code (LLM_OK when nothing failed) and clears it. */
 int llm_pages_status(int device, const llm_page_cache *cache, void *stream);
 /* Copy page src[i] of `from` to page dst[i] of `to` in every layer, i < n.  The caches have the
- * same layers, heads, head_dim and dtype and may be one cache; no dst[i] appears twice or among
- * the sources of the same pool.  Tables are not changed. */
+ * same layers, heads, head_dim and dtype, are both in the memory of `device`, and may be one cache; no
+ * dst[i] appears twice or among the sources of the same pool.  Tables are not changed. */
 int llm_pages_copy(int device, const llm_page_cache *from, const llm_page_cache *to, const int32_t *src,
                    const int32_t *dst, int n, void *stream);
 /* Request i makes slot children[i] a copy of the first lens[i] positions of slot parents[i], with

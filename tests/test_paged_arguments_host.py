@@ -29,3 +29,21 @@ def test_a_copy_with_a_misaligned_status_word_is_refused():
     for odd in (None, X + 1, X + 2):
         bad = cache(status=odd)
         assert L.llm_pages_copy(0, C.addressof(bad), C.addressof(good), X, X, 1, None) == INVALID and "table" in _abi.last_error()
+
+
+def test_a_copy_into_a_cache_on_another_gpu_is_refused():
+    # two caches as their constructor leaves them, on GPUs that need not exist
+    import torch
+    from ane.paged import PagedCache
+    a, b = (object.__new__(PagedCache) for _ in range(2))
+    for c, gpu in ((a, 0), (b, 1)):
+        c._lib, c.device, c.c_struct = _abi.lib(), torch.device("cuda", gpu), cache()
+        c._ref = C.addressof(c.c_struct)
+        c._stream = lambda: 0
+    lists = torch.zeros(0, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    with pytest.raises(_abi.LLMError) as e:
+        a.copy(*lists, to=b)
+    assert e.value.code == INVALID and "cuda:1" in str(e.value)
+    with pytest.raises(_abi.LLMError) as e:
+        a.copy(*lists, to="elsewhere")
+    assert e.value.code == INVALID
