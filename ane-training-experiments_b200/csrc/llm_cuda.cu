@@ -647,6 +647,7 @@ struct llm_ctx {
   // generate state
   int gen_n = 0, gen_steps_done = 0, gen_max_steps = 0, gen_splits = 1;
   std::vector<int> gen_seq, gen_pos0;
+  int gen_share = 0;  // share_gen when the batch was begun
 
   std::map<GraphKey, cudaGraphExec_t> graphs;
   bool use_graphs = true;
@@ -1343,19 +1344,26 @@ int ensure_pages(llm_ctx* c, int seq, int upto, std::vector<int>* dirty) {
 
 int upload_dirty(llm_ctx* c, std::vector<int>& dirty);
 
+// LLM_ERR_STATE where a position from[i]..upto[i] of sequence seq[i], i < n, lies in a page that another
+// sequence holds too: such pages are read-only.
+int check_unshared(llm_ctx* c, int n, const int32_t* seq, const int* from, const int* upto) {
+  if (c->shared_entries == 0) return LLM_OK;
+  for (int i = 0; i < n; ++i) {
+    const int* row = c->h_block_table.data() + static_cast<size_t>(seq[i]) * c->max_pages_per_seq;
+    for (int pg = from[i] / 16; pg <= upto[i] / 16 && pg < c->seq_npages[seq[i]]; ++pg)
+      if (c->page_refs[row[pg]] > 1)
+        return fail(LLM_ERR_STATE, "position %d of sequence %d is shared with another sequence", std::max(from[i], pg * 16), seq[i]);
+  }
+  return LLM_OK;
+}
+
 // Pages through position upto[i] for sequence seq[i], i < n (rows already validated), whose
-// positions from[i]..upto[i] the call writes: none of them may lie in a page that another sequence
-// holds too (checked for all rows before any page is reserved).  If the
+// positions from[i]..upto[i] the call writes (none may be shared: checked for all rows before any
+// page is reserved).  If the
 // pool runs out part way, the rows changed so far are still uploaded, so the device block
 // table matches the host's before the error returns (those sequences keep their new pages).
 int reserve_rows(llm_ctx* c, int n, const int32_t* seq, const int* from, const int* upto) {
-  if (c->shared_entries > 0)
-    for (int i = 0; i < n; ++i) {
-      const int* row = c->h_block_table.data() + static_cast<size_t>(seq[i]) * c->max_pages_per_seq;
-      for (int pg = from[i] / 16; pg <= upto[i] / 16 && pg < c->seq_npages[seq[i]]; ++pg)
-        if (c->page_refs[row[pg]] > 1)
-          return fail(LLM_ERR_STATE, "position %d of sequence %d is shared with another sequence", std::max(from[i], pg * 16), seq[i]);
-    }
+  RC(check_unshared(c, n, seq, from, upto));
   std::vector<int> dirty;
   for (int i = 0; i < n; ++i) {
     const int rc = ensure_pages(c, seq[i], upto[i], &dirty);
@@ -2480,8 +2488,23 @@ extern "C" int llm_generate_begin(llm_ctx* c, const int32_t* seq_ids, const int3
   c->step_kv_positions = kv_positions;
   c->gen_seq.assign(seq_ids, seq_ids + n);
   c->gen_pos0.assign(positions, positions + n);
+  c->gen_share = c->share_gen;
   return LLM_OK;
 }
+
+namespace {
+// The next `steps` steps of the generate batch write positions that llm_generate_begin reserved; a fork
+// since then may have shared their pages.
+int check_gen_steps(llm_ctx* c, int steps) {
+  if (steps == 0 || c->share_gen == c->gen_share) return LLM_OK;
+  std::vector<int> from(c->gen_n), upto(c->gen_n);
+  for (int i = 0; i < c->gen_n; ++i) {
+    from[i] = c->gen_pos0[i] + c->gen_steps_done;
+    upto[i] = from[i] + steps - 1;
+  }
+  return check_unshared(c, c->gen_n, c->gen_seq.data(), from.data(), upto.data());
+}
+}  // namespace
 
 extern "C" int llm_generate_steps(llm_ctx* c, int steps) {
   RC(check_ready(c));
@@ -2489,6 +2512,7 @@ extern "C" int llm_generate_steps(llm_ctx* c, int steps) {
   if (steps < 0 || c->gen_steps_done + steps > c->gen_max_steps)
     return fail(LLM_ERR_INVALID, "steps %d exceed the reserved %d", c->gen_steps_done + steps, c->gen_max_steps);
   RC(set_device(c));
+  RC(check_gen_steps(c, steps));
   for (int i = 0; i < steps; ++i) RC(run_step(c, c->gen_n, c->gen_splits, 2, c->gen_plan));
   c->gen_steps_done += steps;
   return LLM_OK;
@@ -2828,6 +2852,7 @@ extern "C" int llm_profile_step(llm_ctx* c, int iters, char* report, size_t repo
     return fail(LLM_ERR_STATE, "no reserved generate step left to profile (reserve one more in llm_generate_begin)");
   if (iters <= 0) return fail(LLM_ERR_INVALID, "iters must be positive");
   RC(set_device(c));
+  RC(check_gen_steps(c, 1));
   // Eager launches of the next step (its position is reserved; the K/V it writes there are
   // rewritten by the real step), with an event after each one; tokens/positions are not advanced.
   RowsSpec rs;
@@ -2935,6 +2960,7 @@ extern "C" int llm_trace_step(llm_ctx* c, char* report, size_t report_len, doubl
   if (c->gen_n <= 0) return fail(LLM_ERR_STATE, "llm_generate_begin not called");
   if (c->gen_steps_done >= c->gen_max_steps)
     return fail(LLM_ERR_STATE, "no reserved generate step left to trace (reserve one more in llm_generate_begin)");
+  RC(check_gen_steps(c, 1));
   RC(trace_begin(c));
   // The next step of the generate batch (its position is reserved), launched eagerly in the
   // current schedule; tokens and positions are not advanced.

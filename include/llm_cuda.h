@@ -132,8 +132,11 @@ int llm_kv_alloc(llm_ctx *ctx, int max_seqs, int max_pos, int page_tokens);
 int llm_seq_release(llm_ctx *ctx, int seq);
 /* Make each of the n empty slots children[i] a copy of the first `len` positions of slot `parent`
  * (several samples of one prompt, a common system prompt): complete pages are shared and counted, a
- * partly filled last page is copied.  Shared pages are read-only: a call that would write a position
- * inside one fails with LLM_ERR_STATE, so parent and children continue at `len` or later.  A page
+ * partly filled last page is copied.  `len` is at most the positions that the parent has pages for;
+ * which of them it has written is the caller's to know.  Shared pages are read-only: a call that
+ * would write a position inside one fails with LLM_ERR_STATE (llm_generate_steps too, for the steps
+ * asked for, when the fork came after llm_generate_begin), so parent and children continue at `len`
+ * or later.  A page
  * returns to the pool when the last slot that holds it is released.  Decode steps read shared pages
  * once per group of sequences (LLM_OPT_SHARED_PREFIX).  All children are made or none.  No
  * counterpart in the reference (one cache per decoder, ane/stories/infer.go:113-114). */
