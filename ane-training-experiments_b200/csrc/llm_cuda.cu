@@ -2493,16 +2493,18 @@ extern "C" int llm_generate_begin(llm_ctx* c, const int32_t* seq_ids, const int3
 }
 
 namespace {
-// The next `steps` steps of the generate batch write positions that llm_generate_begin reserved; a fork
-// since then may have shared their pages.
+// Before the next `steps` steps of the generate batch (0: before its attention is timed), where a fork
+// or a release since llm_generate_begin may have changed what it shares: the positions that the steps
+// write must not be shared, and the plan must be of the pages that the slots hold now.
 int check_gen_steps(llm_ctx* c, int steps) {
-  if (steps == 0 || c->share_gen == c->gen_share) return LLM_OK;
+  if (c->share_gen == c->gen_share) return LLM_OK;
   std::vector<int> from(c->gen_n), upto(c->gen_n);
   for (int i = 0; i < c->gen_n; ++i) {
     from[i] = c->gen_pos0[i] + c->gen_steps_done;
     upto[i] = from[i] + steps - 1;
   }
-  return check_unshared(c, c->gen_n, c->gen_seq.data(), from.data(), upto.data());
+  if (steps > 0) RC(check_unshared(c, c->gen_n, c->gen_seq.data(), from.data(), upto.data()));
+  return choose_prefix(c, c->gen_prefix, c->gen_n, c->gen_seq.data(), from.data(), &c->gen_plan);
 }
 }  // namespace
 
@@ -2785,6 +2787,7 @@ extern "C" int llm_time_attention(llm_ctx* c, int iters, double* us_per_launch, 
   if (c->gen_steps_done <= 0) return fail(LLM_ERR_STATE, "no generate step has run yet");
   if (iters <= 0) return fail(LLM_ERR_INVALID, "iters must be positive");
   RC(set_device(c));
+  RC(check_gen_steps(c, 0));
   // Time the attention of the last executed step: its positions (pos0 + done - 1) have their
   // K/V written and their pages reserved.  d_pos (the next position) is restored afterwards.
   CU(cudaStreamSynchronize(c->stream));

@@ -1,10 +1,13 @@
 """Forks and releases between the steps of a generate batch.  A shared page is read-only, so steps that
-would write into one are refused before anything is enqueued.  A batch of one slot runs per sequence
-whatever the option, so its tokens are compared bit for bit."""
+would write into one are refused before anything is enqueued, and a batch whose sharing changed
+attends to what its slots hold now.  A batch of one slot runs per sequence whatever the option, so
+its tokens are compared bit for bit; K and V behind attention over shared prefixes within
+parity.REF_ORDER_TOL, the bound of two orders of operations."""
 import numpy as np
 import pytest
 
 from ane import _abi
+from parity import REF_ORDER_TOL
 from test_gpu_fork import CFG, engine
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +80,25 @@ def test_sharing_behind_or_elsewhere_does_not_stop_a_batch():
     eng.generate_steps(17)
     np.testing.assert_array_equal(eng.generate_end(), want)
     eng.close()
+
+def test_a_slot_that_changed_between_steps_is_read_as_it_is_now():
+    """Slot 3 leaves a group over prompt A between two steps and comes back as a copy of prompt B."""
+    rng = np.random.default_rng(5)
+    a, b = (rng.integers(3, CFG.vocab, 72).tolist() for _ in range(2))
+    seqs, pos = [0, 1, 2, 3], [72] * 4
+    got = []
+    for mode in (0, 2):
+        eng = engine(CFG, "fp16", slots=6, max_pos=128)
+        eng.set_option(_abi.LLM_OPT_SHARED_PREFIX, mode)
+        eng.prefill([0, 5], [a, b])
+        eng.fork(0, [1, 2, 3], 72)
+        eng.generate_begin(seqs, [7, 8, 9, 10], pos, 8)
+        eng.generate_steps(0)
+        eng.release(3)
+        eng.fork(5, [3], 72)
+        eng.generate_steps(1)
+        eng.synchronize()
+        got.append([np.stack(eng.read_kv(CFG.n_layers - 1, s, 72)) for s in seqs])
+        eng.close()
+    for x, y in zip(*got):
+        assert float(np.abs(x - y).max()) <= REF_ORDER_TOL["fp16"]
