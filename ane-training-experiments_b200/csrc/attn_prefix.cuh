@@ -4,7 +4,9 @@
 //   o = sum_t 2^(c q.k_t - m) v_t / l,  l = sum_t 2^(c q.k_t - m),  c = scale * log2(e)
 // with any m; m, l and the sum form a state that joins with another set of positions' state as
 //   M = max(m, m'), l = 2^(m-M) l + 2^(m'-M) l', o = 2^(m-M) o + 2^(m'-M) o'.
-// A row that sees nothing (ctx 0, or a row before position 0) gives o = 0 and lse = -inf.
+// A row that sees nothing (ctx 0, a row before position 0, or every score -inf) has l = 0 and gives
+// o = 0 and lse = -inf.  A NaN score, or one of +inf (whose weight is inf - inf), makes l NaN: l is
+// tested against 0 only, so that such a row leaves as NaN from every kernel.
 //
 // The plan cuts the work into items, each a run of score rows (query row, head of the kv head's
 // group) against a run of positions of one block-table row, for every kv head: the shared
@@ -80,7 +82,7 @@ __device__ __forceinline__ int page_entry(const PrefixParams& p, const int* bt, 
   return e;
 }
 __device__ __forceinline__ float natural_lse(float m, float l) {
-  return l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // One warp joins the states of (row, head) and writes the output.  Lane k weighs states k and k + 32
@@ -135,7 +137,7 @@ __device__ __forceinline__ void join_states(const PrefixParams& p, const PrefixJ
       for (int e = 0; e < V; ++e) O[e] += v[i][e] * w[i];
   }
   const long long to = j.outer * p.o_row + head * p.o_head + lane * V;
-  const float inv = L > 0.f ? __fdiv_rn(1.0f, L) : 0.f;
+  const float inv = L == 0.f ? 0.f : __fdiv_rn(1.0f, L);
 #pragma unroll
   for (int e = 0; e < V; e += 2) {
     if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + e) = make_float2(O[e] * inv, O[e + 1] * inv);
@@ -270,8 +272,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
     const float mn0 = fmaxf(st.m0, pm0), mn1 = fmaxf(st.m1, pm1);
     const float2 mu = make_float2(mn0 == -INFINITY ? 0.f : mn0, mn1 == -INFINITY ? 0.f : mn1);
     const float2 al = exp2_det_lo2(sub2_rn(make_float2(st.m0, st.m1), mu));
-    const float2 p01 = exp2_det_lo2(sub2_rn(make_float2(s0, s1), mu));
-    const float2 p23 = exp2_det_lo2(sub2_rn(make_float2(s2, s3), mu));
+    const float2 p01 = exp2_det_lo2<true>(sub2_rn(make_float2(s0, s1), mu));
+    const float2 p23 = exp2_det_lo2<true>(sub2_rn(make_float2(s2, s3), mu));
     st.l0 = st.l0 * al.x + (p01.x + p23.x);
     st.l1 = st.l1 * al.y + (p01.y + p23.y);
     st.m0 = mn0;
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
     for (int i = threadIdx.x; i < it.n_rho * (HD / 2); i += kAttnWarps * 32) {
       const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
       const int row = p.row_info[it.row0 + (it.rho0 + c) / group].w, head = kvh * group + (it.rho0 + c) % group;
-      const float l = s_l[c], inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+      const float l = s_l[c], inv = l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
       const float x = stage[c * HD + d] * inv, y = stage[c * HD + d + 1] * inv;
       const long long at = row * p.o_row + head * p.o_head + d;
       if (p.out_f32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = make_float2(x, y);
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
     s_off[mine] = row * p.o_row + head * p.o_head;
     const size_t at = it.state + static_cast<size_t>(kvh) * it.span;  // of the item's score row 0
     if (!apart) streams_bar();
-    float m = m_ref, l = l_run, w = l_run > 0.f ? 1.f : 0.f;  // the row's state, and this stream's weight in it
+    float m = m_ref, l = l_run, w = l_run == 0.f ? 0.f : 1.f;  // the row's state, and this stream's weight in it
     if (!apart) {
       const float2 other = s_ml[(1 - sg) * 128 + tl];
       m = fmaxf(m_ref, other.x);
@@ -883,7 +885,7 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
       if (it.state >= 0) __stcg(p.ws_ml + at + local, make_float2(m, l));
       else if (p.lse) p.lse[static_cast<size_t>(row) * p.n_heads + head] = natural_lse(m, l);
     }
-    s_w[mine] = it.state < 0 && l > 0.f ? __fdiv_rn(w, l) : w;
+    s_w[mine] = it.state < 0 && l != 0.f ? __fdiv_rn(w, l) : w;
     if (apart) __syncwarp();
     else streams_bar();
     // rows of this warp: its own 32; or 16 of the tile, from both streams
@@ -898,11 +900,11 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
         const int k = r0 + i * PER + lane / CH, rr = row_w + (k < n_w ? k : 0);
         const float wa = s_w[rr];
         const float4 x = stage[rr * CH + (c ^ (rr & (CH - 1)))];  // not finite where the row saw nothing
-        o[i] = wa > 0.f ? make_float4(x.x * wa, x.y * wa, x.z * wa, x.w * wa) : make_float4(0.f, 0.f, 0.f, 0.f);
+        o[i] = wa != 0.f ? make_float4(x.x * wa, x.y * wa, x.z * wa, x.w * wa) : make_float4(0.f, 0.f, 0.f, 0.f);
         if (!apart) {
           const float wb = s_w[128 + rr];
           const float4 y = stage[(128 + rr) * CH + (c ^ (rr & (CH - 1)))];
-          if (wb > 0.f) o[i] = make_float4(o[i].x + y.x * wb, o[i].y + y.y * wb, o[i].z + y.z * wb, o[i].w + y.w * wb);
+          if (wb != 0.f) o[i] = make_float4(o[i].x + y.x * wb, o[i].y + y.y * wb, o[i].z + y.z * wb, o[i].w + y.w * wb);
         }
       }
       if (it.state >= 0) {

@@ -206,10 +206,18 @@ __device__ __forceinline__ float2 mul2_rn(float2 a, float2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
   return bits_f2(d);
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is (fmaxf drops it)
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 // exp2_det_lo of two values with packed f32 pairs: each lane's result is bit-identical to the
-// scalar function (the same round-to-nearest operations per element).
+// scalar function (the same round-to-nearest operations per element).  A NaN gives 0 or, with
+// KEEP_NAN, NaN.
+template <bool KEEP_NAN = false>
 __device__ __forceinline__ float2 exp2_det_lo2(float2 x) {
-  const float2 xc = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+  const float2 xc = KEEP_NAN ? make_float2(max_nan(x.x, -127.0f), max_nan(x.y, -127.0f))
+                             : make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
   const float2 mg = make_float2(kExp2Magic, kExp2Magic);
   const float2 t = add2_rn(xc, mg);
   const float2 f = sub2_rn(xc, sub2_rn(t, mg));

@@ -429,8 +429,11 @@ int llm_pages_compact(int device, const llm_page_cache *cache, void *stream);
  * positions: the shared pages are read once for all query rows of a group, each sequence's own
  * pages once, and the two softmax states are joined.  Row r of sequence s (its rows are
  * consecutive, sequences in order) stands at position ctx[s] - rows[s] + r and sees every position
- * up to its own; a row that sees nothing gives 0.  K and V of a sequence's rows are in the cache
- * before the call.  Replaces attend (ane/stories/infer.go:267-299) for such batches.
+ * up to its own; a row that sees nothing, or nothing but scores of -inf, gives 0.  A row with a NaN
+ * score or one of +inf is NaN.  Values at or past ctx are not read into any result; a V value
+ * before it that is not finite may also reach rows of its sequence or group that stand before it
+ * (weight 0 times infinity).  K and V of a sequence's rows are in the cache before the call.
+ * Replaces attend (ane/stories/infer.go:267-299) for such batches.
  *
  * A plan holds what stays while a batch runs (its layout, work lists and workspace), for every
  * layer and step.  Sequence s reads block-table row slots[s] and has rows[s] >= 0 query rows;
