@@ -609,7 +609,7 @@ struct llm_ctx {
   int shared_prefix = 1;      // LLM_OPT_SHARED_PREFIX
   PrefixUse step_prefix, gen_prefix;
   const llm_prefix_plan* gen_plan = nullptr;  // gen_prefix.plan where the generate batch uses it
-  bool last_prefix = false;   // the last step's attention ran over shared prefixes
+  int prefix_launches = 0;    // a layer's attention launches of the last batch chosen for (0: per sequence)
   std::vector<uint32_t> seq_stamp;  // duplicate-sequence check: seq_stamp[s] == stamp_gen once seen
   uint32_t stamp_gen = 0;
 
@@ -1453,6 +1453,7 @@ int attn_splits_for(const llm_ctx* c, int n_blocks, int max_ctx) {
 constexpr double kPrefixExtraUs = 15.0;
 int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const int32_t* pos, const llm_prefix_plan** plan) {
   *plan = nullptr;
+  c->prefix_launches = 0;
   if (c->shared_prefix == 0 || c->shared_entries == 0 || !c->use_umma) return LLM_OK;
   std::map<int, std::vector<int>> by_first;  // first page -> batch rows
   const size_t width = c->max_pages_per_seq;
@@ -1499,6 +1500,7 @@ int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const i
     use.key = std::move(key);
   }
   *plan = use.plan;
+  c->prefix_launches = llm_detail_prefix_launches(use.plan);
   return LLM_OK;
 }
 
@@ -2086,7 +2088,6 @@ int ensure_logits(llm_ctx* c, int rows) {
 int run_step(llm_ctx* c, int n, int splits, int mode, const llm_prefix_plan* prefix) {
   RowsSpec rs;
   rs.prefix = prefix;
-  c->last_prefix = prefix != nullptr;
   rs.R = n;
   rs.n_blocks = n;
   rs.attn_splits = splits;
@@ -2744,23 +2745,20 @@ extern "C" int llm_synchronize(llm_ctx* c) {
 
 extern "C" int llm_step_parts(llm_ctx* c, int n, int* parts) {
   if (!c || !parts) return fail(LLM_ERR_INVALID, "nil argument");
-  *parts = c->last_prefix ? 1 : overlap_parts(c, n, true);
+  *parts = c->prefix_launches ? 1 : overlap_parts(c, n, true);
   return LLM_OK;
 }
 
 extern "C" int llm_step_kernel_count(llm_ctx* c, int n, int* count) {
   if (!c || !count) return fail(LLM_ERR_INVALID, "nil argument");
   // embed+norm, per layer: qkv, attention, wo, norm, w13, w2 (+ the SwiGLU quant kernel for int8)
-  // + the next layer's norm, then final norm, lm_head, finish
   // + the next layer's norm, then final norm, lm_head, finish; the overlapped schedule runs the
   // per-row part once per micro-batch
   const int per_layer = 6 + (c->in8 ? 1 : 0);
-  const int parts = c->last_prefix ? 1 : overlap_parts(c, n, true);
+  const int parts = c->prefix_launches ? 1 : overlap_parts(c, n, true);
   *count = parts * (1 + c->cfg.n_layers * per_layer + (c->cfg.n_layers - 1)) + 3;
-  if (c->last_prefix) {  // shared prefixes: the plan's launches in attention's place, and the int8 quantiser
-    const PrefixUse& use = c->gen_plan && c->gen_n == n ? c->gen_prefix : c->step_prefix;
-    if (use.plan) *count += c->cfg.n_layers * (llm_detail_prefix_launches(use.plan) - 1 + (c->in8 ? 1 : 0));
-  }
+  if (c->prefix_launches)  // shared prefixes: the plan's launches in attention's place, and the int8 quantiser
+    *count += c->cfg.n_layers * (c->prefix_launches - 1 + (c->in8 ? 1 : 0));
   return LLM_OK;
 }
 

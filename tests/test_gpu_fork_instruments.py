@@ -1,0 +1,44 @@
+"""What a context says of a decode step over shared prefixes: the launches it counts."""
+import numpy as np
+import pytest
+
+from ane import _abi
+from test_gpu_fork import CFG, MHA, engine
+
+pytestmark = pytest.mark.gpu
+
+
+def batch(cfg, dtype, mode):
+    """Two groups (70 positions of 5 slots, 33 of 2) and a lone slot (20), begun."""
+    rng = np.random.default_rng(1)
+    eng = engine(cfg, dtype)
+    eng.set_option(_abi.LLM_OPT_SHARED_PREFIX, mode)
+    eng.prefill([0, 1, 8], [rng.integers(3, cfg.vocab, n).tolist() for n in (70, 33, 20)])
+    eng.fork(0, [2, 3, 4, 5], 70)
+    eng.fork(1, [6], 33)
+    seqs = [0, 6, 2, 3, 8, 4, 1, 5]
+    pos = [{6: 33, 1: 33, 8: 20}.get(s, 70) for s in seqs]
+    eng.generate_begin(seqs, rng.integers(3, cfg.vocab, len(seqs)), pos, 6)
+    return eng, seqs, pos
+
+
+@pytest.mark.parametrize("mode", [0, 2])
+def test_counts_follow_the_step_that_is_asked_about(mode):
+    eng, seqs, _ = batch(CFG, "bf16", mode)
+    shared = eng.kernel_count(len(seqs))       # of the batch that was begun, before its first step
+    eng.generate_steps(1)
+    assert eng.kernel_count(len(seqs)) == shared
+    eng.generate_end()
+    alone = engine(CFG, "bf16")
+    alone.prefill([0], [[5, 6, 7]])
+    alone.decode_step([0], [5], [3])
+    plain = alone.kernel_count(len(seqs))
+    alone.close()
+    # shared: tile, column and join launches where one was
+    assert shared == plain + (2 * CFG.n_layers if mode == 2 else 0)
+    for s in seqs:
+        eng.release(s)
+    eng.prefill([0], [[5, 6, 7]])              # nothing shared any more
+    eng.decode_step([0], [5], [3])
+    assert eng.kernel_count(len(seqs)) == plain and eng.step_parts(len(seqs)) == 1
+    eng.close()
