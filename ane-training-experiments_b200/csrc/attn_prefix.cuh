@@ -63,6 +63,7 @@ struct PrefixParams {
   int* status;
   int n_rows, n_heads, n_kv_heads, n_pages, max_pages, max_ctx;
   float scale_log2;
+  TraceRec* trace;            // llm_trace_step
 };
 
 // Positions sequence s has, at most what its table row and the plan cover.
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   __shared__ float s_m[8], s_l[8];
   __shared__ int s_last;
 
+  trace_start(p.trace);
   griddep_launch_dependents();
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
   const int kvh = blockIdx.x % p.n_kv_heads;
@@ -399,10 +401,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
         join_states<T, HD, 8>(p, j, kvh * group + u % group);
       }
     }
+    trace_end(p.trace);
     return;
   }
   // the launch ends after the one before it, so that whoever waits for it has waited for both; one
   // CTA sees to that, the others make room
+  trace_end(p.trace);
   if (blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
@@ -517,6 +521,7 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
   auto& s_last = sync.s_last;
   uint32_t& s_tmem = sync.s_tmem;
 
+  trace_start(p.trace);
   const uint32_t q_s = smem_u32(gbase);
   const uint32_t k_ring = q_s + Cfg::K_RING;
   const uint32_t v_ring = q_s + Cfg::V_RING;
@@ -933,6 +938,7 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
   }
+  trace_end(p.trace);
 }
 
 // ============================================================================ states of a row -> output
@@ -944,7 +950,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixPara
   const bool on = unit < p.n_joins * p.n_heads;
   const PrefixJoin j = p.joins[on ? unit / p.n_heads : 0];
   griddep_wait();
+  trace_start(p.trace);
   if (on) join_states<T, HD, BATCH>(p, j, unit % p.n_heads);
+  trace_end(p.trace);
 }
 
 }  // namespace llm

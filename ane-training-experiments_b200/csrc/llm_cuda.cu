@@ -1843,6 +1843,8 @@ int enqueue_forward(llm_ctx* c, const RowsSpec& rs) {
       pr.n_pages = c->n_pages;
       pr.max_pages = c->max_pages_per_seq;
       pr.status = c->d_err;
+      const char* names[3];
+      for (int i = 0, n = llm_detail_prefix_launches(rs.prefix, &names); i < n; ++i) pr.trace[i] = tr(names[i], l, P);
       t_prio = 0;
       CU(llm_detail_prefix_run(rs.prefix, pr, P.s));
       if (i8) {

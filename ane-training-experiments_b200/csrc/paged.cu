@@ -402,7 +402,7 @@ double tile_clocks(const std::vector<PrefixItem>& items, int n_kv_heads, int max
 }
 
 template <typename T, int HD>
-cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStream_t s, bool prepare) {
+cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, TraceRec* const* trace, cudaStream_t s, bool prepare) {
   if (prepare) {
     // the whole carve-out for shared memory, so that CTAs of both kernels fit an SM together
     auto set = [](auto kernel, int smem) {
@@ -421,6 +421,7 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
   if (plan->n_items[kTile] > 0) {
     const int grid = plan->n_items[kTile] * plan->n_kv_heads;
     p.items = plan->items[kTile];
+    if (trace) p.trace = *trace++;
     auto launch = [&](auto kernel, int threads, int smem) { kernel<<<grid, threads, smem, s>>>(p); };
     using Wide = PrefixTileCfg<T, HD, 2, true>;
     using Narrow = PrefixTileCfg<T, HD, 2, false>;
@@ -435,6 +436,7 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
     constexpr int smem = kColsSmem<T, HD>;
     const dim3 grid(plan->n_items[kCols] * plan->n_kv_heads), block(kAttnWarps * 32);
     p.items = plan->items[kCols];
+    if (trace) p.trace = *trace++;
     if (first) {
       prefix_cols_kernel<T, HD><<<grid, block, smem, s>>>(p);
       e = cudaGetLastError();
@@ -443,6 +445,7 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
     }
   }
   if (e == cudaSuccess && plan->n_joins > 0 && !plan->tickets) {
+    if (trace) p.trace = *trace;
     const long long units = static_cast<long long>(plan->n_joins) * plan->n_heads;
     const dim3 grid(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
     e = plan->parts > 8 ? launch_dependent(prefix_join_kernel<T, HD, 20>, grid, block, 0, s, p)
@@ -451,11 +454,12 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, cudaStrea
   return e;
 }
 
-cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, cudaStream_t s, bool prepare) {
+// `trace`: nullptr, or the timeline records of the launches in their order.
+cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, TraceRec* const* trace, cudaStream_t s, bool prepare) {
   const bool bf = plan->dtype == LLM_DTYPE_BF16;
   if (plan->head_dim == 64)
-    return bf ? prefix_launch<__nv_bfloat16, 64>(plan, p, s, prepare) : prefix_launch<__half, 64>(plan, p, s, prepare);
-  return bf ? prefix_launch<__nv_bfloat16, 128>(plan, p, s, prepare) : prefix_launch<__half, 128>(plan, p, s, prepare);
+    return bf ? prefix_launch<__nv_bfloat16, 64>(plan, p, trace, s, prepare) : prefix_launch<__half, 64>(plan, p, trace, s, prepare);
+  return bf ? prefix_launch<__nv_bfloat16, 128>(plan, p, trace, s, prepare) : prefix_launch<__half, 128>(plan, p, trace, s, prepare);
 }
 
 // What a plan fixes of its launches.
@@ -493,11 +497,19 @@ cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_
   p.n_pages = r.n_pages;
   p.max_pages = r.max_pages;
   p.scale_log2 = scale_log2(1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
-  return prefix_any(plan, p, s, false);
+  return prefix_any(plan, p, r.trace, s, false);
 }
 
-int llm_detail_prefix_launches(const llm_prefix_plan* plan) {
-  return (plan->n_items[kTile] > 0) + (plan->n_items[kCols] > 0) + (plan->n_joins > 0 && !plan->tickets);
+int llm_detail_prefix_launches(const llm_prefix_plan* plan, const char* (*names)[3]) {
+  int n = 0;
+  auto add = [&](const char* name) {
+    if (names) (*names)[n] = name;
+    ++n;
+  };
+  if (plan->n_items[kTile] > 0) add("attention(tiles)");
+  if (plan->n_items[kCols] > 0) add("attention(cols)");
+  if (plan->n_joins > 0 && !plan->tickets) add("attention(join)");
+  return n;
 }
 
 extern "C" int llm_prefix_plan_destroy(llm_prefix_plan* plan) {
@@ -635,7 +647,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     // may come on a stream that is not ordered with the null stream: wait for them here.
     e = cudaMemcpy(p->block, host.data(), host.size(), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
-    if (e == cudaSuccess) e = prefix_any(p, PrefixParams{}, nullptr, true);
+    if (e == cudaSuccess) e = prefix_any(p, PrefixParams{}, nullptr, nullptr, true);
     if (e != cudaSuccess) {
       llm_prefix_plan_destroy(p);
       return fail_fmt(LLM_ERR_CUDA, "plan set-up failed: %s", cudaGetErrorString(e));
@@ -691,6 +703,6 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   p.n_pages = c->n_pages;
   p.max_pages = c->max_pages;
   p.scale_log2 = scale_log2(scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
-  CU(prefix_any(plan, p, static_cast<cudaStream_t>(stream), false));
+  CU(prefix_any(plan, p, nullptr, static_cast<cudaStream_t>(stream), false));
   return LLM_OK;
 }

@@ -4,6 +4,10 @@
 
 #include "../../include/llm_cuda.h"
 
+namespace llm {
+struct TraceRec;
+}
+
 // llm_prefix_plan_create for sequences listed in `order` (group by group; nullptr: as they are):
 // rows, slots, ctx and the rows of q and out stay in the caller's order.
 int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads, int head_dim, const int* slots,
@@ -20,6 +24,8 @@ struct llm_prefix_rows {
   const int* table;
   int n_pages, max_pages;
   int* status;
+  llm::TraceRec* trace[3];  // timeline records of the launches, in their order; nullptr: none
 };
 cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_rows& r, cudaStream_t s);
-int llm_detail_prefix_launches(const llm_prefix_plan* plan);  // kernels of one llm_detail_prefix_run
+// Kernels of one llm_detail_prefix_run, in their order; names: nullptr, or where to put theirs.
+int llm_detail_prefix_launches(const llm_prefix_plan* plan, const char* (*names)[3] = nullptr);

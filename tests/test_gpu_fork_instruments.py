@@ -1,4 +1,5 @@
-"""What a context says of a decode step over shared prefixes: the launches it counts."""
+"""What a context says of a decode step over shared prefixes: the launches it counts and the
+timeline that it records."""
 import numpy as np
 import pytest
 
@@ -41,4 +42,22 @@ def test_counts_follow_the_step_that_is_asked_about(mode):
     eng.prefill([0], [[5, 6, 7]])              # nothing shared any more
     eng.decode_step([0], [5], [3])
     assert eng.kernel_count(len(seqs)) == plain and eng.step_parts(len(seqs)) == 1
+    eng.close()
+
+
+def launches(table):
+    return [line for line in table.splitlines()[1:] if line.strip()]
+
+
+@pytest.mark.parametrize("cfg,dtype", [(CFG, "bf16"), (MHA, "fp16"), (CFG, "w8a8_bf16")])
+@pytest.mark.parametrize("mode", [0, 2])
+def test_the_timeline_has_every_launch_that_is_counted(cfg, dtype, mode):
+    eng, seqs, _ = batch(cfg, dtype, mode)
+    counted = eng.kernel_count(len(seqs))
+    table, us = eng.trace_step()
+    assert us > 0
+    # the finish kernel keeps no record
+    assert len(launches(table)) == counted - 1, table
+    for layer in range(cfg.n_layers):
+        assert any("attention" in line and f" L{layer} " in line for line in launches(table)), table
     eng.close()
