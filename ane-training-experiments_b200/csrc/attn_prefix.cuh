@@ -63,7 +63,7 @@ struct PrefixParams {
   int* status;
   int n_rows, n_heads, n_kv_heads, n_pages, max_pages, max_ctx;
   float scale_log2;
-  TraceRec* trace;            // llm_trace_step
+  TraceRec* trace;            // llm_trace_step; read by the TRACE instantiations only
 };
 
 // Positions sequence s has, at most what its table row and the plan cover.
@@ -156,7 +156,7 @@ __device__ __forceinline__ void join_states(const PrefixParams& p, const PrefixJ
 template <typename T, int HD>
 constexpr int kColsSmem = kAttnWarps * AttnCfg<T, HD>::WARP_BYTES;
 
-template <typename T, int HD>
+template <typename T, int HD, bool TRACE>
 __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols_kernel(PrefixParams p) {
   using Cfg = AttnCfg<T, HD>;
   constexpr int STAGES = Cfg::STAGES;
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
   __shared__ float s_m[8], s_l[8];
   __shared__ int s_last;
 
-  trace_start(p.trace);
+  if constexpr (TRACE) trace_start(p.trace);
   griddep_launch_dependents();
   const PrefixItem it = p.items[blockIdx.x / p.n_kv_heads];
   const int kvh = blockIdx.x % p.n_kv_heads;
@@ -401,12 +401,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
         join_states<T, HD, 8>(p, j, kvh * group + u % group);
       }
     }
-    trace_end(p.trace);
+    if constexpr (TRACE) trace_end(p.trace);
     return;
   }
   // the launch ends after the one before it, so that whoever waits for it has waited for both; one
   // CTA sees to that, the others make room
-  trace_end(p.trace);
+  if constexpr (TRACE) trace_end(p.trace);
   if (blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
@@ -494,7 +494,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void streams_bar() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
 
-template <typename T, int HD, int STREAMS, bool WIDE>
+template <typename T, int HD, int STREAMS, bool WIDE, bool TRACE>
 __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1)  // both: at most 128 registers
     prefix_tile_kernel(PrefixParams p) {
   using Cfg = PrefixTileCfg<T, HD, STREAMS, WIDE>;
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
   auto& s_last = sync.s_last;
   uint32_t& s_tmem = sync.s_tmem;
 
-  trace_start(p.trace);
+  if constexpr (TRACE) trace_start(p.trace);
   const uint32_t q_s = smem_u32(gbase);
   const uint32_t k_ring = q_s + Cfg::K_RING;
   const uint32_t v_ring = q_s + Cfg::V_RING;
@@ -938,21 +938,21 @@ __global__ void __launch_bounds__(STREAMS == 1 ? 256 : 512, STREAMS == 1 ? 2 : 1
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
   }
-  trace_end(p.trace);
+  if constexpr (TRACE) trace_end(p.trace);
 }
 
 // ============================================================================ states of a row -> output
 constexpr int kJoinWarps = 4;
 
-template <typename T, int HD, int BATCH>
+template <typename T, int HD, int BATCH, bool TRACE>
 __global__ void __launch_bounds__(kJoinWarps * 32) prefix_join_kernel(PrefixParams p) {
   const int unit = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const bool on = unit < p.n_joins * p.n_heads;
   const PrefixJoin j = p.joins[on ? unit / p.n_heads : 0];
   griddep_wait();
-  trace_start(p.trace);
+  if constexpr (TRACE) trace_start(p.trace);
   if (on) join_states<T, HD, BATCH>(p, j, unit % p.n_heads);
-  trace_end(p.trace);
+  if constexpr (TRACE) trace_end(p.trace);
 }
 
 }  // namespace llm

@@ -401,7 +401,9 @@ double tile_clocks(const std::vector<PrefixItem>& items, int n_kv_heads, int max
   return ctas <= 4096 ? *std::max_element(free_at.begin(), free_at.end()) : sum / slots + longest / 2;
 }
 
-template <typename T, int HD>
+// TRACE: the kernels that record their timeline (p.trace).  They are instantiations of their own, since
+// the test of a null pointer costs a small call 0.1 us of 7 on the device.
+template <typename T, int HD, bool TRACE>
 cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, TraceRec* const* trace, cudaStream_t s, bool prepare) {
   if (prepare) {
     // the whole carve-out for shared memory, so that CTAs of both kernels fit an SM together
@@ -410,10 +412,10 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, TraceRec*
       return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                                          cudaSharedmemCarveoutMaxShared);
     };
-    cudaError_t e = set(prefix_tile_kernel<T, HD, 2, false>, PrefixTileCfg<T, HD, 2, false>::SMEM);
-    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 2, true>, PrefixTileCfg<T, HD, 2, true>::SMEM);
-    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 1, false>, PrefixTileCfg<T, HD, 1, false>::SMEM);
-    if (e == cudaSuccess) e = set(prefix_cols_kernel<T, HD>, kColsSmem<T, HD>);
+    cudaError_t e = set(prefix_tile_kernel<T, HD, 2, false, TRACE>, PrefixTileCfg<T, HD, 2, false>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 2, true, TRACE>, PrefixTileCfg<T, HD, 2, true>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_tile_kernel<T, HD, 1, false, TRACE>, PrefixTileCfg<T, HD, 1, false>::SMEM);
+    if (e == cudaSuccess) e = set(prefix_cols_kernel<T, HD, TRACE>, kColsSmem<T, HD>);
     return e;
   }
   bool first = true;  // the first launch waits for the stream's earlier work as a whole
@@ -421,14 +423,14 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, TraceRec*
   if (plan->n_items[kTile] > 0) {
     const int grid = plan->n_items[kTile] * plan->n_kv_heads;
     p.items = plan->items[kTile];
-    if (trace) p.trace = *trace++;
+    if constexpr (TRACE) p.trace = *trace++;
     auto launch = [&](auto kernel, int threads, int smem) { kernel<<<grid, threads, smem, s>>>(p); };
     using Wide = PrefixTileCfg<T, HD, 2, true>;
     using Narrow = PrefixTileCfg<T, HD, 2, false>;
     using Single = PrefixTileCfg<T, HD, 1, false>;
-    if (plan->variant == kWide) launch(prefix_tile_kernel<T, HD, 2, true>, Wide::THREADS, Wide::SMEM);
-    else if (plan->variant == kNarrow) launch(prefix_tile_kernel<T, HD, 2, false>, Narrow::THREADS, Narrow::SMEM);
-    else launch(prefix_tile_kernel<T, HD, 1, false>, Single::THREADS, Single::SMEM);
+    if (plan->variant == kWide) launch(prefix_tile_kernel<T, HD, 2, true, TRACE>, Wide::THREADS, Wide::SMEM);
+    else if (plan->variant == kNarrow) launch(prefix_tile_kernel<T, HD, 2, false, TRACE>, Narrow::THREADS, Narrow::SMEM);
+    else launch(prefix_tile_kernel<T, HD, 1, false, TRACE>, Single::THREADS, Single::SMEM);
     e = cudaGetLastError();
     first = false;
   }
@@ -436,30 +438,32 @@ cudaError_t prefix_launch(const llm_prefix_plan* plan, PrefixParams p, TraceRec*
     constexpr int smem = kColsSmem<T, HD>;
     const dim3 grid(plan->n_items[kCols] * plan->n_kv_heads), block(kAttnWarps * 32);
     p.items = plan->items[kCols];
-    if (trace) p.trace = *trace++;
+    if constexpr (TRACE) p.trace = *trace++;
     if (first) {
-      prefix_cols_kernel<T, HD><<<grid, block, smem, s>>>(p);
+      prefix_cols_kernel<T, HD, TRACE><<<grid, block, smem, s>>>(p);
       e = cudaGetLastError();
     } else {
-      e = launch_dependent(prefix_cols_kernel<T, HD>, grid, block, smem, s, p);
+      e = launch_dependent(prefix_cols_kernel<T, HD, TRACE>, grid, block, smem, s, p);
     }
   }
   if (e == cudaSuccess && plan->n_joins > 0 && !plan->tickets) {
-    if (trace) p.trace = *trace;
+    if constexpr (TRACE) p.trace = *trace;
     const long long units = static_cast<long long>(plan->n_joins) * plan->n_heads;
     const dim3 grid(static_cast<unsigned>((units + kJoinWarps - 1) / kJoinWarps)), block(kJoinWarps * 32);
-    e = plan->parts > 8 ? launch_dependent(prefix_join_kernel<T, HD, 20>, grid, block, 0, s, p)
-                        : launch_dependent(prefix_join_kernel<T, HD, 8>, grid, block, 0, s, p);
+    e = plan->parts > 8 ? launch_dependent(prefix_join_kernel<T, HD, 20, TRACE>, grid, block, 0, s, p)
+                        : launch_dependent(prefix_join_kernel<T, HD, 8, TRACE>, grid, block, 0, s, p);
   }
   return e;
 }
 
-// `trace`: nullptr, or the timeline records of the launches in their order.
+template <bool TRACE>
 cudaError_t prefix_any(const llm_prefix_plan* plan, const PrefixParams& p, TraceRec* const* trace, cudaStream_t s, bool prepare) {
   const bool bf = plan->dtype == LLM_DTYPE_BF16;
   if (plan->head_dim == 64)
-    return bf ? prefix_launch<__nv_bfloat16, 64>(plan, p, trace, s, prepare) : prefix_launch<__half, 64>(plan, p, trace, s, prepare);
-  return bf ? prefix_launch<__nv_bfloat16, 128>(plan, p, trace, s, prepare) : prefix_launch<__half, 128>(plan, p, trace, s, prepare);
+    return bf ? prefix_launch<__nv_bfloat16, 64, TRACE>(plan, p, trace, s, prepare)
+              : prefix_launch<__half, 64, TRACE>(plan, p, trace, s, prepare);
+  return bf ? prefix_launch<__nv_bfloat16, 128, TRACE>(plan, p, trace, s, prepare)
+            : prefix_launch<__half, 128, TRACE>(plan, p, trace, s, prepare);
 }
 
 // What a plan fixes of its launches.
@@ -497,7 +501,9 @@ cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_
   p.n_pages = r.n_pages;
   p.max_pages = r.max_pages;
   p.scale_log2 = scale_log2(1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
-  return prefix_any(plan, p, r.trace, s, false);
+  if (!r.trace[0]) return prefix_any<false>(plan, p, nullptr, s, false);
+  const cudaError_t e = prefix_any<true>(plan, p, nullptr, s, true);
+  return e == cudaSuccess ? prefix_any<true>(plan, p, r.trace, s, false) : e;
 }
 
 int llm_detail_prefix_launches(const llm_prefix_plan* plan, const char* (*names)[3]) {
@@ -647,7 +653,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     // may come on a stream that is not ordered with the null stream: wait for them here.
     e = cudaMemcpy(p->block, host.data(), host.size(), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
-    if (e == cudaSuccess) e = prefix_any(p, PrefixParams{}, nullptr, nullptr, true);
+    if (e == cudaSuccess) e = prefix_any<false>(p, PrefixParams{}, nullptr, nullptr, true);
     if (e != cudaSuccess) {
       llm_prefix_plan_destroy(p);
       return fail_fmt(LLM_ERR_CUDA, "plan set-up failed: %s", cudaGetErrorString(e));
@@ -703,6 +709,6 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   p.n_pages = c->n_pages;
   p.max_pages = c->max_pages;
   p.scale_log2 = scale_log2(scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(plan->head_dim)));
-  CU(prefix_any(plan, p, nullptr, static_cast<cudaStream_t>(stream), false));
+  CU(prefix_any<false>(plan, p, nullptr, static_cast<cudaStream_t>(stream), false));
   return LLM_OK;
 }
