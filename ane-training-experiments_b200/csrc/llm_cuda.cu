@@ -575,6 +575,7 @@ struct GraphKey {
 struct PrefixUse {
   llm_prefix_plan* plan = nullptr;
   std::vector<int> key;  // the batch's sequences, its groups, the sharing generation
+  double saved = 0;      // positions that the batch shares and per-sequence attention would read again
 };
 
 struct llm_ctx {
@@ -1499,6 +1500,7 @@ int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const i
                                 static_cast<int>(sizes.size()), static_cast<int>(width) * 16, &use.plan));
     use.key = std::move(key);
   }
+  use.saved = saved;
   *plan = use.plan;
   c->prefix_launches = llm_detail_prefix_launches(use.plan);
   return LLM_OK;
@@ -1672,6 +1674,22 @@ bool sampling_on(const llm_ctx* c) { return c->sample_temp > 1e-6f; }
 // Launch timeline records one traced step may use.
 constexpr size_t kTraceCap = 1024;
 
+// One layer's attention over shared prefixes of the rows in qbuf at d_pos.
+llm_prefix_rows prefix_rows(const llm_ctx* c, int layer) {
+  llm_prefix_rows pr{};
+  pr.q = c->qbuf;
+  pr.out = c->attn;
+  pr.out_f32 = c->in8 ? 1 : 0;
+  pr.positions = c->d_pos;
+  pr.layer_pool = static_cast<const uint8_t*>(c->kv_pool) +
+                  static_cast<size_t>(layer) * c->n_pages * c->kv_dim * 2 * 16 * act_bytes(c);
+  pr.table = c->d_block_table;
+  pr.n_pages = c->n_pages;
+  pr.max_pages = c->max_pages_per_seq;
+  pr.status = c->d_err;
+  return pr;
+}
+
 int enqueue_forward(llm_ctx* c, const RowsSpec& rs) {
   t_use_pdl = c->use_pdl;
   t_prio = 0;
@@ -1833,16 +1851,7 @@ int enqueue_forward(llm_ctx* c, const RowsSpec& rs) {
       return LLM_OK;
     }
     if (rs.prefix) {  // shared pages once per group, then the int8 quantiser
-      llm_prefix_rows pr{};
-      pr.q = c->qbuf;
-      pr.out = c->attn;
-      pr.out_f32 = i8 ? 1 : 0;
-      pr.positions = c->d_pos;
-      pr.layer_pool = bytes(c->kv_pool, static_cast<size_t>(l) * c->n_pages * KV * 2 * 16 * ab);
-      pr.table = c->d_block_table;
-      pr.n_pages = c->n_pages;
-      pr.max_pages = c->max_pages_per_seq;
-      pr.status = c->d_err;
+      llm_prefix_rows pr = prefix_rows(c, l);
       const char* names[3];
       for (int i = 0, n = llm_detail_prefix_launches(rs.prefix, &names); i < n; ++i) pr.trace[i] = tr(names[i], l, P);
       t_prio = 0;
@@ -2812,20 +2821,19 @@ extern "C" int llm_time_attention(llm_ctx* c, int iters, double* us_per_launch, 
   ap.ws = c->ws;
   ap.counters = c->counters;
   ap.err = c->d_err;
+  auto layer = [&](int l) -> cudaError_t {
+    if (c->gen_plan) return llm_detail_prefix_run(c->gen_plan, prefix_rows(c, l), c->stream);
+    ap.layer = l;
+    return attn_any(c->act, k.head_dim, ap, c->stream, false);
+  };
   cudaEvent_t e0, e1;
   CU(cudaEventCreate(&e0));
   CU(cudaEventCreate(&e1));
   // warm-up pass over every layer
-  for (int l = 0; l < k.n_layers; ++l) {
-    ap.layer = l;
-    CU(attn_any(c->act, k.head_dim, ap, c->stream, false));
-  }
+  for (int l = 0; l < k.n_layers; ++l) CU(layer(l));
   CU(cudaEventRecord(e0, c->stream));
   for (int i = 0; i < iters; ++i)
-    for (int l = 0; l < k.n_layers; ++l) {
-      ap.layer = l;
-      CU(attn_any(c->act, k.head_dim, ap, c->stream, false));
-    }
+    for (int l = 0; l < k.n_layers; ++l) CU(layer(l));
   CU(cudaEventRecord(e1, c->stream));
   CU(cudaEventSynchronize(e1));
   float ms = 0.f;
@@ -2837,10 +2845,11 @@ extern "C" int llm_time_attention(llm_ctx* c, int iters, double* us_per_launch, 
   if (us_per_launch) *us_per_launch = ms * 1e3 / launches;
   if (bytes_per_launch) {
     // K and V of every cached position of the context (positions 0 .. pos0 + done - 1,
-    // inclusive), the q rows read and the attention rows written
+    // inclusive; shared ones once per group), the q rows read and the attention rows written
     double b = 0;
     const double per_tok = 2.0 * c->kv_dim * act_bytes(c);
     for (int i = 0; i < c->gen_n; ++i) b += per_tok * (c->gen_pos0[i] + c->gen_steps_done);
+    if (c->gen_plan) b -= per_tok * c->gen_prefix.saved;
     b += static_cast<double>(c->gen_n) * c->q_dim * act_bytes(c);
     b += static_cast<double>(c->gen_n) * c->q_dim * (c->in8 ? 4.0 : static_cast<double>(act_bytes(c)));
     *bytes_per_launch = b;

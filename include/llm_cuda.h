@@ -290,7 +290,9 @@ int llm_memory_bytes(llm_ctx *ctx, uint64_t *weights, uint64_t *kv_pool, uint64_
  * current generate batch at the positions of its last executed step (at least one
  * llm_generate_steps step must have run) with CUDA events on the context stream; returns
  * the mean duration of one launch in microseconds and the algorithmic bytes one launch
- * reads and writes.  The generate state is left as it was. */
+ * reads and writes.  Of a batch over shared prefixes (LLM_OPT_SHARED_PREFIX) it times that attention, all
+ * launches of a layer as one, and counts shared positions once per group.  The generate state is
+ * left as it was. */
 int llm_time_attention(llm_ctx *ctx, int iters, double *us_per_launch, double *bytes_per_launch);
 
 /* Run `iters` decode steps of the current generate batch eagerly with a CUDA event after

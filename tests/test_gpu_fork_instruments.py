@@ -1,5 +1,5 @@
-"""What a context says of a decode step over shared prefixes: the launches it counts and the
-timeline that it records."""
+"""What a context says of a decode step over shared prefixes: the launches it counts, the timeline it
+records, the attention it times and the bytes that it gives for it."""
 import numpy as np
 import pytest
 
@@ -7,6 +7,8 @@ from ane import _abi
 from test_gpu_fork import CFG, MHA, engine
 
 pytestmark = pytest.mark.gpu
+
+ACT = 2  # bytes of a K or V value
 
 
 def batch(cfg, dtype, mode):
@@ -61,3 +63,26 @@ def test_the_timeline_has_every_launch_that_is_counted(cfg, dtype, mode):
     for layer in range(cfg.n_layers):
         assert any("attention" in line and f" L{layer} " in line for line in launches(table)), table
     eng.close()
+
+
+@pytest.mark.parametrize("cfg,dtype", [(CFG, "bf16"), (MHA, "fp16"), (CFG, "w8a8_bf16")])
+def test_the_timed_attention_is_the_step_s(cfg, dtype):
+    n = 8
+    per = 2 * cfg.n_kv_heads * cfg.head_dim * ACT
+    rows = n * cfg.n_heads * cfg.head_dim * (ACT + (4 if dtype.startswith("w8a8") else ACT))
+    out = []
+    for mode in (0, 2):
+        eng, seqs, pos = batch(cfg, dtype, mode)
+        eng.generate_steps(2)
+        us, nbytes = eng.time_attention(2)
+        assert us > 0
+        # 64 positions of the five and 32 of the two are read once
+        saved = 0 if mode == 0 else 4 * 64 + 32
+        assert nbytes == per * (sum(pos) + 2 * n - saved) + rows
+        eng.generate_steps(4)                  # the state is as it was
+        out.append(eng.generate_end())
+        eng.close()
+    plain, _, _ = batch(cfg, dtype, 2)
+    plain.generate_steps(6)
+    np.testing.assert_array_equal(out[1], plain.generate_end())
+    plain.close()
