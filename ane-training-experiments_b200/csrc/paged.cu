@@ -482,6 +482,18 @@ PrefixParams plan_params(const llm_prefix_plan* plan) {
   return p;
 }
 
+// Whether two of the vectors of `len` elements at r * row + h * head, r < rows and h < heads, overlap.
+bool vectors_overlap(long long rows, long long heads, long long row, long long head, long long len) {
+  if ((heads == 1 || head >= len) && (rows == 1 || row >= (heads - 1) * head + len)) return false;  // row by row
+  if ((rows == 1 || row >= len) && (heads == 1 || head >= (rows - 1) * row + len)) return false;    // head by head
+  if (rows > 1 && row < len) return true;
+  for (long long h = 1; h < heads; ++h) {  // the rows whose distance is nearest to that of h heads
+    const long long x = h * head, r = row > 0 ? std::min(x / row, rows - 1) : 0;
+    if (x - r * row < len || (r + 1 < rows && (r + 1) * row - x < len)) return true;
+  }
+  return false;
+}
+
 float scale_log2(double scale) { return static_cast<float>(scale * 1.4426950408889634); }
 
 }  // namespace
@@ -690,6 +702,9 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   for (int64_t s : {q_row, q_head, o_row, o_head})
     if (s % 8 != 0 || s < 0 || s > (int64_t{1} << 40))
       return fail_fmt(LLM_ERR_INVALID, "stride %lld (a multiple of 8 elements is needed)", static_cast<long long>(s));
+  if (vectors_overlap(plan->n_rows, plan->n_heads, o_row, o_head, plan->head_dim))
+    return fail_fmt(LLM_ERR_INVALID, "rows or heads of out overlap (strides %lld and %lld)", static_cast<long long>(o_row),
+                    static_cast<long long>(o_head));
   if (!std::isfinite(scale)) return fail_fmt(LLM_ERR_INVALID, "scale is not finite");
   DeviceScope dev;
   RC(dev.enter(plan->device));

@@ -449,10 +449,11 @@ int llm_prefix_plan_create(int device, int dtype, int n_heads, int n_kv_heads, i
                            int n_groups, int max_ctx, llm_prefix_plan **out);
 /* Enqueue the attention of `layer` on `stream`; returns without waiting.  ctx [n_seqs] (int32), q and
  * out (the cache's dtype; row and head strides in elements, head_dim contiguous, strides multiples
- * of 8, 16-byte aligned) and lse (NULL, or f32 [rows][n_heads]: the log of each row's sum of
- * exp(scale * q.k), -inf for a row that sees nothing) are device memory.  scale <= 0 means
- * 1 / sqrt(head_dim).  Calls on one plan must be ordered (they share its workspace).  A context
- * beyond max_ctx or the block table, or a bad page, sets the cache's status. */
+ * of 8, 16-byte aligned; out's (row, head) vectors overlap neither one another nor q) and lse (NULL,
+ * or f32 [rows][n_heads]: the log of each row's sum of exp(scale * q.k), -inf for a row that sees
+ * nothing) are device memory.  scale <= 0 means 1 / sqrt(head_dim).  Calls on one plan must be
+ * ordered (they share its workspace).  A context beyond max_ctx or the block table, or a bad page,
+ * sets the cache's status. */
 int llm_prefix_attend(llm_prefix_plan *plan, const llm_page_cache *cache, int layer, const int32_t *ctx, const void *q,
                       int64_t q_row_stride, int64_t q_head_stride, float scale, void *out, int64_t out_row_stride,
                       int64_t out_head_stride, float *lse, void *stream);

@@ -33,7 +33,10 @@ static void* legacy(void* s) { return s == (void*)1 ? NULL : s; } /* cudaStreamL
 int cudaGetDevice(int* d) { return *d = 0, 0; }
 int cudaSetDevice(int d) { return 0; }
 int cudaFuncSetAttribute(const void* f, int a, int v) { return 0; }
-int cudaGetLastError(void) { return 0; }
+static int last; /* launches fail for want of a device */
+int cudaLaunchKernel(const void* f, ...) { return last = 100; }
+int cudaLaunchKernelExC(const void* c, const void* f, void** a) { return last = 100; }
+int cudaGetLastError(void) { int e = last; last = 0; return e; }
 int cudaMalloc(void** p, size_t n) { *p = calloc(n ? n : 1, 1); ++allocations; return *p ? 0 : 2; }
 int cudaFree(void* p) { if (p) --allocations; free(p); return 0; }
 int cudaMemcpyAsync(void* d, const void* s, size_t n, int kind, void* stream) {
@@ -75,5 +78,5 @@ def test_a_new_plan_is_on_the_device(tmp_path, fail):
     child.write_text(CHILD)
     subprocess.run(["cc", "-shared", "-fPIC", "-w", "-o", str(so), str(src)], check=True)
     r = subprocess.run([sys.executable, str(child), str(so), str(Path(_abi.LIB_PATH)), str(fail)], capture_output=True, text=True,
-                       timeout=120, env={**os.environ, "LD_PRELOAD": str(so)})
+                       timeout=120, env={**os.environ, "LD_PRELOAD": str(so), "CUDA_VISIBLE_DEVICES": ""})
     assert r.returncode == 0 and "complete" in r.stdout, r.stdout + r.stderr
