@@ -699,6 +699,8 @@ extern "C" int llm_prefix_attend(llm_prefix_plan* plan, const llm_page_cache* c,
   if (!ctx || !q || !out) return fail_fmt(LLM_ERR_INVALID, "nil buffer");
   if (!aligned(ctx, 4) || !aligned(q, 16) || !aligned(out, 16) || !aligned(lse, 4))
     return fail_fmt(LLM_ERR_INVALID, "misaligned buffer (q and out need 16-byte, ctx and lse 4-byte alignment)");
+  if (plan->n_rows == 1) q_row = o_row = 0;  // no address is formed with these strides
+  if (plan->n_heads == 1) q_head = o_head = 0;
   for (int64_t s : {q_row, q_head, o_row, o_head})
     if (s % 8 != 0 || s < 0 || s > (int64_t{1} << 40))
       return fail_fmt(LLM_ERR_INVALID, "stride %lld (a multiple of 8 elements is needed)", static_cast<long long>(s));

@@ -1,7 +1,8 @@
 """Strides of llm_prefix_attend, without a GPU: the library runs in a child process over stand-ins of
 the runtime calls that a plan makes (test_plan_upload_host), and what passes the checks ends in a
 launch, which the stand-in refuses.  An output whose (row, head) vectors overlap would be
-written by several CTAs at once; it is refused."""
+written by several CTAs at once; it is refused.  A stride that no address is formed with (of a
+single row or head) is not looked at."""
 import os
 import subprocess
 import sys
@@ -58,6 +59,9 @@ for rows, heads in (((1, 1), 4), ((3,), 2), ((2, 1, 2), 6), ((1,), 4), ((5,), 1)
             rc, text = attend(rows, heads, 1, row, head, heads * 64, 64)
             assert rc == _abi.LLM_ERR_CUDA, (rc, text)
 assert bad > 50
+for q_row, q_head, rows, heads in ((260, 64, (1,), 4), (-4, 64, (1,), 4), (64, 3, (2, 1), 1), (7, 9, (1,), 1)):
+    for args in ((q_row, q_head, 4096, 64), (4096, 64, q_row, q_head)):
+        assert attend(rows, heads, 1, *args)[0] == _abi.LLM_ERR_CUDA, args
 for args in ((260, 64, 256, 64), (256, 60, 256, 64), (256, 64, 260, 64), (256, 64, 256, 68), (-256, 64, 256, 64), (256, 64, 256, -64)):
     rc, text = attend((2, 1), 4, 1, *args)
     assert rc == _abi.LLM_ERR_INVALID and "stride" in text, args
