@@ -738,8 +738,7 @@ int check_device_error(llm_ctx* c) {
   if (h != kDevOk) {
     CU(cudaMemsetAsync(c->d_err, 0, sizeof(int), c->stream));
     CU(cudaStreamSynchronize(c->stream));
-    return fail(LLM_ERR_DEVICE, "kernel reported device error %d (%s)", h,
-                h == kDevWaitTimeout ? "bounded wait expired" : (h == kDevBadPage ? "bad page index" : "unknown"));
+    return fail(LLM_ERR_DEVICE, "kernel reported device error %d (%s)", h, llm_detail_device_error(h));
   }
   return LLM_OK;
 }

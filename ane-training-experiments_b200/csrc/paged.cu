@@ -154,10 +154,18 @@ extern "C" int llm_pages_status(int device, const llm_page_cache* c, void* strea
   switch (h) {
     case kPageExhausted: return fail_fmt(LLM_ERR_OOM, "KV page pool exhausted");
     case kPageBadRequest: return fail_fmt(LLM_ERR_INVALID, "page request names a slot, page or length out of range, or a slot twice");
-    case kDevWaitTimeout: return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (bounded wait expired)", h);
-    case kDevBadPage: return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (bad page index)", h);
   }
-  return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (unknown)", h);
+  return fail_fmt(LLM_ERR_DEVICE, "kernel reported device error %d (%s)", h, llm_detail_device_error(h));
+}
+
+const char* llm_detail_device_error(int code) {
+  switch (code) {
+    case kDevWaitTimeout: return "bounded wait expired";
+    case kDevBadPage: return "bad page index";
+    case kPageExhausted: return "KV page pool exhausted";
+    case kPageBadRequest: return "slot, page or length out of range";
+  }
+  return "unknown";
 }
 
 extern "C" int llm_pages_copy(int device, const llm_page_cache* from, const llm_page_cache* to, const int32_t* src,
