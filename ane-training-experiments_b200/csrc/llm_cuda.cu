@@ -1280,8 +1280,9 @@ extern "C" int llm_seq_fork(llm_ctx* c, int parent, const int32_t* children, int
   }
   const int keep = len / 16;
   const bool tail = len % 16 != 0;
-  if (tail && c->free_pages.size() < static_cast<size_t>(n)) return fail(LLM_ERR_OOM, "KV page pool exhausted");
   if (n == 0) return LLM_OK;
+  // A free page for each child's partly filled one is always there: the pool has max_pages_per_seq >= 1
+  // pages for every slot, and the children hold none of theirs.
   RC(set_device(c));
   const size_t width = c->max_pages_per_seq;
   const int* from = c->h_block_table.data() + static_cast<size_t>(parent) * width;
