@@ -15,8 +15,9 @@
 //   copy     listed pages, every layer
 //
 // Every table is an int32 array on the device, so parents chosen by a kernel (beam search) need
-// no host round trip and a step can be captured in a CUDA graph.  A request that cannot be
-// served writes `status` and changes nothing.
+// no host round trip and a step can be captured in a CUDA graph.  What cannot be served writes
+// `status`: a fork with any bad request changes nothing; copy, free and compact skip the entries
+// that are out of range and do the rest.
 #pragma once
 #include "common.cuh"
 

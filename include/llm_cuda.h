@@ -407,7 +407,8 @@ size_t llm_pages_work_words(int n_pages, int max_seqs);
 int llm_pages_status(int device, const llm_page_cache *cache, void *stream);
 /* Copy page src[i] of `from` to page dst[i] of `to` in every layer, i < n.  The caches have the
  * same layers, heads, head_dim and dtype, are both in the memory of `device`, and may be one cache; no
- * dst[i] appears twice or among the sources of the same pool.  Tables are not changed. */
+ * dst[i] appears twice or among the sources of the same pool.  Tables are not changed.  Pairs with a
+ * page out of range are skipped and reported in from's status. */
 int llm_pages_copy(int device, const llm_page_cache *from, const llm_page_cache *to, const int32_t *src,
                    const int32_t *dst, int n, void *stream);
 /* Request i makes slot children[i] a copy of the first lens[i] positions of slot parents[i], with
@@ -419,11 +420,13 @@ int llm_pages_copy(int device, const llm_page_cache *from, const llm_page_cache 
 int llm_pages_fork(int device, const llm_page_cache *cache, const int32_t *parents, const int32_t *children,
                    const int32_t *lens, const int32_t *rooms, int n, void *stream);
 /* Empty slots[i], i < n: refs - 1 for each of their pages; pages that reach 0 go on the free stack
- * in ascending order.  An empty slot, or one listed again, changes nothing. */
+ * in ascending order.  An empty slot, or one listed again, changes nothing; slots out of range are
+ * skipped and reported. */
 int llm_pages_free(int device, const llm_page_cache *cache, const int32_t *slots, int n, void *stream);
 /* Move the live pages to pages 0..L-1 (L = pages with references) in every layer with the fewest
  * moves: the k-th live page at or above L goes to the k-th free page below it.  Block table and
- * references follow; the free stack hands out L, L + 1, ... next. */
+ * references follow; the free stack hands out L, L + 1, ... next.  An entry at or above L that names a page
+ * without references is left as it is and reported. */
 int llm_pages_compact(int device, const llm_page_cache *cache, void *stream);
 
 /* ---------------------------------------------------------------- attention over shared prefixes */
