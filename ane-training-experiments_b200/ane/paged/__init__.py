@@ -98,22 +98,23 @@ class PagedCache:
         to = self if to is None else to
         if not isinstance(to, PagedCache) or to.device != self.device:
             raise LLMError(_abi.LLM_ERR_INVALID, f"`to` must be a PagedCache on {self.device}, not {getattr(to, 'device', to)}")
+        at = self._ints(src, "src")
         n = src.numel()
-        _abi.check(self._lib.llm_pages_copy(self.device.index, self._ref, to._ref, self._ints(src, "src"),
-                                            self._ints(dst, "dst", n), n, self._stream()))
+        _abi.check(self._lib.llm_pages_copy(self.device.index, self._ref, to._ref, at, self._ints(dst, "dst", n), n,
+                                            self._stream()))
 
     def fork(self, parents, children, lens, rooms) -> None:
         """Slot children[i] becomes the first lens[i] positions of slot parents[i] (-1: a new
         sequence; the slot itself: it grows), with pages for rooms[i] positions; all or none."""
+        at = self._ints(parents, "parents")
         n = parents.numel()
-        _abi.check(self._lib.llm_pages_fork(self.device.index, self._ref, self._ints(parents, "parents"),
-                                            self._ints(children, "children", n), self._ints(lens, "lens", n),
-                                            self._ints(rooms, "rooms", n), n, self._stream()))
+        _abi.check(self._lib.llm_pages_fork(self.device.index, self._ref, at, self._ints(children, "children", n),
+                                            self._ints(lens, "lens", n), self._ints(rooms, "rooms", n), n, self._stream()))
 
     def free(self, slots) -> None:
         """Empty the slots; pages without references go back on the free stack, ascending."""
-        _abi.check(self._lib.llm_pages_free(self.device.index, self._ref, self._ints(slots, "slots"), slots.numel(),
-                                            self._stream()))
+        at = self._ints(slots, "slots")
+        _abi.check(self._lib.llm_pages_free(self.device.index, self._ref, at, slots.numel(), self._stream()))
 
     def compact(self) -> None:
         """Move the live pages to the pool's start with the fewest moves."""

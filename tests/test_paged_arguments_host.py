@@ -47,3 +47,15 @@ def test_a_copy_into_a_cache_on_another_gpu_is_refused():
     with pytest.raises(_abi.LLMError) as e:
         a.copy(*lists, to="elsewhere")
     assert e.value.code == INVALID
+
+
+def test_lists_that_are_not_tensors_are_refused_like_other_arguments():
+    import torch
+    from ane.paged import PagedCache
+    c = object.__new__(PagedCache)
+    c._lib, c.device, c.c_struct = _abi.lib(), torch.device("cuda", 0), cache()
+    c._ref, c._stream = C.addressof(c.c_struct), lambda: 0
+    for call in (lambda: c.copy([1], [2]), lambda: c.fork([-1], [0], [0], [16]), lambda: c.free([0]), lambda: c.free(None)):
+        with pytest.raises(_abi.LLMError) as e:
+            call()
+        assert e.value.code == INVALID
