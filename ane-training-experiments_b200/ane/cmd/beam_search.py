@@ -32,7 +32,10 @@ class Model:
     dtype: str
 
 
-def random_model(seed: int, vocab=500, dim=128, heads=4, kv_heads=2, head_dim=64, layers=2, dtype="bf16") -> Model:
+VOCAB = 500
+
+
+def random_model(seed: int, vocab=VOCAB, dim=128, heads=4, kv_heads=2, head_dim=64, layers=2, dtype="bf16") -> Model:
     g = torch.Generator(device="cuda").manual_seed(seed)
     w = lambda *s: torch.randn(s, generator=g, device="cuda") / math.sqrt(dim)  # noqa: E731
     return Model(3 * w(vocab, dim), [(2 * w(dim, heads, head_dim), 2 * w(dim, kv_heads, head_dim), w(dim, kv_heads, head_dim),
@@ -131,6 +134,8 @@ def main(argv=None) -> int:
     a = ap.parse_args(argv)
     if min(a.beams, a.prompt, a.steps) <= 0:
         ap.error("-beams, -prompt and -steps must be positive")
+    if a.beams > VOCAB:
+        ap.error(f"-beams: the first step has {VOCAB} continuations")
     m = random_model(a.seed, dtype=a.dtype)
     g = torch.Generator().manual_seed(a.seed)
     s = Search(m, a.beams, torch.randint(0, m.embed.shape[0], (a.prompt,), generator=g).tolist(), a.steps)

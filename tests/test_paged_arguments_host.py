@@ -59,3 +59,10 @@ def test_lists_that_are_not_tensors_are_refused_like_other_arguments():
         with pytest.raises(_abi.LLMError) as e:
             call()
         assert e.value.code == INVALID
+
+
+def test_more_beams_than_tokens_are_refused():
+    from ane.cmd import beam_search
+    for n in ("501", "100000"):
+        with pytest.raises(SystemExit):
+            beam_search.main(["-beams", n])
