@@ -88,8 +88,8 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
 
 // One warp joins the states of (row, head) and writes the output.  Lane k weighs states k and k + 32
 // (kMaxParts is 64); then a lane adds its HD / 32 dimensions of BATCH states at a time: 8, or 20 where
-// rows have more (18 states of 64 rows: 2.5 us after the last item against 4; but 152 registers, which
-// costs 4 us where 4096 rows and heads have four states each).
+// rows have more (18 states of 64 rows: 2.5 us after the last item against 4; but 128 registers at
+// head_dim 128 against 63, which costs 4 us where 4096 rows and heads have four states each).
 constexpr int kMaxParts = 64;
 
 template <typename T, int HD, int BATCH>
@@ -415,7 +415,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, HD == 64 ? 5 : 4) prefix_cols
 // 64 and O) and four softmax warps with one score row per thread.  64 positions at a time a stream
 // runs S = Q . K^T, softmax, P back over the S columns as hi + lo terms, O += P . V with P from
 // TMEM; the reference max of a row moves only when a tile exceeds it by 2^8 (the pipeline of
-// attn_prefill_tc_kernel, whose header explains it).
+// attn_prefill_tc_kernel, whose header explains it).  The two terms of P leave 2^-17 of a weight in bf16
+// (2^-22 in fp16), about 2^-18 of a sum: one bf16 output in about 1700 rounds to the neighbour of
+// what a sum in f32 rounds to.
 //   more than 128 rows  the streams are two row tiles that share every K/V tile.  At the memory's rate
 //                       an SM gets 24 bytes a clock, 1300 clocks for the 32 KB of a 64-position tile
 //                       of head_dim 128; a row tile takes the tensor core 900 clocks for it (S 384,

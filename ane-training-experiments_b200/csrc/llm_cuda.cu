@@ -1448,9 +1448,10 @@ int attn_splits_for(const llm_ctx* c, int n_blocks, int max_ctx) {
 // sequence.  Sequences with the same first page form a group; its prefix is the pages that all of
 // them have in common and none writes.  Per sequence, shared pages come from L2 after the first
 // reader, and a shared step makes up to two launches a layer more; it gains once the K/V bytes it
-// saves take kPrefixExtraUs to stream.  Measured, ms per step per sequence / shared: Qwen3-0.6B bf16,
-// 128 samples of one prompt of 64 tokens 1.71 / 1.87, 128 1.79 / 1.87, 256 1.96 / 1.88, 1024 3.78 / 2.18;
-// Stories110M fp16, 64 of 128 0.54 / 0.60, 256 of 192 0.87 / 0.80.
+// saves take kPrefixExtraUs to stream.  Measured (40 steps of the device-resident loop, events on the
+// stream), ms per step per sequence / shared: Qwen3-0.6B bf16, 128 samples of one prompt of 64 tokens
+// 1.70 / 1.85, 128 1.79 / 1.86, 256 1.95 / 1.87, 512 2.34 / 1.93, 1024 3.77 / 1.90; W8A8, 256 of 1024
+// 4.89 / 2.68; Stories110M fp16, 64 of 128 0.54 / 0.59, 256 of 192 0.87 / 0.81.
 constexpr double kPrefixExtraUs = 15.0;
 int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const int32_t* pos, const llm_prefix_plan** plan) {
   *plan = nullptr;

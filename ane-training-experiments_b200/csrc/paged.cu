@@ -333,11 +333,17 @@ long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int3
       alone += (rho + 127) / 128;
       own_ctas += tiles_of(rho, tile_rows) * n_kv_heads;
     }
-    // sharing pays when stacking the rows leaves fewer 128-row steps over the prefix
+    // Sharing pays when stacking the rows leaves fewer 128-row steps over the prefix.  One group of 2 to
+    // 10 sequences of 40 to 200 score rows, time shared over not shared (geometric mean, both head
+    // sizes): steps of at most 0.7 of the sequences' own 0.88 after 4096 positions (0.62..1.19) and
+    // 1.00 after 512; more steps than that 0.99 after either (0.72..1.59), so those stay apart.
     pg.shared = active >= 2 && prefixes[g] > 0 && (pg.rho + 127) / 128 * 10 <= alone * 7;
     groups.push_back(pg);
   }
-  // pieces of the own ranges, when one item a sequence leaves most of the machine idle
+  // Pieces of the own ranges, when one item a sequence leaves most of the machine idle.  One sequence of
+  // 16000 own positions, eight kv heads of 128: 190 us in one piece, 20.5 in pieces; 16 sequences 220
+  // and 164.  From 148 CTAs on they stay whole, which costs long ranges: 24 sequences of 16000 take
+  // 260 us and would 228 in pieces for 444 CTAs, 16 of them with twelve heads of 64 242 and 146.
   const int pieces = own_ctas >= 148 ? 1 : static_cast<int>(std::min<long long>(16, 296 / std::max(1ll, own_ctas)));
   const int len[2] = {part_length(groups, kTile, n_kv_heads, kernel_slots(kTile, head_dim), tile_rows),
                       part_length(groups, kCols, n_kv_heads, kernel_slots(kCols, head_dim), tile_rows)};
@@ -389,7 +395,10 @@ long long plan_items(const int32_t* rows, const int32_t* group_sizes, const int3
 // the CTA slot that is free first.  A CTA's clocks a 64-position step and its start and end are
 // measured (24 prompts of 51..203 rows after 2048 positions; two CTAs of the single variant share an
 // SM's tensor core, so each takes longer): 113 us wide, 100 us single; five groups of 79 rows and
-// eight heads on 14960 positions: 67 us wide, 76 us single.
+// eight heads on 14960 positions: 67 us wide, 76 us single.  Over 210 batches without a shared prefix (8
+// to 64 sequences, 200 to 400 score rows, 256 to 4096 positions) its choice takes 0.91 of the wide
+// variant's time, and 1.02 (head_dim 128) or 1.06 (64, whose steps are shorter than these) of the
+// single one's.
 double tile_clocks(const std::vector<PrefixItem>& items, int n_kv_heads, int max_ctx, int variant) {
   const int slots = variant == kSingle ? 296 : 148;
   std::vector<double> free_at(slots, 0.0);  // a heap, earliest first
@@ -602,7 +611,10 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     int parts = 0;
     // Rows in pairs of 128-row tiles read each K/V tile once for both; single tiles spread better and
     // start and end beside one another.  Without pairs, one stream a CTA once the CTAs are more than
-    // one and a half to an SM.
+    // one and a half to an SM.  Two streams over one stream, without a shared prefix (144 batches of 8 to
+    // 64 sequences, 60 and 120 score rows): 1.08 of its time up to 148 CTAs, 1.22 up to 222, 1.17 to 1.28
+    // above; on long shared prefixes two streams are the faster: 64 rows on 32768 positions 41.2 us
+    // against 43.5, eight families of 32 101 against 102.
     long long n_states = 0;
     int variant = kNarrow;
     for (int v : {kWide, kSingle}) {
