@@ -1482,7 +1482,7 @@ int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const i
   std::vector<int> key(seq, seq + n);
   for (const auto* v : {&order, &sizes, &prefixes}) key.insert(key.end(), v->begin(), v->end());
   key.push_back(c->share_gen);
-  if (!use.plan || use.key != key) {
+  if (use.key != key || (!use.plan && c->shared_prefix == 2)) {
     CU(cudaStreamSynchronize(c->stream));
     // graphs that replay the old plan's launches
     for (auto it = c->graphs.begin(); it != c->graphs.end();) {
@@ -1495,12 +1495,16 @@ int choose_prefix(llm_ctx* c, PrefixUse& use, int n, const int32_t* seq, const i
     }
     if (use.plan) llm_prefix_plan_destroy(use.plan);
     use.plan = nullptr;
+    use.key.clear();
     std::vector<int> ones(n, 1);
-    RC(llm_detail_prefix_create(c->device, c->act == 1 ? LLM_DTYPE_F16 : LLM_DTYPE_BF16, c->cfg.n_heads, c->cfg.n_kv_heads,
-                                c->cfg.head_dim, seq, ones.data(), n, order.data(), sizes.data(), prefixes.data(),
-                                static_cast<int>(sizes.size()), static_cast<int>(width) * 16, &use.plan));
+    const int rc = llm_detail_prefix_create(c->device, c->act == 1 ? LLM_DTYPE_F16 : LLM_DTYPE_BF16, c->cfg.n_heads,
+                                            c->cfg.n_kv_heads, c->cfg.head_dim, seq, ones.data(), n, order.data(),
+                                            sizes.data(), prefixes.data(), static_cast<int>(sizes.size()),
+                                            static_cast<int>(width) * 16, &use.plan);
+    if (rc != LLM_OK && (rc != LLM_ERR_OOM || c->shared_prefix == 2)) return rc;
     use.key = std::move(key);
   }
+  if (!use.plan) return LLM_OK;  // no memory for it: not tried again until the batch or its sharing changes
   use.saved = saved;
   *plan = use.plan;
   c->prefix_launches = llm_detail_prefix_launches(use.plan);

@@ -263,7 +263,8 @@ int llm_debug_sample(int device, const float *logits, int rows, int vocab, float
                                     from 0; int8 models never split) */
 #define LLM_OPT_SHARED_PREFIX 18 /* decode steps whose sequences share pages (llm_seq_fork) read them once
                                     per group: 0 never, 1 when that saves more K/V time than its
-                                    extra launches take (default), 2 always.  Attention sums in
+                                    extra launches take and its workspace of a few MB can be
+                                    had (default), 2 always.  Attention sums in
                                     another order than per sequence; tests bound the difference */
 #define LLM_OPT_ATTN_CHAIN 7   /* overlap mode: a micro-batch's attention launch starts once every CTA of
                                   the other's has started (1, default) or once it completed (0)  */
