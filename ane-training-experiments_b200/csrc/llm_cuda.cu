@@ -2782,7 +2782,11 @@ extern "C" int llm_memory_bytes(llm_ctx* c, uint64_t* weights, uint64_t* kv_pool
   if (!c) return fail(LLM_ERR_INVALID, "nil context");
   if (weights) *weights = c->bytes_weights;
   if (kv_pool) *kv_pool = c->bytes_kv;
-  if (other) *other = c->bytes_other;
+  if (other) {
+    *other = c->bytes_other;
+    for (const PrefixUse* u : {&c->step_prefix, &c->gen_prefix})
+      if (u->plan) *other += llm_detail_prefix_bytes(u->plan);
+  }
   return LLM_OK;
 }
 

@@ -256,6 +256,7 @@ struct llm_prefix_plan {
   int device = 0, dtype = 0, n_heads = 0, n_kv_heads = 0, head_dim = 0;
   int n_seqs = 0, n_rows = 0, max_ctx = 0, top_slot = -1;
   void* block = nullptr;  // one device allocation: items, row_info, slots, states, sums
+  size_t bytes = 0;       // of it
   const PrefixItem* items[2] = {};  // [tile, columns]
   int n_items[2] = {};
   int variant = 0;  // of the tile kernel: kWide, kNarrow, kSingle
@@ -535,6 +536,8 @@ cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_
   return e == cudaSuccess ? prefix_any<true>(plan, p, r.trace, s, false) : e;
 }
 
+size_t llm_detail_prefix_bytes(const llm_prefix_plan* plan) { return plan->bytes; }
+
 int llm_detail_prefix_launches(const llm_prefix_plan* plan, const char* (*names)[3]) {
   int n = 0;
   auto add = [&](const char* name) {
@@ -683,6 +686,7 @@ int llm_detail_prefix_create(int device, int dtype, int n_heads, int n_kv_heads,
     }
     // A copy from pageable memory may return with its last bytes still on the way, and the first call
     // may come on a stream that is not ordered with the null stream: wait for them here.
+    p->bytes = bytes;
     e = cudaMemcpy(p->block, host.data(), host.size(), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (e == cudaSuccess) e = prefix_any<false>(p, PrefixParams{}, nullptr, nullptr, true);

@@ -29,5 +29,6 @@ struct llm_prefix_rows {
 cudaError_t llm_detail_prefix_run(const llm_prefix_plan* plan, const llm_prefix_rows& r, cudaStream_t s);
 // Kernels of one llm_detail_prefix_run, in their order; names: nullptr, or where to put theirs.
 int llm_detail_prefix_launches(const llm_prefix_plan* plan, const char* (*names)[3] = nullptr);
+size_t llm_detail_prefix_bytes(const llm_prefix_plan* plan);  // device memory that it holds
 // What a status word that kernels set says (DeviceError, PageError).
 const char* llm_detail_device_error(int code);

@@ -1,5 +1,5 @@
 """Device memory and attention over shared prefixes in a context: a batch whose plan finds none runs per
-sequence (the default).  The shortage is made on the host: the child
+sequence (the default), and what a plan holds is counted.  The shortage is made on the host: the child
 process's allocations of more than 256 KiB are refused while a switch is on."""
 import os
 import subprocess
@@ -9,6 +9,7 @@ from pathlib import Path
 import pytest
 
 from ane import _abi
+from test_gpu_fork import CFG, engine
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,19 @@ def test_a_batch_whose_plan_finds_no_memory_runs_per_sequence(tmp_path):
     r = subprocess.run([sys.executable, str(child), str(so), *paths], capture_output=True, text=True, timeout=300,
                        env={**os.environ, "LD_PRELOAD": str(so)})
     assert r.returncode == 0 and "complete" in r.stdout, r.stdout + r.stderr
+
+
+def test_the_memory_of_a_plan_is_counted():
+    eng = engine(CFG, "bf16")
+    eng.set_option(_abi.LLM_OPT_SHARED_PREFIX, 2)
+    eng.prefill([0], [list(range(3, 103))])
+    eng.fork(0, [1, 2, 3, 4], 100)
+    eng.decode_step([5], [4], [0])
+    before = eng.memory()["other"]
+    eng.decode_step(list(range(5)), [4] * 5, [100] * 5)
+    held = eng.memory()["other"] - before
+    # two or more states of 128 f32 sums and two more for each of 5 rows and 4 heads
+    assert held >= 2 * 5 * 4 * (128 + 2) * 4
+    eng.generate(list(range(5)), [4] * 5, [101] * 5, 2)
+    assert eng.memory()["other"] - before >= 2 * held  # a plan of its own
+    eng.close()
